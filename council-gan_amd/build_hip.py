@@ -13,18 +13,23 @@ from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
-UNITS = ("conv_gemm.hip", "conv_x3.hip", "norm.hip", "elementwise.hip", "collective.hip", "head.hip")
+UNITS = ("conv_gemm.hip", "conv_x3.hip", "norm.hip", "elementwise.hip", "collective.hip", "head.hip", "channel_mlp.hip",
+         "gated.hip")
 SRC = [os.path.join(CSRC, f) for f in UNITS if os.path.exists(os.path.join(CSRC, f))]
 # headers / include files every unit may see (a change recompiles everything)
-SHARED = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".h", ".inc"))] + \
+SHARED = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".h", ".inc")) and f != "cg_vec.h"] + \
          [os.path.join(HERE, "..", "include", "council_gan_hip.h")]
-DEPS = SRC + SHARED
+CHANNEL_UNITS = ("channel_mlp.hip", "gated.hip")       # the units that include cg_vec.h
+EXTRA = {u: [os.path.join(CSRC, "cg_vec.h")] for u in CHANNEL_UNITS}
+DEPS = SRC + SHARED + [os.path.join(CSRC, "cg_vec.h")]
 OUT_DIR = os.path.join(HERE, "lib")
 OBJ_DIR = os.path.join(OUT_DIR, "obj")
 OUT = os.path.join(OUT_DIR, "libcouncilgan_hip.so")
 STAMP = OUT + ".stamp"
 CFLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result"] + os.environ.get("CG_HIPCC_FLAGS", "").split()
 FLAGS = CFLAGS + ["-shared"]
+# no packed fp32 arithmetic: some of its forms have given wrong results on this hardware now and then
+UNIT_FLAGS = {u: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for u in CHANNEL_UNITS}
 
 
 def _digest(paths=DEPS):
@@ -32,16 +37,19 @@ def _digest(paths=DEPS):
     for p in paths:
         h.update(open(p, "rb").read())
     h.update(" ".join(FLAGS).encode())
+    for u in UNITS:
+        if os.path.join(CSRC, u) in paths and u in UNIT_FLAGS:
+            h.update(" ".join(UNIT_FLAGS[u]).encode())
     return h.hexdigest()
 
 
 def _compile(hipcc, src, verbose):
-    dig = _digest([src] + SHARED)
+    dig = _digest([src] + EXTRA.get(os.path.basename(src), []) + SHARED)
     obj = os.path.join(OBJ_DIR, os.path.basename(src) + ".o")
     tag = obj + ".stamp"
     if os.path.exists(obj) and os.path.exists(tag) and open(tag).read() == dig:
         return obj
-    cmd = [hipcc] + CFLAGS + ["-c", src, "-o", obj]
+    cmd = [hipcc] + CFLAGS + UNIT_FLAGS.get(os.path.basename(src), []) + ["-c", src, "-o", obj]
     if verbose:
         print("[build_hip]", " ".join(cmd), flush=True)
     subprocess.check_call(cmd)

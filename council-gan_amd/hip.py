@@ -12,6 +12,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("CG_LIB_PATH") or os.path.join(_HERE, "lib", "libcouncilgan_hip.so")      # CG_LIB_PATH: measurement builds (tools/)
 
 ACT = {"none": 0, None: 0, "relu": 1, "lrelu": 2, "tanh": 3}
+DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # CG_DT_*: element types of the channel-MLP operators
+GATE = {"silu": 0, "gelu": 1, "sigmoid": 2}                       # CG_GATE_*
 MAX_TAPS = 64
 X3_LO_ELEMS = 32             # CG_X3_LO_ELEMS
 X3_WSCALE = 1024.0      # CG_X3_WSCALE: power-of-two pre-scale of split-precision weights
@@ -29,6 +31,12 @@ class ConvGeom(ctypes.Structure):
 class Group(ctypes.Structure):
     """cg_group: n council members whose parameters sit `stride` fp32 elements apart in one pool (optim.ParamPool)."""
     _fields_ = [("n", c_int32), ("reserved", c_int32), ("stride", c_int64)]
+
+
+class GatedDims(ctypes.Structure):
+    """cg_gated_dims: sizes, type and gate of one gated_feed_forward call."""
+    _fields_ = [("rows", c_int64), ("D", c_int32), ("F", c_int32), ("O", c_int32), ("dtype", c_int32), ("gate", c_int32),
+                ("reserved", c_int32)]
 
 
 class X3Epilogue(ctypes.Structure):
@@ -147,6 +155,16 @@ _SIGS = {
     "cg_layernorm_workspace": (c_size_t, [c_int, c_int, c_int]),
     "cg_layernorm_fwd": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_float, _P, c_size_t, _P]),
     "cg_layernorm_bwd": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_float, _P, c_size_t, _P]),
+    "cg_channel_norm_fwd": (c_int, [POINTER(Group), _P, _P, _P, _P, _P, _P, c_size_t, c_int, c_int, c_int, c_float, _P]),
+    "cg_channel_norm_bwd_workspace": (c_size_t, [POINTER(Group), c_size_t, c_int]),
+    "cg_channel_norm_bwd": (c_int, [POINTER(Group), _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_size_t, c_int, c_int, c_int, _P,
+                                    c_size_t, _P]),
+    "cg_dropout_key": (c_int, [_P, _P, _P]),
+    "cg_dropout": (c_int, [_P, _P, _P, c_size_t, c_int, _P, c_int, _P]),
+    "cg_gated_ff_fwd_workspace": (c_size_t, [POINTER(GatedDims), POINTER(Group)]),
+    "cg_gated_ff_fwd": (c_int, [POINTER(GatedDims), POINTER(Group)] + [_P] * 12 + [c_size_t, _P]),
+    "cg_gated_ff_bwd_workspace": (c_size_t, [POINTER(GatedDims), POINTER(Group)]),
+    "cg_gated_ff_bwd": (c_int, [POINTER(GatedDims), POINTER(Group)] + [_P] * 15 + [c_int, _P, c_size_t, _P]),
     "cg_avgpool3s2_fwd": (c_int, [_P, _P, c_int, c_int, c_int, c_int, _P]),
     "cg_avgpool3s2_bwd": (c_int, [_P, _P, c_int, c_int, c_int, c_int, _P]),
     "cg_upsample2x_fwd": (c_int, [_P, _P, c_int, c_int, c_int, c_int, _P]),

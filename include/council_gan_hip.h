@@ -432,6 +432,51 @@ int cg_layernorm_bwd(const float* dy, const float* x, const float* gamma, const 
                      float* dx, float* dgamma, float* dbeta, int N, int HW, int C, float eps, void* ws,
                      size_t ws_bytes, cg_stream_t stream);
 
+/* ---- channel-MLP operators: rows of channels in fp32, fp16 or bf16 (the one part of the library that takes 16-bit tensors) -------
+ * Rows are dense (row r starts at r * C elements, at any alignment its type allows); sums, statistics and accumulators are fp32,
+ * every output is rounded once.  `grp`: the rows are grp->n equal blocks, one per council member, and member z's parameters and
+ * their gradients sit z * grp->stride elements after the lead member's. */
+#define CG_DT_F32 0
+#define CG_DT_F16 1
+#define CG_DT_BF16 2
+
+/* y = (x - mean) * rstd * weight + bias over the C channels of every row; biased variance, rstd = 1 / sqrt(var + eps).
+ * weight / bias: `wdtype` = dtype or CG_DT_F32; bias may be NULL.  mean / rstd (both or neither): [rows], for the backward pass. */
+int cg_channel_norm_fwd(const cg_group* grp, const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                        size_t rows, int C, int dtype, int wdtype, float eps, cg_stream_t stream);
+size_t cg_channel_norm_bwd_workspace(const cg_group* grp, size_t rows, int C);
+/* dx, dweight, dbias: any may be NULL; `accumulate` adds to dweight / dbias instead of overwriting them */
+int cg_channel_norm_bwd(const cg_group* grp, const void* dy, const void* x, const void* weight, const float* mean, const float* rstd,
+                        void* dx, void* dweight, void* dbias, int accumulate, size_t rows, int C, int dtype, int wdtype, void* ws,
+                        size_t ws_bytes, cg_stream_t stream);
+
+/* state and key: two int64 {seed, step} on the device; key = state, then state's step + 1 */
+int cg_dropout_key(void* state, void* key, cg_stream_t stream);
+/* y = residual + (draw >= threshold ? x * 65536 / (65536 - threshold) : 0), residual may be NULL.  The draws of elements 8b .. 8b+7 are
+ * the 16-bit halves (low first) of Philox4x32-10 with counter {b, key[1]} and key key[0]; 0 <= threshold < 65536. */
+int cg_dropout(const void* x, const void* residual, void* y, size_t n, int threshold, const void* key, int dtype, cg_stream_t stream);
+
+#define CG_GATE_SILU 0
+#define CG_GATE_GELU 1 /* a * Phi(a), the error-function form */
+#define CG_GATE_SIGMOID 2
+typedef struct cg_gated_dims {
+    int64_t rows;       /* of all members together */
+    int32_t D, F, O;    /* input channels, hidden units, output channels (0: no output projection, h is the result) */
+    int32_t dtype, gate, reserved;
+} cg_gated_dims;
+/* a = x wg^T + bg, v = x wv^T + bv, h = gate(a) * v, y = h wo^T + bo; wg / wv [F][D], wo [O][F]; biases may be NULL.
+ * a, v (both or neither): kept for the backward pass. */
+size_t cg_gated_ff_fwd_workspace(const cg_gated_dims* d, const cg_group* grp);
+int cg_gated_ff_fwd(const cg_gated_dims* d, const cg_group* grp, const void* x, const void* wg, const void* wv, const void* wo,
+                    const void* bg, const void* bv, const void* bo, void* h, void* a, void* v, void* y, void* ws, size_t ws_bytes,
+                    cg_stream_t stream);
+/* dy: gradient of y (of h when O is 0).  Any gradient may be NULL.  Bit i of `accumulate` adds to parameter gradient i of
+ * {dwg, dwv, dwo, dbg, dbv, dbo} instead of overwriting it. */
+size_t cg_gated_ff_bwd_workspace(const cg_gated_dims* d, const cg_group* grp);
+int cg_gated_ff_bwd(const cg_gated_dims* d, const cg_group* grp, const void* dy, const void* x, const void* wg, const void* wv,
+                    const void* wo, const void* h, const void* a, const void* v, void* dx, void* dwg, void* dwv, void* dwo, void* dbg,
+                    void* dbv, void* dbo, int accumulate, void* ws, size_t ws_bytes, cg_stream_t stream);
+
 /* ---- resampling --------------------------------------------------------------------------- */
 /* nn.AvgPool2d(3, stride=2, padding=1, count_include_pad=False), networks.py:32,129 */
 int cg_avgpool3s2_fwd(const float* x, float* y, int N, int H, int W, int C, cg_stream_t stream);
