@@ -1,6 +1,6 @@
 // gated_feed_forward: y = (act(x Wg^T + bg) * (x Wv^T + bv)) Wo^T + bo, forward and backward (gfx950).
 //
-// Every product is C[m, n] = sum_k A(m, k) B(n, k) with operands of any strides.  The gate and the value projection are one product
+// Every product is C[m, n] = sum_k A(m, k) B(n, k).  The gate and the value projection are one product
 // whose output tile holds 32 gate columns next to the 32 value columns of the same hidden units, so that act(a) * v is formed from the
 // accumulators; the backward pass forms da = dh v act'(a) and dv = dh act(a) in the same way from the accumulators of dh = dy Wo, which
 // is never stored.
@@ -12,23 +12,26 @@ namespace {
 inline int grp_n(const cg_group* g) { return g && g->n > 1 ? g->n : 1; }
 inline size_t grp_stride(const cg_group* g) { return g && g->n > 1 ? (size_t)g->stride : 0; }
 
-// element (row, k) of operand z: p[z * zs + row * rs + k * ks]
-template <typename T> struct Mat { const T* p; size_t zs, rs, ks; };
-
 enum { EPI_STORE = 0, EPI_GATE_FWD = 1, EPI_GATE_BWD = 2 };
 
+// C[m, n] = sum_k A(m, k) B(n, k).  Operands are "K-contiguous" (A(m, k) = A[m * ld + k]) or "row-contiguous" (A(m, k) = A[k * ld + m]).
 template <typename T> struct Gemm {
-    Mat<T> A[2], B[2];        // EPI_STORE: nseg pairs, summed; EPI_GATE_FWD: B[0] gate, B[1] value weights
-    int nseg;
+    const T *A[2], *B[2];     // nseg pairs are summed; nsel results share B[0] (sel picks A and C); EPI_GATE_FWD: B = gate, value weights
+    size_t az, bz, lda, ldb;  // member strides, leading dimensions
+    int nseg, nsel;
     size_t M, K;
     int N;                    // EPI_GATE_FWD: hidden units
+    T* c[2];                  // EPI_STORE: C[m * N + n]
+    size_t cz;
+    int accumulate;           // bit sel
+    const T* bias[2];
+    size_t biasz;
     int gate;
-    T* c; size_t cz;          // EPI_STORE: C[m * N + n]
-    int accumulate;
-    const T* bias[2]; size_t bz;
     T *o0, *o1, *o2;          // EPI_GATE_FWD: h, a, v; EPI_GATE_BWD: da, dv
     const T *i0, *i1;         // EPI_GATE_BWD: a, v
     size_t oz;
+    float* part;              // splits > 1: partial sums [split][member * nsel + sel][M][planes][NP]
+    int splits, tiles_m, tiles_n;
 };
 
 __device__ __forceinline__ void gate_fn(float a, int gate, float& u, float& du) {
@@ -43,83 +46,349 @@ __device__ __forceinline__ void gate_fn(float a, int gate, float& u, float& du) 
     }
 }
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-constexpr int TM = 64, TN = 64, TK = 16, LD = 68;
-
-// 64 x 64 tile, four waves of 16 rows, exact fp32 products on v_mfma_f32_16x16x4_f32 for every type
+// ------------------------------------------------------------------------------------------
+// epilogue of 8 consecutive columns: v = the sums (EPI_GATE_FWD: of the gate, w of the value projection)
+// ------------------------------------------------------------------------------------------
 template <typename T, int EPI>
-__global__ __launch_bounds__(256) void gemm_kernel(Gemm<T> g) {
-    __shared__ float As[TK][LD], Bs[TK][LD];
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-    const size_t z = blockIdx.z;
-    const size_t m0 = (size_t)blockIdx.x * TM;
-    const int n0 = blockIdx.y * (EPI == EPI_GATE_FWD ? TN / 2 : TN);
-    f32x4 acc[4] = {};
-    for (int s = 0; s < g.nseg; ++s) {
-        for (size_t k0 = 0; k0 < g.K; k0 += TK) {
-            __syncthreads();
+__device__ __forceinline__ void emit(const Gemm<T>& g, size_t z, int sel, size_t m, int n, float (&v)[8], float (&w)[8]) {
+    const int left = g.N - n;
+    float x[8], y[8];
+    if (EPI == EPI_STORE) {
+        T* c = g.c[sel] + z * g.cz + m * g.N + n;
+        if (g.bias[0]) {
+            cg_load<T, 8>(g.bias[0] + z * g.biasz + n, left, x);
 #pragma unroll
-            for (int q = 0; q < TM * TK / 256; ++q) {
-                const int e = q * 256 + tid;
-                // the faster index of the load follows the unit stride of the operand
-                const Mat<T>& a = g.A[s];
-                const int ar = a.ks == 1 ? e / TK : e % TM, ak = a.ks == 1 ? e % TK : e / TM;
-                As[ak][ar] = m0 + ar < g.M && k0 + ak < g.K ? (float)a.p[z * a.zs + (m0 + ar) * a.rs + (k0 + ak) * a.ks] : 0.f;
-                const int second = EPI == EPI_GATE_FWD ? 1 : s;
-                const int ks1 = g.B[second].ks == 1;
-                const int br = ks1 ? e / TK : e % TN, bk = ks1 ? e % TK : e / TN;
-                const Mat<T>& b = EPI == EPI_GATE_FWD ? g.B[br >> 5] : g.B[s];
-                const int n = EPI == EPI_GATE_FWD ? n0 + (br & 31) : n0 + br;
-                Bs[bk][br] = n < g.N && k0 + bk < g.K ? (float)b.p[z * b.zs + (size_t)n * b.rs + (k0 + bk) * b.ks] : 0.f;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int kk = 0; kk < TK; kk += 4) {
-                const float av = As[kk + (lane >> 4)][wid * 16 + (lane & 15)];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(av, Bs[kk + (lane >> 4)][j * 16 + (lane & 15)], acc[j], 0, 0, 0);
-            }
+            for (int i = 0; i < 8; ++i) v[i] += x[i];
         }
+        if (g.accumulate >> sel & 1) {
+            cg_load<T, 8>(c, left, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += x[i];
+        }
+        cg_store<T, 8>(c, left, v);
+        return;
     }
+    const size_t o = z * g.oz + m * g.N + n;
+    float u, du;
+    if (EPI == EPI_GATE_FWD) {
+        if (g.bias[0]) cg_load<T, 8>(g.bias[0] + z * g.biasz + n, left, x);
+        if (g.bias[1]) cg_load<T, 8>(g.bias[1] + z * g.biasz + n, left, y);
+        float h[8];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const size_t m = m0 + wid * 16 + 4 * (lane >> 4) + r;
-        if (m >= g.M) continue;
-#pragma unroll
-        for (int j = 0; j < (EPI == EPI_GATE_FWD ? 2 : 4); ++j) {
-            const int n = n0 + j * 16 + (lane & 15);
-            if (n >= g.N) continue;
-            const size_t o = m * g.N + n;
-            if (EPI == EPI_STORE) {
-                float v = acc[j][r] + (g.bias[0] ? (float)g.bias[0][z * g.bz + n] : 0.f);
-                T* c = g.c + z * g.cz + o;
-                *c = (T)(g.accumulate ? (float)*c + v : v);
-            } else if (EPI == EPI_GATE_FWD) {
-                const T a = (T)(acc[j][r] + (g.bias[0] ? (float)g.bias[0][z * g.bz + n] : 0.f));
-                const T v = (T)(acc[j + 2][r] + (g.bias[1] ? (float)g.bias[1][z * g.bz + n] : 0.f));
-                float u, du;
-                // act(a) v from the rounded a, v that the backward pass differentiates
-                gate_fn((float)a, g.gate, u, du);
-                g.o0[z * g.oz + o] = (T)(u * (float)v);
-                if (g.o1) {
-                    g.o1[z * g.oz + o] = a;
-                    g.o2[z * g.oz + o] = v;
-                }
-            } else {
-                float u, du;
-                gate_fn((float)g.i0[z * g.oz + o], g.gate, u, du);
-                const float d = acc[j][r];
-                g.o0[z * g.oz + o] = (T)(d * (float)g.i1[z * g.oz + o] * du);
-                g.o1[z * g.oz + o] = (T)(d * u);
-            }
+        for (int i = 0; i < 8; ++i) {
+            // act(a) v is formed from the rounded a, v: the values the backward pass differentiates
+            v[i] = (float)(T)(v[i] + (g.bias[0] ? x[i] : 0.f));
+            w[i] = (float)(T)(w[i] + (g.bias[1] ? y[i] : 0.f));
+            gate_fn(v[i], g.gate, u, du);
+            h[i] = u * w[i];
         }
+        cg_store<T, 8>(g.o0 + o, left, h);
+        if (g.o1) {
+            cg_store<T, 8>(g.o1 + o, left, v);
+            cg_store<T, 8>(g.o2 + o, left, w);
+        }
+    } else {
+        cg_load<T, 8>(g.i0 + o, left, x);
+        cg_load<T, 8>(g.i1 + o, left, y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            gate_fn(x[i], g.gate, u, du);
+            w[i] = v[i] * u;
+            v[i] = v[i] * y[i] * du;
+        }
+        cg_store<T, 8>(g.o0 + o, left, v);
+        cg_store<T, 8>(g.o1 + o, left, w);
     }
 }
 
-template <typename T, int EPI> void gemm(const Gemm<T>& g, int nz, hipStream_t st) {
+template <int EPI> constexpr int planes() { return EPI == EPI_GATE_FWD ? 2 : 1; }
+__host__ __device__ __forceinline__ size_t pad8(int n) { return (size_t)((n + 7) & ~7); }
+
+// ------------------------------------------------------------------------------------------
+// tile kernel on v_mfma_f32_32x32x16 (fp16 / bf16).
+//
+// fp32 operands are split exactly into three bf16 values on their way to LDS, x = h + m + l (round to nearest even, 8 + 8 + 8
+// significant bits), and a product is the six terms hh, hm, mh, hl, mm, lh: what is left out is below 2^-23 of |x y|, half a
+// rounding of an fp32 product.  Six products on the 16-bit matrix pipe take less than half the time of one fp32 product on the fp32 one.
+//
+// LDS: a K-contiguous operand lies as [row][K-step] with its 16-byte chunks xor-swizzled by the row, so the eight rows that one
+// pass of ds_read_b128 touches start at eight different bank groups; a row-contiguous one lies as [k][row] and is transposed by the read
+// (ds_read_b64_tr_b16: inside 16 lanes, lane s names the address of 4 values X[s][0..3] and lane i gets X[4 j + i / 4][i % 4]).
+// ------------------------------------------------------------------------------------------
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((__vector_size__(4 * sizeof(short))));
+
+template <typename T> struct Mx { typedef T E; static constexpr int P = 1, BK = 64; };
+template <> struct Mx<float> { typedef cg_b16 E; static constexpr int P = 3, BK = 32; };
+
+template <typename E> struct V8 { typedef E V __attribute__((ext_vector_type(8))); };
+__device__ __forceinline__ f32x16 mfma(typename V8<cg_h16>::V a, typename V8<cg_h16>::V b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(typename V8<cg_b16>::V a, typename V8<cg_b16>::V b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// One operand of a tile: global -> registers -> LDS, and the fragments of one 16-deep step
+template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
+    typedef typename Mx<T>::E E;
+    typedef typename V8<E>::V Frag;
+    typedef typename CgT<T>::V Raw;
+    static constexpr int P = Mx<T>::P, BK = Mx<T>::BK, W = CgT<T>::N;
+    static constexpr int CPR = KC ? BK / W : ROWS / W;             // chunks of W elements per LDS row
+    static constexpr int CH = (KC ? ROWS : BK) * CPR / NT;
+    static constexpr int PITCH = KC ? BK * 2 : ROWS * 2 + 64;      // bytes
+    static constexpr int PLANE = (KC ? ROWS : BK) * PITCH;
+    static constexpr int BYTES = P * PLANE;
+    static_assert(CH >= 1 && ((KC ? ROWS : BK) * CPR) % NT == 0, "every thread has the same number of chunks");
+
+    size_t off[CH];
+    Raw raw[CH];
+    int tid;
+
+    static __device__ __forceinline__ int lrow(int tid, int i) { return (tid + i * NT) / CPR; }
+    static __device__ __forceinline__ int lch(int tid) { return tid % CPR; }
+    static_assert(NT % CPR == 0, "a thread keeps its chunk column");
+
+    // rows past the end are read from a row that exists: what they give is never stored
+    __device__ __forceinline__ void init(int t, size_t row0, size_t rows, size_t ld) {
+        tid = t;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            if (KC) {
+                int j = lrow(tid, i);
+                if (GATE) j = (j >> 6) * 32 + (j & 31);
+                const size_t r = row0 + j;
+                off[i] = (r < rows ? r : rows - 1) * ld + lch(tid) * W;
+            } else {
+                const size_t r = row0 + lch(tid) * W;
+                off[i] = lrow(tid, i) * ld + (r < rows ? r : 0);
+            }
+        }
+    }
+    // `last`: the operand's last K-step -- everything past K reads as zero, nothing past the tensor is touched.  Elsewhere a chunk may
+    // run over the end of a row into the next one (a row-contiguous operand of at least W rows has it): rows that are never stored.
+    __device__ __forceinline__ void load(const T* p0, const T* p1, size_t k0, size_t K, size_t ld, size_t row0, size_t rows, bool last) {
+        const size_t step = KC ? k0 : k0 * ld;
+        if ((last && (K % BK != 0 || (!KC && rows % W != 0))) || (!KC && rows < W)) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const T* p = (GATE && (lrow(tid, i) >> 5 & 1) ? p1 : p0) + step + off[i];
+                const size_t k = k0 + (KC ? lch(tid) * W : lrow(tid, i));
+                const size_t r = row0 + lch(tid) * W;
+#pragma unroll
+                for (int e = 0; e < W; ++e) raw[i][e] = (KC ? k + e < K : k < K && r + e < rows) ? p[e] : (T)0.f;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) raw[i] = *(const Raw*)((GATE && (lrow(tid, i) >> 5 & 1) ? p1 : p0) + step + off[i]);
+        }
+    }
+    static __device__ __forceinline__ unsigned swz(int row, int chunk) {       // 16-byte chunk of a K-contiguous row
+        return BK == 64 ? (unsigned)(chunk ^ (row & 7)) : (unsigned)(chunk ^ ((row >> 1) & 3));
+    }
+    __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int r = lrow(tid, i), c = lch(tid);
+            if constexpr (P == 1) {
+                *(Frag*)(lds + r * PITCH + (KC ? swz(r, c) : (unsigned)c) * 16) = __builtin_bit_cast(Frag, raw[i]);
+            } else {
+                typedef E E4 __attribute__((ext_vector_type(4)));
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = raw[i][e];
+                char* d = lds + r * PITCH + (KC ? swz(r, c >> 1) * 16 + (c & 1) * 8 : (unsigned)c * 8);
+#pragma unroll
+                for (int p = 0; p < 3; ++p) {
+                    E4 h;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        h[e] = (E)x[e];
+                        x[e] -= (float)h[e];
+                    }
+                    *(E4*)(d + p * PLANE) = h;
+                }
+            }
+        }
+    }
+    // rows r0 .. r0 + 31, K-step ks: lane l holds row r0 + l % 32, k = 16 ks + 8 (l / 32) .. + 7
+    static __device__ __forceinline__ Frag frag(const char* lds, int lane, int r0, int ks, int p) {
+        if constexpr (KC) {
+            const int r = r0 + (lane & 31);
+            return *(const Frag*)(lds + p * PLANE + r * PITCH + swz(r, 2 * ks + (lane >> 5)) * 16);
+        } else {
+            typedef __attribute__((address_space(3))) s16x4* Q;
+            const int sl = lane & 15;
+            const int at = p * PLANE + (ks * 16 + (lane >> 5) * 8 + (sl >> 2)) * PITCH + (r0 + 16 * ((lane >> 4) & 1) + 4 * (sl & 3)) * 2;
+            const Q q = (Q)((const __attribute__((address_space(3))) char*)lds + at);
+            struct { s16x4 a, b; } f;
+            f.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(q);
+            f.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(q + 4 * PITCH / 8);
+            return __builtin_bit_cast(Frag, f);
+        }
+    }
+};
+
+template <typename T, int BM, int BN, int WM, int WN, bool KA, bool KB, int EPI>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void gemm_kernel(Gemm<T> g) {
+    constexpr int NW = (BM / WM) * (BN / WN), NT = NW * 64, TM = WM / 32, TN = WN / 32;
+    typedef Operand<T, BM, NT, KA, false> OA;
+    typedef Operand<T, BN, NT, KB, EPI == EPI_GATE_FWD> OB;
+    constexpr int P = OA::P, BK = OA::BK, EP = WN + 4;
+    constexpr int SMEM = OA::BYTES + OB::BYTES > NW * 32 * EP * 4 ? OA::BYTES + OB::BYTES : NW * 32 * EP * 4;
+    static_assert(WN == 64, "a wave's 64 columns are 32 gate and 32 value columns");
+    __shared__ __attribute__((aligned(16))) char smem[SMEM];
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+
+    // blocks go to the 8 XCDs in turn: each XCD takes a run of neighbouring tiles, in panels of 8 tile rows, so that what its L2 holds is
+    // read again
+    const unsigned nt = gridDim.x, xcd = blockIdx.x & 7, q = nt / 8, rem = nt % 8;
+    const unsigned t = xcd * q + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
+    const unsigned panel = 8 * g.tiles_n, pm = t / panel * 8, pr = t % panel, ph = g.tiles_m - pm < 8 ? g.tiles_m - pm : 8;
+    const size_t m0 = (size_t)(pm + pr % ph) * BM;
+    const int n0 = (int)(pr / ph) * (EPI == EPI_GATE_FWD ? BN / 2 : BN);
+    const int split = blockIdx.z % g.splits, zs = blockIdx.z / g.splits, sel = zs % g.nsel;
+    const size_t z = zs / g.nsel;
+
+    f32x16 acc[TM][TN] = {};
+    const int wm = wid / (BN / WN) * WM, wn = wid % (BN / WN) * WN;
+    const int kt = (int)((g.K + BK - 1) / BK), all = kt * g.nseg;
+    const int k_begin = (int)((long long)all * split / g.splits), k_end = (int)((long long)all * (split + 1) / g.splits);
+    OA a;
+    OB b;
+    a.init(tid, m0, g.M, g.lda);
+    b.init(tid, n0, g.N, g.ldb);
+    auto load = [&](int step) {
+        const int s = step >= kt ? 1 : 0, k = step - s * kt;
+        a.load(g.A[g.nseg == 2 ? s : sel] + z * g.az, nullptr, (size_t)k * BK, g.K, g.lda, m0, g.M, k == kt - 1);
+        b.load(g.B[g.nseg == 2 ? s : 0] + z * g.bz, EPI == EPI_GATE_FWD ? g.B[1] + z * g.bz : nullptr, (size_t)k * BK, g.K, g.ldb, n0,
+               g.N, k == kt - 1);
+    };
+    if (k_begin < k_end) load(k_begin);
+    for (int step = k_begin; step < k_end; ++step) {
+        __syncthreads();
+        a.store(smem);
+        b.store(smem + OA::BYTES);
+        __syncthreads();
+        if (step + 1 < k_end) load(step + 1);
+#pragma unroll
+        for (int ks = 0; ks < BK / 16; ++ks) {
+            typename OA::Frag fa[TM][P], fb[TN][P];
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i) fa[i][p] = OA::frag(smem, lane, wm + i * 32, ks, p);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) fb[j][p] = OB::frag(smem + OA::BYTES, lane, wn + j * 32, ks, p);
+            }
+            // the smaller terms first
+#pragma unroll
+            for (int d = P - 1; d >= 0; --d)
+#pragma unroll
+                for (int p = 0; p <= d; ++p)
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) acc[i][j] = mfma(fa[i][p], fb[j][d - p], acc[i][j]);
+        }
+    }
+
+    // the accumulators go through LDS (32 rows of a wave at a time) so that every lane stores 8 consecutive columns
+    __syncthreads();
+    float* ep = (float*)smem + wid * 32 * EP;
+    constexpr int LPR = EPI == EPI_GATE_FWD ? 4 : 8, RPP = 64 / LPR;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ep[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * EP + j * 32 + (lane & 31)] = acc[i][j][r];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int pass = 0; pass < 32 / RPP; ++pass) {
+            const int row = pass * RPP + lane / LPR, col = lane % LPR * 8;
+            const size_t m = m0 + wm + i * 32 + row;
+            const int n = n0 + (EPI == EPI_GATE_FWD ? wn / 2 : wn) + col;
+            float v[8], w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = ep[row * EP + col + e];
+                if (EPI == EPI_GATE_FWD) w[e] = ep[row * EP + 32 + col + e];
+            }
+            if (m < g.M && n < g.N) {
+                if (g.splits == 1) {
+                    emit<T, EPI>(g, z, sel, m, n, v, w);
+                } else {
+                    const size_t np = pad8(g.N);
+                    float* p = g.part + (((size_t)split * (gridDim.z / g.splits) + zs) * g.M + m) * planes<EPI>() * np + n;
+                    cg_store<float, 8>(p, 8, v);
+                    if (EPI == EPI_GATE_FWD) cg_store<float, 8>(p + np, 8, w);
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// joins the partial sums of a split product, in the order of the splits
+template <typename T, int EPI> __global__ __launch_bounds__(256) void join_kernel(Gemm<T> g, int nz) {
+    const size_t np = pad8(g.N), per = g.M * (np / 8), total = per * nz, plane = (size_t)nz * g.M * planes<EPI>() * np;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
+        const int zs = (int)(i / per), n = (int)(i % (np / 8)) * 8;
+        const size_t m = i % per / (np / 8);
+        const float* p = g.part + ((size_t)zs * g.M + m) * planes<EPI>() * np + n;
+        float v[8] = {}, w[8] = {}, x[8];
+        for (int s = 0; s < g.splits; ++s, p += plane) {
+            cg_load<float, 8>(p, 8, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += x[e];
+            if (EPI == EPI_GATE_FWD) {
+                cg_load<float, 8>(p + np, 8, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] += x[e];
+            }
+        }
+        emit<T, EPI>(g, zs / g.nsel, zs % g.nsel, m, n, v, w);
+    }
+}
+
+// Tile and number of K splits.  128 x 128 tiles (4 waves of 64 x 64) wherever they can fill the chip, split or not; 64 x 64 (2 waves)
+// below.  A split takes at least 4 K-steps; splits are added until there are two blocks for every CU.  The number of members is left out:
+// a member's results do not depend on how many run beside it.
+struct Plan { int big, splits; };
+Plan plan(size_t M, size_t N, size_t K, int nsel, int esz) {
+    const size_t bk = esz == 4 ? 32 : 64, steps = (K + bk - 1) / bk, most = steps / 4 > 1 ? steps / 4 : 1;
+    const size_t t128 = (size_t)cg_div_up(M, 128) * cg_div_up(N, 128) * nsel, t64 = (size_t)cg_div_up(M, 64) * cg_div_up(N, 64) * nsel;
+    Plan p = {0, 1};
+    if (!t128) return p;        // no rows
+    p.big = t128 * most >= 192;
+    const size_t t = p.big ? t128 : t64, want = (512 + t - 1) / t;
+    p.splits = t >= 256 ? 1 : (int)(want < most ? want : most);
+    return p;
+}
+size_t part_bytes(size_t M, size_t N, size_t K, int members, int nsel, int esz, int np) {      // N: columns of the product
+    const Plan p = plan(M, N, K, nsel, esz);
+    return p.splits > 1 ? (size_t)p.splits * members * nsel * M * np * pad8((int)(N / np)) * 4 : 0;
+}
+
+template <typename T, bool KA, bool KB, int EPI> void gemm(Gemm<T>& g, int members, float* part, hipStream_t st) {
     if (!g.M || !g.N) return;
-    gemm_kernel<T, EPI><<<dim3(cg_div_up(g.M, TM), cg_div_up(g.N, EPI == EPI_GATE_FWD ? TN / 2 : TN), nz), 256, 0, st>>>(g);
+    const int nz = members * g.nsel;
+    const size_t N = (size_t)g.N * planes<EPI>();
+    const Plan p = plan(g.M, N, g.K * g.nseg, g.nsel, sizeof(T));
+    g.part = part, g.splits = p.splits;
+    const int bt = p.big ? 128 : 64;
+    g.tiles_m = cg_div_up(g.M, bt), g.tiles_n = cg_div_up(N, bt);
+    const dim3 grid((unsigned)g.tiles_m * g.tiles_n, 1, nz * p.splits);
+    if (p.big) gemm_kernel<T, 128, 128, 64, 64, KA, KB, EPI><<<grid, 256, 0, st>>>(g);
+    else gemm_kernel<T, 64, 64, 32, 64, KA, KB, EPI><<<grid, 128, 0, st>>>(g);
+    if (p.splits > 1) {
+        const size_t nb = (g.M * (pad8(g.N) / 8) * nz + 255) / 256;
+        join_kernel<T, EPI><<<(unsigned)(nb < 4096 ? nb : 4096), 256, 0, st>>>(g, nz);
+    }
 }
 
 // da, dv from a stored gradient of h (no output projection)
@@ -135,23 +404,46 @@ __global__ __launch_bounds__(256) void gate_bwd_kernel(const T* __restrict__ dh,
     }
 }
 
-// out[z * zs + c] (+)= sum over the member's rows of p[r * C + c]
-template <typename T>
-__global__ __launch_bounds__(256) void colsum_kernel(const T* __restrict__ p, T* __restrict__ out, size_t rows, int C, size_t zs,
-                                                     int accumulate) {
-    __shared__ float sm[4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-    const size_t z = blockIdx.y;
-    float s = 0.f;
-    if (c < C)
-        for (size_t r = w; r < rows; r += 4) s += (float)p[(z * rows + r) * C + c];
-    sm[w][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (w == 0 && c < C) {
-        s = sm[0][threadIdx.x] + sm[1][threadIdx.x] + sm[2][threadIdx.x] + sm[3][threadIdx.x];
-        T* o = out + z * zs + c;
-        *o = (T)(accumulate ? (float)*o + s : s);
+// Column sums of one or two [rows][C] tensors (bias gradients): strips of rows, then the strips in turn.
+constexpr int STRIP_ROWS = 128, MAX_STRIPS = 256;
+inline int strips_of(size_t rows) {
+    const size_t s = (rows + STRIP_ROWS - 1) / STRIP_ROWS;
+    return (int)(s < 1 ? 1 : s > MAX_STRIPS ? MAX_STRIPS : s);
+}
+template <typename T> struct ColSum { const T* p[2]; T* out[2]; size_t rows, zs; int C, strips, accumulate; float* part; };
+
+template <typename T> __global__ __launch_bounds__(256) void colsum_part_kernel(ColSum<T> g) {
+    constexpr int N = CgT<T>::N;
+    __shared__ float sm[3][64 * N];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = (blockIdx.x * 64 + lane) * N;
+    const size_t z = blockIdx.z >> 1, per = (g.rows + g.strips - 1) / g.strips, r0 = blockIdx.y * per;
+    const size_t r1 = r0 + per < g.rows ? r0 + per : g.rows;
+    const T* p = g.p[blockIdx.z & 1];
+    float s[N] = {}, v[N];
+    if (p && c < g.C)
+        for (size_t r = r0 + w; r < r1; r += 4) {
+            cg_load<T>(p + (z * g.rows + r) * g.C + c, g.C - c, v);
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[i] += v[i];
+        }
+    if (w) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) sm[w - 1][i * 64 + lane] = s[i];
     }
+    __syncthreads();
+    if (!w && p && c < g.C) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] += sm[0][i * 64 + lane] + sm[1][i * 64 + lane] + sm[2][i * 64 + lane];
+        cg_store<float, N>(g.part + ((size_t)blockIdx.z * g.strips + blockIdx.y) * g.C + c, g.C - c, s);
+    }
+}
+template <typename T> __global__ __launch_bounds__(256) void colsum_join_kernel(ColSum<T> g) {
+    const int c = blockIdx.x * 256 + threadIdx.x, sel = blockIdx.z & 1;
+    if (c >= g.C || !g.out[sel]) return;
+    float s = 0.f;
+    for (int i = 0; i < g.strips; ++i) s += g.part[((size_t)blockIdx.z * g.strips + i) * g.C + c];
+    T* o = g.out[sel] + (blockIdx.z >> 1) * g.zs + c;
+    *o = (T)(g.accumulate >> sel & 1 ? (float)*o + s : s);
 }
 
 bool dims_ok(const cg_gated_dims* d, const cg_group* grp) {
@@ -163,48 +455,63 @@ bool dims_ok(const cg_gated_dims* d, const cg_group* grp) {
 inline size_t esize(int dt) { return dt == CG_DT_F32 ? 4 : 2; }
 inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// scratch of the forward and the backward pass: both use it for one product or sum after the other
+size_t fwd_part(const cg_gated_dims* d, const cg_group* grp) {
+    const int nz = grp_n(grp), e = (int)esize(d->dtype);
+    const size_t M = d->rows / nz, p = part_bytes(M, 2 * (size_t)d->F, d->D, nz, 1, e, 2);
+    const size_t q = d->O ? part_bytes(M, d->O, d->F, nz, 1, e, 1) : 0;
+    return p > q ? p : q;
+}
+size_t bwd_part(const cg_gated_dims* d, const cg_group* grp) {
+    const int nz = grp_n(grp), e = (int)esize(d->dtype);
+    const size_t M = d->rows / nz, F = d->F, D = d->D, O = d->O;
+    const size_t n[] = {O ? part_bytes(M, F, O, nz, 1, e, 1) : 0, part_bytes(M, D, 2 * F, nz, 1, e, 1), part_bytes(F, D, M, nz, 1, e, 1),
+                        part_bytes(F, D, M, nz, 2, e, 1), O ? part_bytes(O, F, M, nz, 1, e, 1) : 0,
+                        (size_t)2 * nz * strips_of(M) * (F > O ? F : O) * 4};
+    size_t most = 0;
+    for (size_t v : n) most = v > most ? v : most;
+    return up256(most);
+}
+
 template <typename T>
 void fwd(const cg_gated_dims* d, const cg_group* grp, const T* x, const T* wg, const T* wv, const T* wo, const T* bg, const T* bv,
-         const T* bo, T* h, T* a, T* v, T* y, hipStream_t st) {
+         const T* bo, T* h, T* a, T* v, T* y, float* part, hipStream_t st) {
     const int nz = grp_n(grp);
-    const size_t M = d->rows / nz, gs = grp_stride(grp);
-    const size_t D = d->D, F = d->F;
+    const size_t M = d->rows / nz, gs = grp_stride(grp), D = d->D, F = d->F;
     Gemm<T> g = {};
-    g.nseg = 1;
-    g.A[0] = {x, M * D, D, 1};
-    g.B[0] = {wg, gs, D, 1};
-    g.B[1] = {wv, gs, D, 1};
+    g.nseg = g.nsel = 1;
+    g.A[0] = x, g.az = M * D, g.lda = D;
+    g.B[0] = wg, g.B[1] = wv, g.bz = gs, g.ldb = D;
     g.M = M, g.K = D, g.N = d->F, g.gate = d->gate;
-    g.bias[0] = bg, g.bias[1] = bv, g.bz = gs;
+    g.bias[0] = bg, g.bias[1] = bv, g.biasz = gs;
     g.o0 = h, g.o1 = a, g.o2 = v, g.oz = M * F;
-    gemm<T, EPI_GATE_FWD>(g, nz, st);
-    if (d->O) {
-        Gemm<T> p = {};
-        p.nseg = 1;
-        p.A[0] = {h, M * F, F, 1};
-        p.B[0] = {wo, gs, F, 1};
-        p.M = M, p.K = F, p.N = d->O;
-        p.bias[0] = bo, p.bz = gs;
-        p.c = y, p.cz = M * d->O;
-        gemm<T, EPI_STORE>(p, nz, st);
-    }
+    gemm<T, true, true, EPI_GATE_FWD>(g, nz, part, st);
+    if (!d->O) return;
+    Gemm<T> p = {};
+    p.nseg = p.nsel = 1;
+    p.A[0] = h, p.az = M * F, p.lda = F;
+    p.B[0] = wo, p.bz = gs, p.ldb = F;
+    p.M = M, p.K = F, p.N = d->O;
+    p.bias[0] = bo, p.biasz = gs;
+    p.c[0] = y, p.cz = M * d->O;
+    gemm<T, true, true, EPI_STORE>(p, nz, part, st);
 }
 
 template <typename T>
 void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, const T* wg, const T* wv, const T* wo, const T* h,
-         const T* a, const T* v, T* dx, T* dwg, T* dwv, T* dwo, T* dbg, T* dbv, T* dbo, int acc, T* da, T* dv, hipStream_t st) {
+         const T* a, const T* v, T* dx, T* dwg, T* dwv, T* dwo, T* dbg, T* dbv, T* dbo, int acc, T* da, T* dv, float* part,
+         hipStream_t st) {
     const int nz = grp_n(grp);
-    const size_t M = d->rows / nz, gs = grp_stride(grp);
-    const size_t D = d->D, F = d->F, O = d->O;
+    const size_t M = d->rows / nz, gs = grp_stride(grp), D = d->D, F = d->F, O = d->O;
     if (dx || dwg || dwv || dbg || dbv) {
         if (O) {
             Gemm<T> g = {};
-            g.nseg = 1;
-            g.A[0] = {dy, M * O, O, 1};
-            g.B[0] = {wo, gs, 1, F};
+            g.nseg = g.nsel = 1;
+            g.A[0] = dy, g.az = M * O, g.lda = O;
+            g.B[0] = wo, g.bz = gs, g.ldb = F;
             g.M = M, g.K = O, g.N = d->F, g.gate = d->gate;
             g.o0 = da, g.o1 = dv, g.i0 = a, g.i1 = v, g.oz = M * F;
-            gemm<T, EPI_GATE_BWD>(g, nz, st);
+            gemm<T, true, false, EPI_GATE_BWD>(g, nz, part, st);
         } else if (M) {
             const size_t n = (size_t)d->rows * F, nb = (n + 255) / 256;
             gate_bwd_kernel<T><<<(unsigned)(nb < 16384 ? nb : 16384), 256, 0, st>>>(dy, a, v, da, dv, n, d->gate);
@@ -212,72 +519,73 @@ void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, c
     }
     if (dx) {
         Gemm<T> g = {};
-        g.nseg = 2;
-        g.A[0] = {da, M * F, F, 1}, g.A[1] = {dv, M * F, F, 1};
-        g.B[0] = {wg, gs, 1, D}, g.B[1] = {wv, gs, 1, D};
+        g.nseg = 2, g.nsel = 1;
+        g.A[0] = da, g.A[1] = dv, g.az = M * F, g.lda = F;
+        g.B[0] = wg, g.B[1] = wv, g.bz = gs, g.ldb = D;
         g.M = M, g.K = F, g.N = d->D;
-        g.c = dx, g.cz = M * D;
-        gemm<T, EPI_STORE>(g, nz, st);
+        g.c[0] = dx, g.cz = M * D;
+        gemm<T, true, false, EPI_STORE>(g, nz, part, st);
     }
-    auto wgrad = [&](const T* p, size_t P, const T* q, size_t Q, T* dw, int bit) {
-        if (!dw) return;
+    auto wgrad = [&](const T* p0, const T* p1, size_t P, const T* q, size_t Q, T* dw0, T* dw1, int accumulate) {
+        if (!dw0 && !dw1) return;
         Gemm<T> g = {};
-        g.nseg = 1;
-        g.A[0] = {p, M * P, 1, P};
-        g.B[0] = {q, M * Q, 1, Q};
+        g.nseg = 1, g.nsel = dw0 && dw1 ? 2 : 1;
+        g.A[0] = dw0 ? p0 : p1, g.A[1] = p1, g.az = M * P, g.lda = P;
+        g.B[0] = q, g.bz = M * Q, g.ldb = Q;
         g.M = P, g.K = M, g.N = (int)Q;
-        g.c = dw, g.cz = gs, g.accumulate = acc >> bit & 1;
-        gemm<T, EPI_STORE>(g, nz, st);
+        g.c[0] = dw0 ? dw0 : dw1, g.c[1] = dw1, g.cz = gs, g.accumulate = dw0 ? accumulate : accumulate >> 1;
+        gemm<T, false, false, EPI_STORE>(g, nz, part, st);
     };
-    wgrad(da, F, x, D, dwg, 0);
-    wgrad(dv, F, x, D, dwv, 1);
-    if (O) wgrad(dy, O, h, F, dwo, 2);
-    auto bgrad = [&](const T* p, int C, T* db, int bit) {
-        if (db) colsum_kernel<T><<<dim3(cg_div_up(C, 64), nz), 256, 0, st>>>(p, db, M, C, gs, acc >> bit & 1);
+    wgrad(da, dv, F, x, D, dwg, dwv, acc & 3);
+    if (O) wgrad(dy, nullptr, O, h, F, dwo, nullptr, acc >> 2 & 1);
+    auto bgrad = [&](const T* p0, const T* p1, int C, T* db0, T* db1, int accumulate) {
+        if (!db0 && !db1) return;
+        ColSum<T> g = {{db0 ? p0 : nullptr, db1 ? p1 : nullptr}, {db0, db1}, M, gs, C, strips_of(M), accumulate, part};
+        colsum_part_kernel<T><<<dim3(cg_div_up(C, 64 * CgT<T>::N), g.strips, 2 * nz), 256, 0, st>>>(g);
+        colsum_join_kernel<T><<<dim3(cg_div_up(C, 256), 1, 2 * nz), 256, 0, st>>>(g);
     };
-    bgrad(da, d->F, dbg, 3);
-    bgrad(dv, d->F, dbv, 4);
-    if (O) bgrad(dy, d->O, dbo, 5);
+    bgrad(da, dv, d->F, dbg, dbv, acc >> 3 & 3);
+    if (O) bgrad(dy, nullptr, d->O, dbo, nullptr, acc >> 5 & 1);
 }
 
 }  // namespace
 
-extern "C" size_t cg_gated_ff_fwd_workspace(const cg_gated_dims* d, const cg_group* grp) {
-    (void)d, (void)grp;
-    return 0;
-}
+extern "C" size_t cg_gated_ff_fwd_workspace(const cg_gated_dims* d, const cg_group* grp) { return dims_ok(d, grp) ? fwd_part(d, grp) : 0; }
 
 extern "C" int cg_gated_ff_fwd(const cg_gated_dims* d, const cg_group* grp, const void* x, const void* wg, const void* wv, const void* wo,
                                const void* bg, const void* bv, const void* bo, void* h, void* a, void* v, void* y, void* ws,
                                size_t ws_bytes, cg_stream_t stream) {
-    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && !a == !v && (!d->O || wo) && (!d->rows || (x && h && (!d->O || y))), "cg_gated_ff_fwd: bad args");
-    if (ws_bytes < cg_gated_ff_fwd_workspace(d, grp) || (!ws && cg_gated_ff_fwd_workspace(d, grp)))
-        return cg_set_error(CG_ERR_WORKSPACE, "cg_gated_ff_fwd: workspace too small");
+    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && !a == !v && (!d->O || wo) && (!d->rows || (x && h && (!d->O || y))),
+                 "cg_gated_ff_fwd: bad args");
+    const size_t need = fwd_part(d, grp);
+    if (ws_bytes < need || (!ws && need)) return cg_set_error(CG_ERR_WORKSPACE, "cg_gated_ff_fwd: workspace too small");
     if (!d->rows) return CG_OK;
     CG_DISPATCH_DT(d->dtype, T, (fwd<T>(d, grp, (const T*)x, (const T*)wg, (const T*)wv, (const T*)wo, (const T*)bg, (const T*)bv,
-                                        (const T*)bo, (T*)h, (T*)a, (T*)v, (T*)y, cg_s(stream))));
+                                        (const T*)bo, (T*)h, (T*)a, (T*)v, (T*)y, (float*)ws, cg_s(stream))));
     CG_LAUNCH_CHECK("cg_gated_ff_fwd");
     return CG_OK;
 }
 
+static size_t bwd_hidden(const cg_gated_dims* d) { return up256((size_t)d->rows * d->F * esize(d->dtype)); }
+
 extern "C" size_t cg_gated_ff_bwd_workspace(const cg_gated_dims* d, const cg_group* grp) {
-    (void)grp;
-    return dims_ok(d, nullptr) ? 2 * up256((size_t)d->rows * d->F * esize(d->dtype)) : 0;
+    return dims_ok(d, grp) ? 2 * bwd_hidden(d) + bwd_part(d, grp) : 0;
 }
 
 extern "C" int cg_gated_ff_bwd(const cg_gated_dims* d, const cg_group* grp, const void* dy, const void* x, const void* wg,
                                const void* wv, const void* wo, const void* h, const void* a, const void* v, void* dx, void* dwg,
                                void* dwv, void* dwo, void* dbg, void* dbv, void* dbo, int accumulate, void* ws, size_t ws_bytes,
                                cg_stream_t stream) {
-    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && (!d->O || wo) &&
-                     (!d->rows || (dy && x && a && v && (!d->O || h))), "cg_gated_ff_bwd: bad args");
+    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && (!d->O || wo) && (!d->rows || (dy && x && a && v && (!d->O || h))),
+                 "cg_gated_ff_bwd: bad args");
     const size_t need = cg_gated_ff_bwd_workspace(d, grp);
     if (ws_bytes < need || (!ws && need)) return cg_set_error(CG_ERR_WORKSPACE, "cg_gated_ff_bwd: workspace too small");
     CG_DISPATCH_DT(d->dtype, T, {
         T* da = (T*)ws;
-        T* dv = (T*)((char*)ws + need / 2);
+        T* dv = (T*)((char*)ws + bwd_hidden(d));
+        float* part = (float*)((char*)ws + 2 * bwd_hidden(d));
         bwd<T>(d, grp, (const T*)dy, (const T*)x, (const T*)wg, (const T*)wv, (const T*)wo, (const T*)h, (const T*)a, (const T*)v, (T*)dx,
-               (T*)dwg, (T*)dwv, (T*)dwo, (T*)dbg, (T*)dbv, (T*)dbo, accumulate, da, dv, cg_s(stream));
+               (T*)dwg, (T*)dwv, (T*)dwo, (T*)dbg, (T*)dbv, (T*)dbo, accumulate, da, dv, part, cg_s(stream));
     });
     CG_LAUNCH_CHECK("cg_gated_ff_bwd");
     return CG_OK;

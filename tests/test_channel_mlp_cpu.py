@@ -83,6 +83,20 @@ def test_library_refuses_bad_arguments_before_any_launch():
     assert b"workspace" in lib.cg_last_error()
 
 
+def test_workspaces_of_any_size_are_finite():
+    lib = hip.load()
+    for rows in (0, 1, 7, 4096, 10 ** 7):
+        for dt in (0, 1, 2):
+            for n in (1, 3) if dt == 0 else (1,):
+                if rows % n:
+                    continue
+                d, grp = ctypes.byref(hip.GatedDims(rows, 264, 520, 72, dt, 0, 0)), ctypes.byref(hip.Group(n, 0, 1 << 20))
+                assert lib.cg_gated_ff_fwd_workspace(d, grp) < 1 << 33
+                hidden = rows * 520 * (4 if dt == 0 else 2)
+                assert 2 * hidden <= lib.cg_gated_ff_bwd_workspace(d, grp) < 2 * hidden + (1 << 33)
+        assert lib.cg_channel_norm_bwd_workspace(None, rows, 264) < 1 << 33
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
 def test_reference_of_the_gated_block_against_autograd(act):
     g = torch.Generator().manual_seed(1)
