@@ -230,6 +230,58 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
     }
 };
 
+// Blocks go to the 8 XCDs in turn: each XCD takes a run of neighbouring tiles, in panels of 8 tile rows, so that what its L2 holds is
+// read again.
+template <int BM, int BN> __device__ __forceinline__ void tile_origin(int tiles_m, int tiles_n, size_t& m0, int& n0) {
+    const unsigned nt = gridDim.x, xcd = blockIdx.x & 7, q = nt / 8, rem = nt % 8;
+    const unsigned t = xcd * q + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
+    const unsigned panel = 8 * tiles_n, pm = t / panel * 8, pr = t % panel, ph = tiles_m - pm < 8 ? tiles_m - pm : 8;
+    m0 = (size_t)(pm + pr % ph) * BM;
+    n0 = (int)(pr / ph) * BN;
+}
+
+// A wave's accumulators (TM x TN blocks of 32 x 32; TN = 2) go through its own 32 x 68 floats of LDS, 32 rows at a time, so that every
+// lane stores 8 consecutive columns.  EPI_GATE_FWD: the left 32 columns are the gate, the right ones the value projection.
+template <typename T, int EPI, int TM, int TN>
+__device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)[TM][TN], float* ep, int lane, size_t mw, int nw,
+                                           size_t z, int sel, int split, int zs) {
+    constexpr int EP = TN * 32 + 4, LPR = EPI == EPI_GATE_FWD ? 4 : 8, RPP = 64 / LPR;
+    static_assert(TN == 2, "a wave's 64 columns are 32 gate and 32 value columns");
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ep[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * EP + j * 32 + (lane & 31)] = acc[i][j][r];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int pass = 0; pass < 32 / RPP; ++pass) {
+            const int row = pass * RPP + lane / LPR, col = lane % LPR * 8;
+            const size_t m = mw + i * 32 + row;
+            const int n = nw + col;
+            float v[8], w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = ep[row * EP + col + e];
+                if (EPI == EPI_GATE_FWD) w[e] = ep[row * EP + 32 + col + e];
+            }
+            if (m < g.M && n < g.N) {
+                if (g.splits == 1) {
+                    emit<T, EPI>(g, z, sel, m, n, v, w);
+                } else {
+                    const size_t np = pad8(g.N);
+                    float* p = g.part + (((size_t)split * (gridDim.z / g.splits) + zs) * g.M + m) * planes<EPI>() * np + n;
+                    cg_store<float, 8>(p, 8, v);
+                    if (EPI == EPI_GATE_FWD) cg_store<float, 8>(p + np, 8, w);
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 template <typename T, int BM, int BN, int WM, int WN, bool KA, bool KB, int EPI>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void gemm_kernel(Gemm<T> g) {
     constexpr int NW = (BM / WM) * (BN / WN), NT = NW * 64, TM = WM / 32, TN = WN / 32;
@@ -237,17 +289,12 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void gemm_kernel(Gem
     typedef Operand<T, BN, NT, KB, EPI == EPI_GATE_FWD> OB;
     constexpr int P = OA::P, BK = OA::BK, EP = WN + 4;
     constexpr int SMEM = OA::BYTES + OB::BYTES > NW * 32 * EP * 4 ? OA::BYTES + OB::BYTES : NW * 32 * EP * 4;
-    static_assert(WN == 64, "a wave's 64 columns are 32 gate and 32 value columns");
     __shared__ __attribute__((aligned(16))) char smem[SMEM];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
 
-    // blocks go to the 8 XCDs in turn: each XCD takes a run of neighbouring tiles, in panels of 8 tile rows, so that what its L2 holds is
-    // read again
-    const unsigned nt = gridDim.x, xcd = blockIdx.x & 7, q = nt / 8, rem = nt % 8;
-    const unsigned t = xcd * q + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
-    const unsigned panel = 8 * g.tiles_n, pm = t / panel * 8, pr = t % panel, ph = g.tiles_m - pm < 8 ? g.tiles_m - pm : 8;
-    const size_t m0 = (size_t)(pm + pr % ph) * BM;
-    const int n0 = (int)(pr / ph) * (EPI == EPI_GATE_FWD ? BN / 2 : BN);
+    size_t m0;
+    int n0;
+    tile_origin<BM, EPI == EPI_GATE_FWD ? BN / 2 : BN>(g.tiles_m, g.tiles_n, m0, n0);
     const int split = blockIdx.z % g.splits, zs = blockIdx.z / g.splits, sel = zs % g.nsel;
     const size_t z = zs / g.nsel;
 
@@ -294,43 +341,180 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void gemm_kernel(Gem
         }
     }
 
-    // the accumulators go through LDS (32 rows of a wave at a time) so that every lane stores 8 consecutive columns
     __syncthreads();
-    float* ep = (float*)smem + wid * 32 * EP;
-    constexpr int LPR = EPI == EPI_GATE_FWD ? 4 : 8, RPP = 64 / LPR;
+    store_tile<T, EPI, TM, TN>(g, acc, (float*)smem + wid * 32 * EP, lane, m0 + wm, n0 + (EPI == EPI_GATE_FWD ? wn / 2 : wn), z, sel,
+                               split, zs);
+}
+
+// ------------------------------------------------------------------------------------------
+// The same product of 16-bit operands in 256 x 256 tiles, for operands whose rows start on 16 bytes: 8 waves of 128 x 64, one block a CU.
+//
+// The tiles come straight from memory into LDS (buffer_load_dwordx4 ... lds: 64 lanes x 16 bytes to consecutive LDS addresses, no
+// registers on the way), so the swizzle is in the address that each lane fetches: chunk c of row r of a K-contiguous tile lies at
+// c ^ (r & 7); chunk c of depth k of a row-contiguous tile at c ^ 4 (k & 3), which puts the four depths that 16 lanes of a transposing
+// read gather 64 bytes apart.  What lies outside the operand reads as zero (buffer bounds).
+// Two buffers of 64 K-steps: while one is multiplied, the other is filled.  The fragments of a 16-deep step are read while the step
+// before it is on the matrix pipe, across the buffer change too: before the last step of a buffer every wave has its fragments in
+// registers, waits for its own loads of the next buffer, meets the others, and starts refilling the buffer that is now free.
+// The loads are issued from inline assembly because the compiler takes the builtin for a store to all of LDS and would wait for it before
+// every read; the waits are therefore by hand.
+// ------------------------------------------------------------------------------------------
+typedef int rsrc4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void dma16(rsrc4 rsrc, unsigned lds, unsigned off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
+}
+
+constexpr unsigned OUTSIDE = 0x80000000u, MOST = 0x7fffff00u;      // an offset past every bound; the largest bound
+
+template <typename T, bool KC> struct WideOperand {
+    typedef typename V8<T>::V Frag;
+    static constexpr int ROWS = 256, BK = 64, PIECES = 4, BYTES = ROWS * BK * 2;
+    unsigned off[PIECES], k_of[PIECES];     // K-contiguous: first k of the lane's chunk
+
+    // wave w fills LDS rows w * 32 + 8 i .. (K-contiguous) or depths w * 8 + 2 i .. (row-contiguous)
+    __device__ __forceinline__ void init(int w, int lane, size_t ld) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) ep[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * EP + j * 32 + (lane & 31)] = acc[i][j][r];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int pass = 0; pass < 32 / RPP; ++pass) {
-            const int row = pass * RPP + lane / LPR, col = lane % LPR * 8;
-            const size_t m = m0 + wm + i * 32 + row;
-            const int n = n0 + (EPI == EPI_GATE_FWD ? wn / 2 : wn) + col;
-            float v[8], w[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[e] = ep[row * EP + col + e];
-                if (EPI == EPI_GATE_FWD) w[e] = ep[row * EP + 32 + col + e];
-            }
-            if (m < g.M && n < g.N) {
-                if (g.splits == 1) {
-                    emit<T, EPI>(g, z, sel, m, n, v, w);
-                } else {
-                    const size_t np = pad8(g.N);
-                    float* p = g.part + (((size_t)split * (gridDim.z / g.splits) + zs) * g.M + m) * planes<EPI>() * np + n;
-                    cg_store<float, 8>(p, 8, v);
-                    if (EPI == EPI_GATE_FWD) cg_store<float, 8>(p + np, 8, w);
-                }
+        for (int i = 0; i < PIECES; ++i) {
+            if (KC) {
+                const int r = lane >> 3, c = (lane & 7) ^ r;
+                k_of[i] = c * 8;
+                off[i] = (unsigned)((w * 32 + i * 8 + r) * ld * 2) + c * 16;
+            } else {
+                const int k = w * 8 + i * 2 + (lane >> 5), c = (lane & 31) ^ ((k & 3) << 2);
+                off[i] = (unsigned)(k * ld * 2) + c * 16;
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
     }
+    // GATE operands: wave w's rows come from the gate (w even) or value (w odd) weights, 32 rows of each in turn
+    __device__ __forceinline__ void init_gate(int w, int lane, size_t ld) {
+        init(w, lane, ld);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) off[i] -= (unsigned)((w * 32 - (w >> 1) * 32) * ld * 2);
+    }
+    // p: the operand; row0, k0: the tile's origin; rows, K: the operand's extent
+    __device__ __forceinline__ void fill(const T* p, size_t ld, size_t row0, size_t rows, size_t k0, size_t K, unsigned lds, int w) const {
+        const size_t total = (KC ? rows : K) * ld * 2, at = (KC ? row0 * ld + k0 : k0 * ld + row0) * 2;
+        const size_t left = at < total ? total - at : 0;
+        const unsigned long long a = (unsigned long long)p + at;
+        rsrc4 r;
+        r[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
+        r[1] = __builtin_amdgcn_readfirstlane((int)((unsigned)(a >> 32) & 0xffffu));
+        r[2] = __builtin_amdgcn_readfirstlane((int)(left < MOST ? (unsigned)left : MOST));
+        r[3] = 0x00020000;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const unsigned o = KC && k0 + k_of[i] >= K ? OUTSIDE : off[i];
+            dma16(r, lds + (w * PIECES + i) * 1024, o);
+        }
+    }
+    static __device__ __forceinline__ Frag at(unsigned a) { return *(const __attribute__((address_space(3))) Frag*)(size_t)a; }
+    // address of the fragment of rows r0 + 32 j (r0 a multiple of 64) at step 0; frag() adds the step
+    static __device__ __forceinline__ unsigned addr(int lane, int r0, int j) {
+        if (KC) return (r0 + j * 32 + (lane & 31)) * 128 + (((lane >> 5) ^ (lane & 7)) << 4);
+        const int sl = lane & 15, c = (r0 + j * 32) / 8 + ((lane >> 4) & 1) * 2 + ((sl & 3) >> 1);
+        return ((lane >> 5) * 8 + (sl >> 2)) * 512 + ((c ^ ((sl >> 2) << 2)) << 4) + (sl & 1) * 8;
+    }
+    static __device__ __forceinline__ Frag frag(unsigned base, unsigned a, int ks) {
+        if constexpr (KC) {
+            return at(base + (a ^ (ks << 5)));
+        } else {
+            typedef __attribute__((address_space(3))) s16x4* Q;
+            struct { s16x4 a, b; } f;
+            f.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Q)(size_t)(base + a + ks * 8192));
+            f.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Q)(size_t)(base + a + ks * 8192 + 2048));
+            return __builtin_bit_cast(Frag, f);
+        }
+    }
+};
+
+template <typename T, bool KA, bool KB, int EPI> __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(Gemm<T> g) {
+    typedef WideOperand<T, KA> OA;
+    typedef WideOperand<T, KB> OB;
+    constexpr int TM = 4, TN = 2, BK = 64, BUF = OA::BYTES + OB::BYTES;
+    __shared__ __attribute__((aligned(1024))) char smem[2 * BUF];
+    const unsigned lds = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    size_t m0;
+    int n0;
+    tile_origin<256, EPI == EPI_GATE_FWD ? 128 : 256>(g.tiles_m, g.tiles_n, m0, n0);
+    const int split = blockIdx.z % g.splits, zs = blockIdx.z / g.splits, sel = zs % g.nsel;
+    const size_t z = zs / g.nsel;
+    const int wm = (wid >> 2) * 128, wn = (wid & 3) * 64;
+
+    f32x16 acc[TM][TN] = {};
+    const int kt = (int)((g.K + BK - 1) / BK), all = kt * g.nseg;
+    const int k_begin = (int)((long long)all * split / g.splits), k_end = (int)((long long)all * (split + 1) / g.splits);
+    OA a;
+    OB b;
+    a.init(wid, lane, g.lda);
+    if (EPI == EPI_GATE_FWD) b.init_gate(wid, lane, g.ldb);
+    else b.init(wid, lane, g.ldb);
+    auto fill = [&](int step, int buf) {
+        const int s = step >= kt ? 1 : 0;
+        const size_t k = (size_t)(step - s * kt) * BK;
+        a.fill((g.nseg == 2 ? g.A[s] : g.A[sel]) + z * g.az, g.lda, m0, g.M, k, g.K, lds + buf * BUF, wid);
+        b.fill((EPI == EPI_GATE_FWD ? g.B[wid & 1] : g.nseg == 2 ? g.B[s] : g.B[0]) + z * g.bz, g.ldb, n0, g.N, k, g.K,
+               lds + buf * BUF + OA::BYTES, wid);
+    };
+    unsigned aa[TM], ba[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) aa[i] = OA::addr(lane, wm, i);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) ba[j] = OB::addr(lane, wn, j);
+    typename OA::Frag fa[2][TM];
+    typename OB::Frag fb[2][TN];
+    auto read = [&](int buf, int ks, int f) {
+        const unsigned base = lds + buf * BUF;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) fb[f][j] = OB::frag(base + OA::BYTES, ba[j], ks);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) fa[f][i] = OA::frag(base, aa[i], ks);
+    };
+    auto multiply = [&](int f) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = mfma(fa[f][i], fb[f][j], acc[i][j]);
+    };
+    constexpr int READS = TM * (KA ? 1 : 2) + TN * (KB ? 1 : 2), PER = READS > TM * TN ? 2 : 1;
+    auto interleave = [&]() {       // the reads of the next step spread between the products of this one
+#pragma unroll
+        for (int i = 0; i < TM * TN; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (k_begin < k_end) {
+        fill(k_begin, 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (k_begin + 1 < k_end) fill(k_begin + 1, 1);
+        read(0, 0, 0);
+        int buf = 0;
+        for (int step = k_begin; step < k_end; ++step, buf ^= 1) {
+#pragma unroll
+            for (int ks = 0; ks < 3; ++ks) {
+                read(buf, ks + 1, (ks + 1) & 1);
+                multiply(ks & 1);
+                interleave();
+            }
+            if (step + 1 < k_end) {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if (step + 2 < k_end) fill(step + 2, buf);
+                read(buf ^ 1, 0, 0);
+                multiply(1);
+                interleave();
+            }
+        }
+        multiply(1);
+    }
+    __syncthreads();
+    store_tile<T, EPI, TM, TN>(g, acc, (float*)smem + wid * 32 * 68, lane, m0 + wm, n0 + (EPI == EPI_GATE_FWD ? wn / 2 : wn), z, sel, split,
+                               zs);
 }
 
 // joins the partial sums of a split product, in the order of the splits
@@ -355,36 +539,60 @@ template <typename T, int EPI> __global__ __launch_bounds__(256) void join_kerne
     }
 }
 
-// Tile and number of K splits.  128 x 128 tiles (4 waves of 64 x 64) wherever they can fill the chip, split or not; 64 x 64 (2 waves)
-// below.  A split takes at least 4 K-steps; splits are added until there are two blocks for every CU.  The number of members is left out:
-// a member's results do not depend on how many run beside it.
-struct Plan { int big, splits; };
-Plan plan(size_t M, size_t N, size_t K, int nsel, int esz) {
+// Tile and number of K splits.  `wide` (both operands 16 bit, rows on 16 bytes): 256 x 256 tiles wherever they can fill the chip, split
+// or not; then 128 x 128 tiles (4 waves of 64 x 64), then 64 x 64 (2 waves).  A split takes at least 4 K-steps.  Wide tiles run one a CU
+// in rounds of 256: the number of splits is the one with the least rounds + join (a K-step of a tile takes about 1 us; the partial
+// sums are written and read at about 5 TB/s).  Smaller tiles are split until there are two blocks for every CU.  The number of members
+// is left out: a member's results do not depend on how many run beside it.
+struct Plan { int tile, splits; };
+Plan plan(size_t M, size_t N, size_t K, int nsel, int esz, bool wide) {
     const size_t bk = esz == 4 ? 32 : 64, steps = (K + bk - 1) / bk, most = steps / 4 > 1 ? steps / 4 : 1;
-    const size_t t128 = (size_t)cg_div_up(M, 128) * cg_div_up(N, 128) * nsel, t64 = (size_t)cg_div_up(M, 64) * cg_div_up(N, 64) * nsel;
-    Plan p = {0, 1};
-    if (!t128) return p;        // no rows
-    p.big = t128 * most >= 192;
-    const size_t t = p.big ? t128 : t64, want = (512 + t - 1) / t;
-    p.splits = t >= 256 ? 1 : (int)(want < most ? want : most);
-    return p;
+    auto tiles = [&](size_t t) { return (size_t)cg_div_up(M, t) * cg_div_up(N, t) * nsel; };
+    if (!M || !N) return {64, 1};
+    if (wide && tiles(256) * most >= 192) {
+        Plan p = {256, 1};
+        double best = 0;
+        for (size_t s = 1; s <= most && s <= 16; ++s) {
+            const double t = (double)((tiles(256) * s + 255) / 256) * (double)((steps + s - 1) / s) + 4 +
+                             (s > 1 ? 2.0 * 4 * s * M * N * nsel / 5e6 + 4 : 0);
+            if (s == 1 || t < best) best = t, p.splits = (int)s;
+        }
+        return p;
+    }
+    const int tile = tiles(128) * most >= 192 ? 128 : 64;
+    const size_t t = tiles(tile), want = (512 + t - 1) / t;
+    return {tile, t >= 256 ? 1 : (int)(want < most ? want : most)};
 }
 size_t part_bytes(size_t M, size_t N, size_t K, int members, int nsel, int esz, int np) {      // N: columns of the product
-    const Plan p = plan(M, N, K, nsel, esz);
-    return p.splits > 1 ? (size_t)p.splits * members * nsel * M * np * pad8((int)(N / np)) * 4 : 0;
+    size_t most = 0;
+    for (int wide = 0; wide < (esz == 2 ? 2 : 1); ++wide) {
+        const Plan p = plan(M, N, K, nsel, esz, wide);
+        const size_t n = p.splits > 1 ? (size_t)p.splits * members * nsel * M * np * pad8((int)(N / np)) * 4 : 0;
+        most = n > most ? n : most;
+    }
+    return most;
 }
 
 template <typename T, bool KA, bool KB, int EPI> void gemm(Gemm<T>& g, int members, float* part, hipStream_t st) {
     if (!g.M || !g.N) return;
     const int nz = members * g.nsel;
     const size_t N = (size_t)g.N * planes<EPI>();
-    const Plan p = plan(g.M, N, g.K * g.nseg, g.nsel, sizeof(T));
+    bool wide = false;
+    if constexpr (sizeof(T) == 2) {
+        wide = g.lda % 8 == 0 && g.ldb % 8 == 0 && g.lda <= 1 << 20 && g.ldb <= 1 << 20 && (!KA || g.K % 8 == 0) && members == 1;
+        for (int i = 0; i < 2; ++i) wide = wide && ((uintptr_t)g.A[i] | (uintptr_t)g.B[i]) % 16 == 0;
+    }
+    const Plan p = plan(g.M, N, g.K * g.nseg, g.nsel, sizeof(T), wide);
     g.part = part, g.splits = p.splits;
-    const int bt = p.big ? 128 : 64;
-    g.tiles_m = cg_div_up(g.M, bt), g.tiles_n = cg_div_up(N, bt);
+    g.tiles_m = cg_div_up(g.M, p.tile), g.tiles_n = cg_div_up(N, p.tile);
     const dim3 grid((unsigned)g.tiles_m * g.tiles_n, 1, nz * p.splits);
-    if (p.big) gemm_kernel<T, 128, 128, 64, 64, KA, KB, EPI><<<grid, 256, 0, st>>>(g);
-    else gemm_kernel<T, 64, 64, 32, 64, KA, KB, EPI><<<grid, 128, 0, st>>>(g);
+    if (p.tile == 256) {
+        if constexpr (sizeof(T) == 2) gemm_wide_kernel<T, KA, KB, EPI><<<grid, 512, 0, st>>>(g);
+    } else if (p.tile == 128) {
+        gemm_kernel<T, 128, 128, 64, 64, KA, KB, EPI><<<grid, 256, 0, st>>>(g);
+    } else {
+        gemm_kernel<T, 64, 64, 32, 64, KA, KB, EPI><<<grid, 128, 0, st>>>(g);
+    }
     if (p.splits > 1) {
         const size_t nb = (g.M * (pad8(g.N) / 8) * nz + 255) / 256;
         join_kernel<T, EPI><<<(unsigned)(nb < 4096 ? nb : 4096), 256, 0, st>>>(g, nz);

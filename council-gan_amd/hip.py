@@ -156,7 +156,7 @@ _SIGS = {
     "cg_layernorm_fwd": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_float, _P, c_size_t, _P]),
     "cg_layernorm_bwd": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_float, _P, c_size_t, _P]),
     "cg_channel_norm_fwd": (c_int, [POINTER(Group), _P, _P, _P, _P, _P, _P, c_size_t, c_int, c_int, c_int, c_float, _P]),
-    "cg_channel_norm_bwd_workspace": (c_size_t, [POINTER(Group), c_size_t, c_int]),
+    "cg_channel_norm_bwd_workspace": (c_size_t, [POINTER(Group), c_size_t, c_int, c_int]),
     "cg_channel_norm_bwd": (c_int, [POINTER(Group), _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_size_t, c_int, c_int, c_int, _P,
                                     c_size_t, _P]),
     "cg_dropout_key": (c_int, [_P, _P, _P]),

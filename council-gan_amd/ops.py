@@ -1700,6 +1700,7 @@ def l1_mean(a, b):
 # accumulators are fp32, every stored value is rounded once.  Scratch memory comes from torch's caching allocator, per call: a captured
 # graph owns its own, and two graphs share none.  All of them run on the current stream of the tensors' device.
 _ctx_null = contextlib.nullcontext()
+_stream_handle = hip._stream_handle
 
 
 def _dev(t):
@@ -1715,6 +1716,12 @@ def _addr(t):
 
 def _dense(t):
     return t.contiguous(memory_format=CL) if t.dim() == 4 else t.contiguous()
+
+
+def _once(what):
+    # autograd leaves recording on in a backward pass that is itself differentiated (create_graph=True)
+    if torch.is_grad_enabled():
+        raise hip.HipError("%s: the backward pass cannot be differentiated again" % what)
 
 
 def _check_rows(what, x):
@@ -1771,7 +1778,7 @@ def _channel_norm_fwd(x, w, b, eps, grp, stats):
     st = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else None
     check(_lib().cg_channel_norm_fwd(grp, x.data_ptr(), w.data_ptr(), _addr(b), y.data_ptr(), _addr(st),
                                      st.data_ptr() + 4 * rows if stats else None, rows, C, hip.DT[x.dtype], hip.DT[w.dtype], eps,
-                                     stream()), "cg_channel_norm_fwd")
+                                     _stream_handle()), "cg_channel_norm_fwd")
     return y, st
 
 
@@ -1785,29 +1792,23 @@ class _ChannelNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _once("channel_norm")
         x, w, st = ctx.saved_tensors
-        need = ctx.needs_input_grad
+        need, lib, grp = ctx.needs_input_grad, _lib(), ctx.grp
         C = w.numel()
         rows = x.numel() // C
+        dt = hip.DT[x.dtype]
         dy = _dense(dy)
         dx = torch.empty_like(x) if need[0] else None
-        dw, aw, rw = _grad_target(w, ctx.bufs[0], need[1], ctx.grp)
-        db, ab, rb = _grad_target(ctx.b, ctx.bufs[1], need[2], ctx.grp)
-        lib = _lib()
-        args = (rows, C, hip.DT[x.dtype], hip.DT[w.dtype])
-        ws = torch.empty(lib.cg_channel_norm_bwd_workspace(ctx.grp, rows, C), dtype=torch.uint8, device=x.device)
-
-        def run(dx, dw, db, acc):
-            check(lib.cg_channel_norm_bwd(ctx.grp, dy.data_ptr(), x.data_ptr(), w.data_ptr(), st.data_ptr(), st.data_ptr() + 4 * rows,
-                                          _addr(dx), _addr(dw), _addr(db), acc, *args, ws.data_ptr(), ws.numel(), stream()),
-                  "cg_channel_norm_bwd")
-        if dw is not None and db is not None and aw != ab:      # one of the two gradients has a buffer of its optimizer
-            run(dx, dw, None, aw)
-            run(None, None, db, ab)
-        else:
-            run(dx, dw, db, aw | ab)
+        dw, aw, rw = _grad_target(w, ctx.bufs[0], need[1], grp)
+        db, ab, rb = _grad_target(ctx.b, ctx.bufs[1], need[2], grp)
+        nws = lib.cg_channel_norm_bwd_workspace(grp, rows, C, dt) if need[1] or need[2] else 0
+        ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
+        sp = st.data_ptr()
+        check(lib.cg_channel_norm_bwd(grp, dy.data_ptr(), x.data_ptr(), w.data_ptr(), sp, sp + 4 * rows, _addr(dx), _addr(dw), _addr(db),
+                                      aw | ab << 1, rows, C, dt, hip.DT[w.dtype], _addr(ws), nws, _stream_handle()),
+              "cg_channel_norm_bwd")
         return dx, rw, rb, None, None, None
 
 
@@ -1849,14 +1850,14 @@ def dropout_key(state):
     _check_key("dropout_key", state)
     with _dev(state):
         key = torch.empty_like(state)
-        check(_lib().cg_dropout_key(state.data_ptr(), key.data_ptr(), stream()), "cg_dropout_key")
+        check(_lib().cg_dropout_key(state.data_ptr(), key.data_ptr(), _stream_handle()), "cg_dropout_key")
         torch.autograd.graph.increment_version(state)
     return key
 
 
 def _dropout_run(x, res, t, key):
     y = torch.empty_like(x)
-    check(_lib().cg_dropout(x.data_ptr(), _addr(res), y.data_ptr(), x.numel(), t, key.data_ptr(), hip.DT[x.dtype], stream()),
+    check(_lib().cg_dropout(x.data_ptr(), _addr(res), y.data_ptr(), x.numel(), t, key.data_ptr(), hip.DT[x.dtype], _stream_handle()),
           "cg_dropout")
     return y
 
@@ -1872,8 +1873,8 @@ class _Dropout(torch.autograd.Function):
         return _dropout_run(x, None if res is None else _dense(res), t, key)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _once("dropout")
         (key,) = ctx.saved_tensors
         dx = _dropout_run(_dense(dy), None, ctx.t, key) if ctx.needs_input_grad[0] else None
         return dx, dy if ctx.needs_input_grad[1] else None, None, None
@@ -1934,7 +1935,7 @@ def _gated_fwd(x, wg, wv, wo, bg, bv, bo, gate, grp, keep):
     nws = lib.cg_gated_ff_fwd_workspace(dims, grp)
     ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
     check(lib.cg_gated_ff_fwd(dims, grp, x.data_ptr(), wg.data_ptr(), wv.data_ptr(), _addr(wo), _addr(bg), _addr(bv), _addr(bo),
-                              h.data_ptr(), _addr(a), _addr(v), _addr(y), _addr(ws), nws, stream()), "cg_gated_ff_fwd")
+                              h.data_ptr(), _addr(a), _addr(v), _addr(y), _addr(ws), nws, _stream_handle()), "cg_gated_ff_fwd")
     return y, h, a, v
 
 
@@ -1950,8 +1951,8 @@ class _GatedFeedForward(torch.autograd.Function):
         return h if y is None else y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _once("gated_feed_forward")
         x, wg, wv, wo, h, a, v = ctx.saved_tensors
         grp, need = ctx.grp, ctx.needs_input_grad
         F, D = wg.shape
@@ -1967,7 +1968,7 @@ class _GatedFeedForward(torch.autograd.Function):
             ret.append(r)
         ws = torch.empty(lib.cg_gated_ff_bwd_workspace(dims, grp), dtype=torch.uint8, device=x.device)
         check(lib.cg_gated_ff_bwd(dims, grp, dy.data_ptr(), x.data_ptr(), wg.data_ptr(), wv.data_ptr(), _addr(wo), _addr(h),
-                                  a.data_ptr(), v.data_ptr(), _addr(dx), *outs, acc, ws.data_ptr(), ws.numel(), stream()),
+                                  a.data_ptr(), v.data_ptr(), _addr(dx), *outs, acc, ws.data_ptr(), ws.numel(), _stream_handle()),
               "cg_gated_ff_bwd")
         return (dx, *ret, None, None, None)
 

@@ -444,8 +444,8 @@ int cg_layernorm_bwd(const float* dy, const float* x, const float* gamma, const 
  * weight / bias: `wdtype` = dtype or CG_DT_F32; bias may be NULL.  mean / rstd (both or neither): [rows], for the backward pass. */
 int cg_channel_norm_fwd(const cg_group* grp, const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
                         size_t rows, int C, int dtype, int wdtype, float eps, cg_stream_t stream);
-size_t cg_channel_norm_bwd_workspace(const cg_group* grp, size_t rows, int C);
-/* dx, dweight, dbias: any may be NULL; `accumulate` adds to dweight / dbias instead of overwriting them */
+size_t cg_channel_norm_bwd_workspace(const cg_group* grp, size_t rows, int C, int dtype);
+/* dx, dweight, dbias: any may be NULL; `accumulate` bit 0 / 1 adds to dweight / dbias instead of overwriting it */
 int cg_channel_norm_bwd(const cg_group* grp, const void* dy, const void* x, const void* weight, const float* mean, const float* rstd,
                         void* dx, void* dweight, void* dbias, int accumulate, size_t rows, int C, int dtype, int wdtype, void* ws,
                         size_t ws_bytes, cg_stream_t stream);

@@ -69,7 +69,7 @@ def test_library_refuses_bad_arguments_before_any_launch():
     assert lib.cg_channel_norm_fwd(None, p, p, None, p, None, None, 4, 0, 0, 0, 1e-5, None) == -1
     assert lib.cg_channel_norm_fwd(None, p, p, None, p, None, None, 4, 8, 0, 1, 1e-5, None) == -1       # fp16 weight of an fp32 row
     assert lib.cg_channel_norm_fwd(None, p, p, None, p, p, None, 4, 8, 0, 0, 1e-5, None) == -1          # mean without rstd
-    assert lib.cg_channel_norm_bwd(None, p, p, p, p, p, p, p, p, 0, 4, 8, 0, 0, p, 8, None) == -3       # workspace
+    assert lib.cg_channel_norm_bwd(None, p, p, p, p, p, p, p, p, 0, 4096, 8, 0, 0, p, 8, None) == -3       # workspace
     assert lib.cg_channel_norm_bwd(ctypes.byref(hip.Group(3, 0, 32)), p, p, p, p, p, p, p, p, 0, 4, 8, 0, 0, p, 1 << 20, None) == -1
     assert lib.cg_dropout(p, None, p, 4, 65536, p, 0, None) == -1
     assert lib.cg_dropout(p, None, p, 4, 1, p, 3, None) == -1
@@ -94,7 +94,7 @@ def test_workspaces_of_any_size_are_finite():
                 assert lib.cg_gated_ff_fwd_workspace(d, grp) < 1 << 33
                 hidden = rows * 520 * (4 if dt == 0 else 2)
                 assert 2 * hidden <= lib.cg_gated_ff_bwd_workspace(d, grp) < 2 * hidden + (1 << 33)
-        assert lib.cg_channel_norm_bwd_workspace(None, rows, 264) < 1 << 33
+        assert lib.cg_channel_norm_bwd_workspace(None, rows, 264, 0) < 1 << 33
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])

@@ -503,3 +503,13 @@ def test_member_batched_refusals(cga):
             cga.ops.channel_norm(x, ps[0][0])
         with pytest.raises(cga.hip.HipError, match="equal blocks"):
             cga.ops.gated_feed_forward(x, *ps[0][2:])
+
+
+def test_backward_passes_are_not_differentiated_again(cga):
+    x, ps, dy = gated_inputs(gen(40), 6, 16, 24, 16, False, F32)
+    w = torch.ones(16, device="cuda")
+    for f in (lambda t: cga.ops.channel_norm(t, w), lambda t: cga.ops.dropout(t, 0.5, key_of(1, 2)),
+              lambda t: cga.ops.gated_feed_forward(t, *ps)):
+        xl = x.detach().requires_grad_(True)
+        with pytest.raises(cga.hip.HipError, match="cannot be differentiated again"):
+            torch.autograd.grad(f(xl), xl, dy, create_graph=True)
