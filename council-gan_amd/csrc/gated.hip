@@ -30,6 +30,8 @@ template <typename T> struct Gemm {
     T *o0, *o1, *o2;          // EPI_GATE_FWD: h, a, v; EPI_GATE_BWD: da, dv
     const T *i0, *i1;         // EPI_GATE_BWD: a, v
     size_t oz;
+    float* sums;              // EPI_GATE_BWD, or NULL: column sums of da and dv over a wave's rows, [member][2][strips][N]
+    int strips;
     float* part;              // splits > 1: partial sums [split][member * nsel + sel][M][planes][NP]
     int splits, tiles_m, tiles_n;
 };
@@ -47,38 +49,61 @@ __device__ __forceinline__ void gate_fn(float a, int gate, float& u, float& du) 
 }
 
 // ------------------------------------------------------------------------------------------
-// epilogue of 8 consecutive columns: v = the sums (EPI_GATE_FWD: of the gate, w of the value projection)
+// epilogue of 8 consecutive columns: v = the sums (EPI_GATE_FWD: of the gate, w of the value projection).  What it reads is fetched
+// ahead: the biases of its columns once, the rest of a row (`Row`) while earlier rows are on their way out.
 // ------------------------------------------------------------------------------------------
+template <typename T> struct Chunk { typename CgT<T>::V q[8 / CgT<T>::N]; };
+template <typename T> __device__ __forceinline__ void get(Chunk<T>& c, const T* p, int left) {
+    constexpr int W = CgT<T>::N;
+    if (left >= 8) {
+#pragma unroll
+        for (int i = 0; i < 8 / W; ++i) c.q[i] = *(const typename CgT<T>::V*)(p + i * W);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c.q[i / W][i % W] = i < left ? p[i] : (T)0.f;
+    }
+}
+template <typename T> struct Row { Chunk<T> x, y; };
+template <typename T, int EPI> __device__ __forceinline__ void fetch_row(const Gemm<T>& g, size_t z, int sel, size_t m, int n, Row<T>& r) {
+    const int left = m < g.M ? g.N - n : 0;
+    if (EPI == EPI_STORE && (g.accumulate >> sel & 1)) get<T>(r.x, g.c[sel] + z * g.cz + m * g.N + n, left);
+    if (EPI == EPI_GATE_BWD) {
+        const size_t o = z * g.oz + m * g.N + n;
+        get<T>(r.x, g.i0 + o, left);
+        get<T>(r.y, g.i1 + o, left);
+    }
+}
+struct Bias { float x[8], y[8]; };
+template <typename T, int EPI> __device__ __forceinline__ void fetch_bias(const Gemm<T>& g, size_t z, int n, Bias& b) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b.x[i] = b.y[i] = 0.f;
+    if (EPI != EPI_GATE_BWD && g.bias[0]) cg_load<T, 8>(g.bias[0] + z * g.biasz + n, g.N - n, b.x);
+    if (EPI == EPI_GATE_FWD && g.bias[1]) cg_load<T, 8>(g.bias[1] + z * g.biasz + n, g.N - n, b.y);
+}
+
 template <typename T, int EPI>
-__device__ __forceinline__ void emit(const Gemm<T>& g, size_t z, int sel, size_t m, int n, float (&v)[8], float (&w)[8]) {
+__device__ __forceinline__ void emit(const Gemm<T>& g, size_t z, int sel, size_t m, int n, float (&v)[8], float (&w)[8], const Bias& b,
+                                     const Row<T>& row, float (&sx)[8], float (&sy)[8]) {
+    constexpr int W = CgT<T>::N;
     const int left = g.N - n;
-    float x[8], y[8];
     if (EPI == EPI_STORE) {
-        T* c = g.c[sel] + z * g.cz + m * g.N + n;
-        if (g.bias[0]) {
-            cg_load<T, 8>(g.bias[0] + z * g.biasz + n, left, x);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += x[i];
+        for (int i = 0; i < 8; ++i) {
+            v[i] += b.x[i];
+            if (g.accumulate >> sel & 1) v[i] += (float)row.x.q[i / W][i % W];
         }
-        if (g.accumulate >> sel & 1) {
-            cg_load<T, 8>(c, left, x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += x[i];
-        }
-        cg_store<T, 8>(c, left, v);
+        cg_store<T, 8>(g.c[sel] + z * g.cz + m * g.N + n, left, v);
         return;
     }
     const size_t o = z * g.oz + m * g.N + n;
     float u, du;
     if (EPI == EPI_GATE_FWD) {
-        if (g.bias[0]) cg_load<T, 8>(g.bias[0] + z * g.biasz + n, left, x);
-        if (g.bias[1]) cg_load<T, 8>(g.bias[1] + z * g.biasz + n, left, y);
         float h[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             // act(a) v is formed from the rounded a, v: the values the backward pass differentiates
-            v[i] = (float)(T)(v[i] + (g.bias[0] ? x[i] : 0.f));
-            w[i] = (float)(T)(w[i] + (g.bias[1] ? y[i] : 0.f));
+            v[i] = (float)(T)(v[i] + b.x[i]);
+            w[i] = (float)(T)(w[i] + b.y[i]);
             gate_fn(v[i], g.gate, u, du);
             h[i] = u * w[i];
         }
@@ -88,13 +113,13 @@ __device__ __forceinline__ void emit(const Gemm<T>& g, size_t z, int sel, size_t
             cg_store<T, 8>(g.o2 + o, left, w);
         }
     } else {
-        cg_load<T, 8>(g.i0 + o, left, x);
-        cg_load<T, 8>(g.i1 + o, left, y);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            gate_fn(x[i], g.gate, u, du);
+            gate_fn((float)row.x.q[i / W][i % W], g.gate, u, du);
             w[i] = v[i] * u;
-            v[i] = v[i] * y[i] * du;
+            v[i] = v[i] * (float)row.y.q[i / W][i % W] * du;
+            sx[i] += v[i];
+            sy[i] += w[i];
         }
         cg_store<T, 8>(g.o0 + o, left, v);
         cg_store<T, 8>(g.o1 + o, left, w);
@@ -245,30 +270,44 @@ template <int BM, int BN> __device__ __forceinline__ void tile_origin(int tiles_
 template <typename T, int EPI, int TM, int TN>
 __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)[TM][TN], float* ep, int lane, size_t mw, int nw,
                                            size_t z, int sel, int split, int zs) {
-    constexpr int EP = TN * 32 + 4, LPR = EPI == EPI_GATE_FWD ? 4 : 8, RPP = 64 / LPR;
+    constexpr int EP = TN * 32 + 4, LPR = EPI == EPI_GATE_FWD ? 4 : 8, RPP = 64 / LPR, PASSES = 32 / RPP;
     static_assert(TN == 2, "a wave's 64 columns are 32 gate and 32 value columns");
+    const int n = nw + lane % LPR * 8;
+    const size_t ml = mw + lane / LPR;
+    const bool whole = g.splits == 1;
+    Bias bias;
+    float sx[8] = {}, sy[8] = {};
+    Row<T> row[2][PASSES];
+    auto fetch = [&](int i) {
+#pragma unroll
+        for (int pass = 0; pass < PASSES; ++pass) fetch_row<T, EPI>(g, z, sel, ml + i * 32 + pass * RPP, n, row[i & 1][pass]);
+    };
+    if (whole) {
+        fetch_bias<T, EPI>(g, z, n, bias);
+        fetch(0);
+    }
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) ep[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * EP + j * 32 + (lane & 31)] = acc[i][j][r];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
         __builtin_amdgcn_wave_barrier();
+        if (whole && i + 1 < TM) fetch(i + 1);
 #pragma unroll
-        for (int pass = 0; pass < 32 / RPP; ++pass) {
-            const int row = pass * RPP + lane / LPR, col = lane % LPR * 8;
-            const size_t m = mw + i * 32 + row;
-            const int n = nw + col;
+        for (int pass = 0; pass < PASSES; ++pass) {
+            const int at = (pass * RPP + lane / LPR) * EP + lane % LPR * 8;
+            const size_t m = ml + i * 32 + pass * RPP;
             float v[8], w[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                v[e] = ep[row * EP + col + e];
-                if (EPI == EPI_GATE_FWD) w[e] = ep[row * EP + 32 + col + e];
+                v[e] = ep[at + e];
+                if (EPI == EPI_GATE_FWD) w[e] = ep[at + 32 + e];
             }
             if (m < g.M && n < g.N) {
-                if (g.splits == 1) {
-                    emit<T, EPI>(g, z, sel, m, n, v, w);
+                if (whole) {
+                    emit<T, EPI>(g, z, sel, m, n, v, w, bias, row[i & 1][pass], sx, sy);
                 } else {
                     const size_t np = pad8(g.N);
                     float* p = g.part + (((size_t)split * (gridDim.z / g.splits) + zs) * g.M + m) * planes<EPI>() * np + n;
@@ -277,8 +316,23 @@ __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)
                 }
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
         __builtin_amdgcn_wave_barrier();
+    }
+    if (EPI == EPI_GATE_BWD && whole && g.sums) {
+        // lanes of the same columns, then one strip of TM x 32 rows for every wave
+#pragma unroll
+        for (int o = LPR; o < 64; o <<= 1)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                sx[e] += __shfl_xor(sx[e], o, 64);
+                sy[e] += __shfl_xor(sy[e], o, 64);
+            }
+        if (lane < LPR && n < g.N) {
+            float* p = g.sums + (z * 2 * g.strips + mw / (TM * 32)) * g.N + n;
+            cg_store<float, 8>(p, g.N - n, sx);
+            cg_store<float, 8>(p + (size_t)g.strips * g.N, g.N - n, sy);
+        }
     }
 }
 
@@ -535,7 +589,12 @@ template <typename T, int EPI> __global__ __launch_bounds__(256) void join_kerne
                 for (int e = 0; e < 8; ++e) w[e] += x[e];
             }
         }
-        emit<T, EPI>(g, zs / g.nsel, zs % g.nsel, m, n, v, w);
+        Bias bias;
+        Row<T> row;
+        fetch_bias<T, EPI>(g, zs / g.nsel, n, bias);
+        fetch_row<T, EPI>(g, zs / g.nsel, zs % g.nsel, m, n, row);
+        float sx[8] = {}, sy[8] = {};
+        emit<T, EPI>(g, zs / g.nsel, zs % g.nsel, m, n, v, w, bias, row, sx, sy);
     }
 }
 
@@ -585,6 +644,8 @@ template <typename T, bool KA, bool KB, int EPI> void gemm(Gemm<T>& g, int membe
     const Plan p = plan(g.M, N, g.K * g.nseg, g.nsel, sizeof(T), wide);
     g.part = part, g.splits = p.splits;
     g.tiles_m = cg_div_up(g.M, p.tile), g.tiles_n = cg_div_up(N, p.tile);
+    g.strips = 2 * g.tiles_m;
+    if (p.splits > 1) g.sums = nullptr;
     const dim3 grid((unsigned)g.tiles_m * g.tiles_n, 1, nz * p.splits);
     if (p.tile == 256) {
         if constexpr (sizeof(T) == 2) gemm_wide_kernel<T, KA, KB, EPI><<<grid, 512, 0, st>>>(g);
@@ -600,15 +661,23 @@ template <typename T, bool KA, bool KB, int EPI> void gemm(Gemm<T>& g, int membe
 }
 
 // da, dv from a stored gradient of h (no output projection)
-template <typename T>
-__global__ __launch_bounds__(256) void gate_bwd_kernel(const T* __restrict__ dh, const T* __restrict__ a, const T* __restrict__ v,
-                                                       T* __restrict__ da, T* __restrict__ dv, size_t n, int gate) {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        float u, du;
-        gate_fn((float)a[i], gate, u, du);
-        const float d = (float)dh[i];
-        da[i] = (T)(d * (float)v[i] * du);
-        dv[i] = (T)(d * u);
+template <typename T> struct GateBwd { const T *dh, *a, *v; T *da, *dv; size_t n; int gate; };
+template <typename T> __global__ __launch_bounds__(256) void gate_bwd_kernel(GateBwd<T> g) {
+    for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 8; i < g.n; i += (size_t)gridDim.x * 2048) {
+        const int left = g.n - i < 8 ? (int)(g.n - i) : 8;
+        float d[8], a[8], v[8];
+        cg_load<T, 8>(g.dh + i, left, d);
+        cg_load<T, 8>(g.a + i, left, a);
+        cg_load<T, 8>(g.v + i, left, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float u, du;
+            gate_fn(a[e], g.gate, u, du);
+            a[e] = d[e] * v[e] * du;
+            v[e] = d[e] * u;
+        }
+        cg_store<T, 8>(g.da + i, left, a);
+        cg_store<T, 8>(g.dv + i, left, v);
     }
 }
 
@@ -645,11 +714,23 @@ template <typename T> __global__ __launch_bounds__(256) void colsum_part_kernel(
         cg_store<float, N>(g.part + ((size_t)blockIdx.z * g.strips + blockIdx.y) * g.C + c, g.C - c, s);
     }
 }
-template <typename T> __global__ __launch_bounds__(256) void colsum_join_kernel(ColSum<T> g) {
-    const int c = blockIdx.x * 256 + threadIdx.x, sel = blockIdx.z & 1;
-    if (c >= g.C || !g.out[sel]) return;
+// the strips: 32 columns a block, 32 threads a column, each with its share of the strips in order
+template <typename T> __global__ __launch_bounds__(1024) void colsum_join_kernel(ColSum<T> g) {
+    __shared__ float sm[32][33];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5, sel = blockIdx.z & 1;
+    if (!g.out[sel]) return;
     float s = 0.f;
-    for (int i = 0; i < g.strips; ++i) s += g.part[((size_t)blockIdx.z * g.strips + i) * g.C + c];
+    if (c < g.C) {
+        const float* p = g.part + (size_t)blockIdx.z * g.strips * g.C + c;
+#pragma unroll 8
+        for (int i = k; i < g.strips; i += 32) s += p[(size_t)i * g.C];
+    }
+    sm[k][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (k || c >= g.C) return;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += sm[i][threadIdx.x];
     T* o = g.out[sel] + (blockIdx.z >> 1) * g.zs + c;
     *o = (T)(g.accumulate >> sel & 1 ? (float)*o + s : s);
 }
@@ -675,7 +756,7 @@ size_t bwd_part(const cg_gated_dims* d, const cg_group* grp) {
     const size_t M = d->rows / nz, F = d->F, D = d->D, O = d->O;
     const size_t n[] = {O ? part_bytes(M, F, O, nz, 1, e, 1) : 0, part_bytes(M, D, 2 * F, nz, 1, e, 1), part_bytes(F, D, M, nz, 1, e, 1),
                         part_bytes(F, D, M, nz, 2, e, 1), O ? part_bytes(O, F, M, nz, 1, e, 1) : 0,
-                        (size_t)2 * nz * strips_of(M) * (F > O ? F : O) * 4};
+                        (size_t)2 * nz * strips_of(M) * (F > O ? F : O) * 4, (size_t)4 * nz * cg_div_up(M, 64) * F * 4};
     size_t most = 0;
     for (size_t v : n) most = v > most ? v : most;
     return up256(most);
@@ -719,10 +800,16 @@ void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, c
             g.B[0] = wo, g.bz = gs, g.ldb = F;
             g.M = M, g.K = O, g.N = d->F, g.gate = d->gate;
             g.o0 = da, g.o1 = dv, g.i0 = a, g.i1 = v, g.oz = M * F;
+            if (dbg || dbv) g.sums = part;
             gemm<T, true, false, EPI_GATE_BWD>(g, nz, part, st);
+            if (g.sums && M) {
+                ColSum<T> c = {{da, dv}, {dbg, dbv}, M, gs, d->F, g.strips, acc >> 3 & 3, part};
+                colsum_join_kernel<T><<<dim3(cg_div_up(F, 32), 1, 2 * nz), 1024, 0, st>>>(c);
+                dbg = dbv = nullptr;
+            }
         } else if (M) {
-            const size_t n = (size_t)d->rows * F, nb = (n + 255) / 256;
-            gate_bwd_kernel<T><<<(unsigned)(nb < 16384 ? nb : 16384), 256, 0, st>>>(dy, a, v, da, dv, n, d->gate);
+            const size_t n = (size_t)d->rows * F, nb = (n + 2047) / 2048;
+            gate_bwd_kernel<T><<<(unsigned)(nb < 16384 ? nb : 16384), 256, 0, st>>>(GateBwd<T>{dy, a, v, da, dv, n, d->gate});
         }
     }
     if (dx) {
@@ -750,7 +837,7 @@ void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, c
         if (!db0 && !db1) return;
         ColSum<T> g = {{db0 ? p0 : nullptr, db1 ? p1 : nullptr}, {db0, db1}, M, gs, C, strips_of(M), accumulate, part};
         colsum_part_kernel<T><<<dim3(cg_div_up(C, 64 * CgT<T>::N), g.strips, 2 * nz), 256, 0, st>>>(g);
-        colsum_join_kernel<T><<<dim3(cg_div_up(C, 256), 1, 2 * nz), 256, 0, st>>>(g);
+        colsum_join_kernel<T><<<dim3(cg_div_up(C, 32), 1, 2 * nz), 1024, 0, st>>>(g);
     };
     bgrad(da, dv, d->F, dbg, dbv, acc >> 3 & 3);
     if (O) bgrad(dy, nullptr, d->O, dbo, nullptr, acc >> 5 & 1);
