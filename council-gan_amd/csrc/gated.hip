@@ -136,8 +136,8 @@ __host__ __device__ __forceinline__ size_t pad8(int n) { return (size_t)((n + 7)
 // significant bits), and a product is the six terms hh, hm, mh, hl, mm, lh: what is left out is below 2^-23 of |x y|, half a
 // rounding of an fp32 product.  Six products on the 16-bit matrix pipe take less than half the time of one fp32 product on the fp32 one.
 //
-// LDS: a K-contiguous operand lies as [row][K-step] with its 16-byte chunks xor-swizzled by the row, so the eight rows that one
-// pass of ds_read_b128 touches start at eight different bank groups; a row-contiguous one lies as [k][row] and is transposed by the read
+// LDS: a K-contiguous operand lies as [row][K-step] with its 16-byte chunks xor-swizzled by the row, so that the 16 rows that one
+// pass of ds_read_b128 reads (a chunk of each) cover all 64 banks once; a row-contiguous one lies as [k][row] and is transposed by the read
 // (ds_read_b64_tr_b16: inside 16 lanes, lane s names the address of 4 values X[s][0..3] and lane i gets X[4 j + i / 4][i % 4]).
 // ------------------------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -210,7 +210,7 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
         }
     }
     static __device__ __forceinline__ unsigned swz(int row, int chunk) {       // 16-byte chunk of a K-contiguous row
-        return BK == 64 ? (unsigned)(chunk ^ (row & 7)) : (unsigned)(chunk ^ ((row >> 1) & 3));
+        return BK == 64 ? (unsigned)(chunk ^ ((row >> 1) & 7)) : (unsigned)(chunk ^ ((row >> 2) & 3));
     }
     __device__ __forceinline__ void store(char* lds) const {
 #pragma unroll
@@ -405,7 +405,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void gemm_kernel(Gem
 //
 // The tiles come straight from memory into LDS (buffer_load_dwordx4 ... lds: 64 lanes x 16 bytes to consecutive LDS addresses, no
 // registers on the way), so the swizzle is in the address that each lane fetches: chunk c of row r of a K-contiguous tile lies at
-// c ^ (r & 7); chunk c of depth k of a row-contiguous tile at c ^ 4 (k & 3), which puts the four depths that 16 lanes of a transposing
+// c ^ (r / 2 & 7); chunk c of depth k of a row-contiguous tile at c ^ 4 (k & 3), which puts the four depths that 16 lanes of a transposing
 // read gather 64 bytes apart.  What lies outside the operand reads as zero (buffer bounds).
 // Two buffers of 64 K-steps: while one is multiplied, the other is filled.  The fragments of a 16-deep step are read while the step
 // before it is on the matrix pipe, across the buffer change too: before the last step of a buffer every wave has its fragments in
@@ -430,7 +430,7 @@ template <typename T, bool KC> struct WideOperand {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             if (KC) {
-                const int r = lane >> 3, c = (lane & 7) ^ r;
+                const int r = lane >> 3, c = (lane & 7) ^ (((i * 8 + r) >> 1) & 7);
                 k_of[i] = c * 8;
                 off[i] = (unsigned)((w * 32 + i * 8 + r) * ld * 2) + c * 16;
             } else {
@@ -464,7 +464,7 @@ template <typename T, bool KC> struct WideOperand {
     static __device__ __forceinline__ Frag at(unsigned a) { return *(const __attribute__((address_space(3))) Frag*)(size_t)a; }
     // address of the fragment of rows r0 + 32 j (r0 a multiple of 64) at step 0; frag() adds the step
     static __device__ __forceinline__ unsigned addr(int lane, int r0, int j) {
-        if (KC) return (r0 + j * 32 + (lane & 31)) * 128 + (((lane >> 5) ^ (lane & 7)) << 4);
+        if (KC) return (r0 + j * 32 + (lane & 31)) * 128 + (((lane >> 5) ^ ((lane >> 1) & 7)) << 4);
         const int sl = lane & 15, c = (r0 + j * 32) / 8 + ((lane >> 4) & 1) * 2 + ((sl & 3) >> 1);
         return ((lane >> 5) * 8 + (sl >> 2)) * 512 + ((c ^ ((sl >> 2) << 2)) << 4) + (sl & 1) * 8;
     }
