@@ -407,9 +407,13 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void gemm_kernel(Gem
 // registers on the way), so the swizzle is in the address that each lane fetches: chunk c of row r of a K-contiguous tile lies at
 // c ^ (r / 2 & 7); chunk c of depth k of a row-contiguous tile at c ^ 4 (k & 3), which puts the four depths that 16 lanes of a transposing
 // read gather 64 bytes apart.  What lies outside the operand reads as zero (buffer bounds).
-// Two buffers of 64 K-steps: while one is multiplied, the other is filled.  The fragments of a 16-deep step are read while the step
-// before it is on the matrix pipe, across the buffer change too: before the last step of a buffer every wave has its fragments in
-// registers, waits for its own loads of the next buffer, meets the others, and starts refilling the buffer that is now free.
+// A K-contiguous row gives a whole 128-byte line (64 K-steps) to a load: with 64 bytes of a line at a time a piece of 1 KB takes 20 ns
+// instead of 9 (the other half has left the 32 KB L1 when its turn comes).
+// What bounds the loop is the time from a load to its data, more than a microsecond where it is the first to touch a line, against one
+// microsecond of products per 64-deep step.  All 160 KB of LDS hold tiles on their way: three of A and two of B, so A is requested
+// almost two steps ahead and B, first of all after a buffer has become free, one step.  The fragments of a 16-deep step are read while the
+// step before it is on the matrix pipe, across the change of tiles too: before the last step of a tile every wave has its fragments in
+// registers, waits for its own loads of the next tiles, and meets the others.
 // The loads are issued from inline assembly because the compiler takes the builtin for a store to all of LDS and would wait for it before
 // every read; the waits are therefore by hand.
 // ------------------------------------------------------------------------------------------
@@ -423,45 +427,58 @@ constexpr unsigned OUTSIDE = 0x80000000u, MOST = 0x7fffff00u;      // an offset 
 template <typename T, bool KC> struct WideOperand {
     typedef typename V8<T>::V Frag;
     static constexpr int ROWS = 256, BK = 64, PIECES = 4, BYTES = ROWS * BK * 2;
-    unsigned off[PIECES], k_of[PIECES];     // K-contiguous: first k of the lane's chunk
+    unsigned off[PIECES];
+    int k_of[2];     // K-contiguous: first k of the lane's chunk in even and odd pieces
+    // the tile to fill next: its address, the bytes and the K-steps from there to the operand's end, the bytes to the next tile
+    unsigned long long at;
+    long long left, step;
+    int room;
 
     // wave w fills LDS rows w * 32 + 8 i .. (K-contiguous) or depths w * 8 + 2 i .. (row-contiguous)
     __device__ __forceinline__ void init(int w, int lane, size_t ld) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
             if (KC) {
-                const int r = lane >> 3, c = (lane & 7) ^ (((i * 8 + r) >> 1) & 7);
-                k_of[i] = c * 8;
-                off[i] = (unsigned)((w * 32 + i * 8 + r) * ld * 2) + c * 16;
+                const int row = lane >> 3, c = (lane & 7) ^ (((i * 8 + row) >> 1) & 7);
+                k_of[i & 1] = c * 8;
+                off[i] = (unsigned)((w * 32 + i * 8 + row) * ld * 2) + c * 16;
             } else {
                 const int k = w * 8 + i * 2 + (lane >> 5), c = (lane & 31) ^ ((k & 3) << 2);
                 off[i] = (unsigned)(k * ld * 2) + c * 16;
             }
         }
     }
-    // GATE operands: wave w's rows come from the gate (w even) or value (w odd) weights, 32 rows of each in turn
+    // gate / value weights: wave w's rows come from the gate (w even) or the value (w odd) weights, 32 rows of each in turn
     __device__ __forceinline__ void init_gate(int w, int lane, size_t ld) {
         init(w, lane, ld);
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) off[i] -= (unsigned)((w * 32 - (w >> 1) * 32) * ld * 2);
     }
     // p: the operand; row0, k0: the tile's origin; rows, K: the operand's extent
-    __device__ __forceinline__ void fill(const T* p, size_t ld, size_t row0, size_t rows, size_t k0, size_t K, unsigned lds, int w) const {
-        const size_t total = (KC ? rows : K) * ld * 2, at = (KC ? row0 * ld + k0 : k0 * ld + row0) * 2;
-        const size_t left = at < total ? total - at : 0;
-        const unsigned long long a = (unsigned long long)p + at;
-        rsrc4 r;
-        r[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
-        r[1] = __builtin_amdgcn_readfirstlane((int)((unsigned)(a >> 32) & 0xffffu));
-        r[2] = __builtin_amdgcn_readfirstlane((int)(left < MOST ? (unsigned)left : MOST));
-        r[3] = 0x00020000;
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-            const unsigned o = KC && k0 + k_of[i] >= K ? OUTSIDE : off[i];
-            dma16(r, lds + (w * PIECES + i) * 1024, o);
-        }
+    __device__ __forceinline__ void aim(const T* p, size_t ld, size_t row0, size_t rows, size_t k0, size_t K) {
+        const size_t o = (KC ? row0 * ld + k0 : k0 * ld + row0) * 2;
+        at = (unsigned long long)p + o;
+        left = (long long)((KC ? rows : K) * ld * 2) - (long long)o;
+        step = (KC ? BK : BK * (long long)ld) * 2;
+        room = K - k0 < 0x40000000 ? (int)(K - k0) : 0x40000000;
     }
-    static __device__ __forceinline__ Frag at(unsigned a) { return *(const __attribute__((address_space(3))) Frag*)(size_t)a; }
+    __device__ __forceinline__ void next() {
+        at += step;
+        left -= step;
+        room -= BK;
+    }
+    __device__ __forceinline__ rsrc4 window() const {
+        rsrc4 r;
+        r[0] = (int)(unsigned)at;
+        r[1] = (int)((unsigned)(at >> 32) & 0xffffu);
+        r[2] = left <= 0 ? 0 : left < (long long)MOST ? (int)left : (int)MOST;
+        r[3] = 0x00020000;
+        return r;
+    }
+    __device__ __forceinline__ void fill(rsrc4 r, int i, unsigned lds, int w) const {
+        dma16(r, lds + (w * PIECES + i) * 1024, KC && k_of[i & 1] >= room ? OUTSIDE : off[i]);
+    }
+    static __device__ __forceinline__ Frag lds_at(unsigned a) { return *(const __attribute__((address_space(3))) Frag*)(size_t)a; }
     // address of the fragment of rows r0 + 32 j (r0 a multiple of 64) at step 0; frag() adds the step
     static __device__ __forceinline__ unsigned addr(int lane, int r0, int j) {
         if (KC) return (r0 + j * 32 + (lane & 31)) * 128 + (((lane >> 5) ^ ((lane >> 1) & 7)) << 4);
@@ -470,7 +487,7 @@ template <typename T, bool KC> struct WideOperand {
     }
     static __device__ __forceinline__ Frag frag(unsigned base, unsigned a, int ks) {
         if constexpr (KC) {
-            return at(base + (a ^ (ks << 5)));
+            return lds_at(base + (a ^ (ks << 5)));
         } else {
             typedef __attribute__((address_space(3))) s16x4* Q;
             struct { s16x4 a, b; } f;
@@ -484,8 +501,8 @@ template <typename T, bool KC> struct WideOperand {
 template <typename T, bool KA, bool KB, int EPI> __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(Gemm<T> g) {
     typedef WideOperand<T, KA> OA;
     typedef WideOperand<T, KB> OB;
-    constexpr int TM = 4, TN = 2, BK = 64, BUF = OA::BYTES + OB::BYTES;
-    __shared__ __attribute__((aligned(1024))) char smem[2 * BUF];
+    constexpr int TM = 4, TN = 2, BK = OA::BK, A_BUFS = 3, LDS_B = A_BUFS * OA::BYTES;
+    __shared__ __attribute__((aligned(1024))) char smem[A_BUFS * OA::BYTES + 2 * OB::BYTES];
     const unsigned lds = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     size_t m0;
@@ -503,12 +520,28 @@ template <typename T, bool KA, bool KB, int EPI> __global__ __launch_bounds__(51
     a.init(wid, lane, g.lda);
     if (EPI == EPI_GATE_FWD) b.init_gate(wid, lane, g.ldb);
     else b.init(wid, lane, g.ldb);
-    auto fill = [&](int step, int buf) {
-        const int s = step >= kt ? 1 : 0;
-        const size_t k = (size_t)(step - s * kt) * BK;
-        a.fill((g.nseg == 2 ? g.A[s] : g.A[sel]) + z * g.az, g.lda, m0, g.M, k, g.K, lds + buf * BUF, wid);
-        b.fill((EPI == EPI_GATE_FWD ? g.B[wid & 1] : g.nseg == 2 ? g.B[s] : g.B[0]) + z * g.bz, g.ldb, n0, g.N, k, g.K,
-               lds + buf * BUF + OA::BYTES, wid);
+    // the tile to fetch next of either operand: K-step k of segment s, nothing behind k_end
+    auto aim_a = [&](int step) {
+        const int s = g.nseg == 2 && step >= kt ? 1 : 0;
+        const T* p = g.nseg == 2 ? (s ? g.A[1] : g.A[0]) : (sel ? g.A[1] : g.A[0]);
+        a.aim(p + z * g.az, g.lda, m0, g.M, (size_t)(step - s * kt) * BK, g.K);
+    };
+    auto aim_b = [&](int step) {
+        const int s = g.nseg == 2 && step >= kt ? 1 : 0;
+        const T* p = EPI == EPI_GATE_FWD ? (wid & 1 ? g.B[1] : g.B[0]) : s ? g.B[1] : g.B[0];
+        b.aim(p + z * g.bz, g.ldb, n0, g.N, (size_t)(step - s * kt) * BK, g.K);
+    };
+    int next_a = k_begin, next_b = k_begin;
+    const int second = g.nseg == 2 && k_begin < kt ? kt : -1;      // the step at which the second segment begins
+    auto advance_a = [&]() {
+        a.next();
+        if (++next_a == second) aim_a(next_a);
+        if (next_a >= k_end) a.left = 0;
+    };
+    auto advance_b = [&]() {
+        b.next();
+        if (++next_b == second) aim_b(next_b);
+        if (next_b >= k_end) b.left = 0;
     };
     unsigned aa[TM], ba[TN];
 #pragma unroll
@@ -517,55 +550,78 @@ template <typename T, bool KA, bool KB, int EPI> __global__ __launch_bounds__(51
     for (int j = 0; j < TN; ++j) ba[j] = OB::addr(lane, wn, j);
     typename OA::Frag fa[2][TM];
     typename OB::Frag fb[2][TN];
-    auto read = [&](int buf, int ks, int f) {
-        const unsigned base = lds + buf * BUF;
+    auto read = [&](unsigned la, unsigned lb, int ks, int f) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) fb[f][j] = OB::frag(base + OA::BYTES, ba[j], ks);
+        for (int j = 0; j < TN; ++j) fb[f][j] = OB::frag(lb, ba[j], ks);
 #pragma unroll
-        for (int i = 0; i < TM; ++i) fa[f][i] = OA::frag(base, aa[i], ks);
+        for (int i = 0; i < TM; ++i) fa[f][i] = OA::frag(la, aa[i], ks);
     };
-    auto multiply = [&](int f) {
+    auto multiply = [&](int f, int i0) {       // two of the four row blocks
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int i = i0; i < i0 + 2; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[i][j] = mfma(fa[f][i], fb[f][j], acc[i][j]);
     };
-    constexpr int READS = TM * (KA ? 1 : 2) + TN * (KB ? 1 : 2), PER = READS > TM * TN ? 2 : 1;
-    auto interleave = [&]() {       // the reads of the next step spread between the products of this one
+    constexpr int READS = TM * (KA ? 1 : 2) + TN * (KB ? 1 : 2), PER = (READS + 3) / 4;
+    auto interleave = [&]() {       // the reads of the next step spread between the first four products of this one
 #pragma unroll
-        for (int i = 0; i < TM * TN; ++i) {
+        for (int i = 0; i < 4; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
     };
     if (k_begin < k_end) {
-        fill(k_begin, 0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        aim_a(k_begin);
+        aim_b(k_begin);
+        auto fill_a = [&](rsrc4 r, int i, unsigned to) { a.fill(r, i, to, wid); };
+        unsigned a0 = lds, a1 = a0 + OA::BYTES, a2 = a1 + OA::BYTES, b0 = lds + LDS_B, b1 = b0 + OB::BYTES;
+        // tiles 0 of both, then B of step 1 and A of step 1 -- the order that the loop keeps: B of the next step, A of the one after it
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fill_a(a.window(), i, a0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b.fill(b.window(), i, b0, wid);
+        advance_a();
+        advance_b();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fill_a(a.window(), i, a1);
+        asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (k_begin + 1 < k_end) fill(k_begin + 1, 1);
-        read(0, 0, 0);
-        int buf = 0;
-        for (int step = k_begin; step < k_end; ++step, buf ^= 1) {
+        {
+            const rsrc4 rb = b.window();
 #pragma unroll
-            for (int ks = 0; ks < 3; ++ks) {
-                read(buf, ks + 1, (ks + 1) & 1);
-                multiply(ks & 1);
-                interleave();
-            }
-            if (step + 1 < k_end) {
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                if (step + 2 < k_end) fill(step + 2, buf);
-                read(buf ^ 1, 0, 0);
-                multiply(1);
-                interleave();
-            }
+            for (int i = 0; i < 4; ++i) b.fill(rb, i, b1, wid);
         }
-        multiply(1);
+        read(a0, b0, 0, 0);
+        for (int step = k_begin; step < k_end; ++step) {
+            advance_a();
+            advance_b();
+            const rsrc4 ra = a.window(), rb = b.window();
+            read(a0, b0, 1, 1), multiply(0, 0), interleave();
+            fill_a(ra, 0, a2);
+            multiply(0, 2);
+            fill_a(ra, 1, a2);
+            read(a0, b0, 2, 0), multiply(1, 0), interleave();
+            fill_a(ra, 2, a2);
+            multiply(1, 2);
+            fill_a(ra, 3, a2);
+            read(a0, b0, 3, 1), multiply(0, 0), interleave(), multiply(0, 2);
+            // all but the newest four loads (A of the step after the next) have landed
+            asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            b.fill(rb, 0, b0, wid);
+            b.fill(rb, 1, b0, wid);
+            read(a1, b1, 0, 0), multiply(1, 0), interleave();
+            b.fill(rb, 2, b0, wid);
+            b.fill(rb, 3, b0, wid);
+            multiply(1, 2);
+            const unsigned ta = a0, tb = b0;
+            a0 = a1, a1 = a2, a2 = ta, b0 = b1, b1 = tb;
+        }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     store_tile<T, EPI, TM, TN>(g, acc, (float*)smem + wid * 32 * 68, lane, m0 + wm, n0 + (EPI == EPI_GATE_FWD ? wn / 2 : wn), z, sel, split,
                                zs);
