@@ -137,8 +137,9 @@ __host__ __device__ __forceinline__ size_t pad8(int n) { return (size_t)((n + 7)
 // rounding of an fp32 product.  Six products on the 16-bit matrix pipe take less than half the time of one fp32 product on the fp32 one.
 //
 // LDS: a K-contiguous operand lies as [row][K-step] with its 16-byte chunks xor-swizzled by the row, so that the 16 rows that one
-// pass of ds_read_b128 reads (a chunk of each) cover all 64 banks once; a row-contiguous one lies as [k][row] and is transposed by the read
-// (ds_read_b64_tr_b16: inside 16 lanes, lane s names the address of 4 values X[s][0..3] and lane i gets X[4 j + i / 4][i % 4]).
+// pass of ds_read_b128 reads (a chunk of each) cover all 64 banks once; a row-contiguous one lies as [k][row], its chunks xor-swizzled by
+// the depth, and is transposed by the read (ds_read_b64_tr_b16: inside 16 lanes, lane s names the address of 4 values X[s][0..3] and lane
+// i gets X[4 j + i / 4][i % 4]; the four depths that they gather lie 64 bytes apart).
 // ------------------------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((__vector_size__(4 * sizeof(short))));
@@ -162,7 +163,7 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
     static constexpr int P = Mx<T>::P, BK = Mx<T>::BK, W = CgT<T>::N;
     static constexpr int CPR = KC ? BK / W : ROWS / W;             // chunks of W elements per LDS row
     static constexpr int CH = (KC ? ROWS : BK) * CPR / NT;
-    static constexpr int PITCH = KC ? BK * 2 : ROWS * 2 + 64;      // bytes
+    static constexpr int PITCH = KC ? BK * 2 : ROWS * 2;           // bytes
     static constexpr int PLANE = (KC ? ROWS : BK) * PITCH;
     static constexpr int BYTES = P * PLANE;
     static_assert(CH >= 1 && ((KC ? ROWS : BK) * CPR) % NT == 0, "every thread has the same number of chunks");
@@ -209,7 +210,9 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
             for (int i = 0; i < CH; ++i) raw[i] = *(const Raw*)((GATE && (lrow(tid, i) >> 5 & 1) ? p1 : p0) + step + off[i]);
         }
     }
-    static __device__ __forceinline__ unsigned swz(int row, int chunk) {       // 16-byte chunk of a K-contiguous row
+    // where 16-byte chunk `chunk` of LDS row `row` lies in it (a row-contiguous operand's LDS rows are its depths)
+    static __device__ __forceinline__ unsigned swz(int row, int chunk) {
+        if (!KC) return (unsigned)(chunk ^ (ROWS >= 128 ? (row & 3) << 2 : (row >> 1 & 1) << 2));
         return BK == 64 ? (unsigned)(chunk ^ ((row >> 1) & 7)) : (unsigned)(chunk ^ ((row >> 2) & 3));
     }
     __device__ __forceinline__ void store(char* lds) const {
@@ -217,13 +220,13 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
         for (int i = 0; i < CH; ++i) {
             const int r = lrow(tid, i), c = lch(tid);
             if constexpr (P == 1) {
-                *(Frag*)(lds + r * PITCH + (KC ? swz(r, c) : (unsigned)c) * 16) = __builtin_bit_cast(Frag, raw[i]);
+                *(Frag*)(lds + r * PITCH + swz(r, c) * 16) = __builtin_bit_cast(Frag, raw[i]);
             } else {
                 typedef E E4 __attribute__((ext_vector_type(4)));
                 float x[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[e] = raw[i][e];
-                char* d = lds + r * PITCH + (KC ? swz(r, c >> 1) * 16 + (c & 1) * 8 : (unsigned)c * 8);
+                char* d = lds + r * PITCH + swz(r, c >> 1) * 16 + (c & 1) * 8;
 #pragma unroll
                 for (int p = 0; p < 3; ++p) {
                     E4 h;
@@ -245,7 +248,9 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
         } else {
             typedef __attribute__((address_space(3))) s16x4* Q;
             const int sl = lane & 15;
-            const int at = p * PLANE + (ks * 16 + (lane >> 5) * 8 + (sl >> 2)) * PITCH + (r0 + 16 * ((lane >> 4) & 1) + 4 * (sl & 3)) * 2;
+            // depths k and k + 4 have the same swizzle
+            const int k = ks * 16 + (lane >> 5) * 8 + (sl >> 2), c = r0 / 8 + 2 * ((lane >> 4) & 1) + ((sl & 3) >> 1);
+            const int at = p * PLANE + k * PITCH + swz(k, c) * 16 + (sl & 1) * 8;
             const Q q = (Q)((const __attribute__((address_space(3))) char*)lds + at);
             struct { s16x4 a, b; } f;
             f.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(q);
@@ -337,7 +342,7 @@ __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)
 }
 
 template <typename T, int BM, int BN, int WM, int WN, bool KA, bool KB, int EPI>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void gemm_kernel(Gemm<T> g) {
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && sizeof(T) == 4 && KA && KB ? 3 : 2) void gemm_kernel(Gemm<T> g) {
     constexpr int NW = (BM / WM) * (BN / WN), NT = NW * 64, TM = WM / 32, TN = WN / 32;
     typedef Operand<T, BM, NT, KA, false> OA;
     typedef Operand<T, BN, NT, KB, EPI == EPI_GATE_FWD> OB;
@@ -716,6 +721,247 @@ template <typename T, bool KA, bool KB, int EPI> void gemm(Gemm<T>& g, int membe
     }
 }
 
+// ------------------------------------------------------------------------------------------
+// Few rows (at most FEW_ROWS): every product is one launch and reads its weights once, straight into registers -- bound by the weights'
+// bytes and, below a few MB, by the launches.  A block owns 16 or 32 columns of the result, its 16 waves share K, and their sums are
+// joined through LDS in wave order.  v_mfma_f32_16x16x4_f32 takes 16 columns x 4 K-steps of the weights against 16 rows x 4 K-steps of
+// the rows, one value a lane (lane l: column or row l % 16, K-step l / 16): with weights that are K-contiguous a lane loads 16 bytes of
+// its row and the K-steps of a product are whichever the lanes hold; row-contiguous weights need no transposition at all.  Every type is
+// multiplied in fp32 (16-bit K-contiguous operands on v_mfma_f32_16x16x32, which takes the 16 bytes as they are).
+// ------------------------------------------------------------------------------------------
+constexpr int FEW_ROWS = 32, FEW_WAVES = 16;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x4 mfma16(typename V8<cg_h16>::V a, typename V8<cg_h16>::V b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(typename V8<cg_b16>::V a, typename V8<cg_b16>::V b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+template <typename T, int EPI> __device__ __forceinline__ void emit1(const Gemm<T>& g, size_t z, size_t m, int n, float v, float w) {
+    float u, du;
+    const size_t o = z * g.oz + m * g.N + n;
+    if (EPI == EPI_STORE) {
+        g.c[0][z * g.cz + m * g.N + n] = (T)(v + (g.bias[0] ? (float)g.bias[0][z * g.biasz + n] : 0.f));
+    } else if (EPI == EPI_GATE_FWD) {
+        v = (float)(T)(v + (g.bias[0] ? (float)g.bias[0][z * g.biasz + n] : 0.f));
+        w = (float)(T)(w + (g.bias[1] ? (float)g.bias[1][z * g.biasz + n] : 0.f));
+        gate_fn(v, g.gate, u, du);
+        g.o0[o] = (T)(u * w);
+        if (g.o1) g.o1[o] = (T)v, g.o2[o] = (T)w;
+    } else {
+        gate_fn((float)g.i0[o], g.gate, u, du);
+        g.o0[o] = (T)(v * (float)g.i1[o] * du);
+        g.o1[o] = (T)(v * u);
+    }
+}
+
+// MT: blocks of 16 rows; KB: the weights are K-contiguous
+template <typename T, int MT, bool KB, int EPI> __global__ __launch_bounds__(FEW_WAVES * 64) void few_kernel(Gemm<T> g) {
+    constexpr int W = CgT<T>::N, NT = EPI == EPI_GATE_FWD || !KB ? 2 : 1;       // 16-column tiles: gate and value, or even and odd columns
+    constexpr int REGS = MT * NT * 4;
+    typedef typename CgT<T>::V V;
+    __shared__ float sm[FEW_WAVES * REGS * 64];
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, l16 = lane & 15, lk = lane >> 4;
+    const size_t z = blockIdx.y;
+    const int n0 = blockIdx.x * (KB ? 16 : 32), K = (int)g.K;
+    f32x4 acc[MT][NT] = {};
+    for (int s = 0; s < g.nseg; ++s) {
+        const T* x[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const size_t m = i * 16 + l16;
+            x[i] = g.A[s] + z * g.az + (m < g.M ? m : g.M - 1) * g.lda;
+        }
+        if constexpr (KB) {
+            const size_t n = n0 + l16 < g.N ? n0 + l16 : g.N - 1;
+            const T* b[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) b[j] = g.B[j] + z * g.bz + n * g.ldb;
+            constexpr int U = 2, STEP = U * 4 * W;      // a wave takes whole 128-byte lines of its rows
+            auto multiply = [&](const V(&xa)[MT], const V(&ba)[NT]) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        if constexpr (sizeof(T) == 2) {
+                            typedef typename V8<T>::V F;
+                            acc[i][j] = mfma16(__builtin_bit_cast(F, ba[j]), __builtin_bit_cast(F, xa[i]), acc[i][j]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(ba[j][e], xa[i][e], acc[i][j], 0, 0, 0);
+                        }
+                    }
+            };
+            int k0 = wid * STEP;
+#pragma unroll 2
+            for (; k0 + STEP <= K; k0 += FEW_WAVES * STEP) {
+                V xa[U][MT], ba[U][NT];
+#pragma unroll
+                for (int q = 0; q < U; ++q) {
+                    const int k = k0 + (q * 4 + lk) * W;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) ba[q][j] = *(const V*)(b[j] + k);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) xa[q][i] = *(const V*)(x[i] + k);
+                }
+#pragma unroll
+                for (int q = 0; q < U; ++q) multiply(xa[q], ba[q]);
+            }
+            if (k0 < K) {
+#pragma unroll
+                for (int q = 0; q < U; ++q) {
+                    const int k = k0 + (q * 4 + lk) * W;
+                    V xa[MT], ba[NT];
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        const bool in = k + e < K;
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) ba[j][e] = in ? b[j][k + e] : (T)0.f;
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) xa[i][e] = in ? x[i][k + e] : (T)0.f;
+                    }
+                    multiply(xa, ba);
+                }
+            }
+        } else {
+            // lane: columns n0 + 2 l16, + 1 of K-step lk; a pair is one load (moved back inside the row where it would cross its end: what the
+            // columns past the end get is never stored).  U K-steps are in flight at a time: a block's chain of loads is what takes the time.
+            const int n = n0 + 2 * l16, cb = n + 1 < g.N ? n : g.N > 1 ? g.N - 2 : 0;
+            const bool odd = n > cb;
+            const T* b = g.B[s] + z * g.bz + cb;
+            typedef T V2 __attribute__((ext_vector_type(2), aligned(sizeof(T))));
+            // K-step e of a chunk of 4 W is k0 + W lk + e in lane group lk: the rows' values are one 16-byte load a lane
+            constexpr int U = (MT == 1 ? 64 : 32) / (4 * W);
+            for (int k0 = wid * 4 * W * U; k0 < K; k0 += FEW_WAVES * 4 * W * U) {
+                V2 ba[U][W];
+                V xa[U][MT];
+#pragma unroll
+                for (int q = 0; q < U; ++q) {
+                    const int k = k0 + (q * 4 + lk) * W;
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        const T* r = b + (size_t)(k + e < K ? k + e : K - 1) * g.ldb;
+                        if (g.N > 1) ba[q][e] = *(const V2*)r;
+                        else ba[q][e][0] = ba[q][e][1] = *r;
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        if (k + W <= K) {
+                            xa[q][i] = *(const V*)(x[i] + k);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < W; ++e) xa[q][i][e] = k + e < K ? x[i][k + e] : (T)0.f;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < U; ++q)
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        const bool in = k0 + (q * 4 + lk) * W + e < K;
+                        const float w0 = in ? (float)(odd ? ba[q][e][1] : ba[q][e][0]) : 0.f, w1 = in ? (float)ba[q][e][1] : 0.f;
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            acc[i][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(w0, (float)xa[q][i][e], acc[i][0], 0, 0, 0);
+                            acc[i][1] = __builtin_amdgcn_mfma_f32_16x16x4f32(w1, (float)xa[q][i][e], acc[i][1], 0, 0, 0);
+                        }
+                    }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sm[(wid * REGS + (i * NT + j) * 4 + r) * 64 + lane] = acc[i][j][r];
+    __syncthreads();
+    if (tid < REGS * 64) {
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < FEW_WAVES; ++q) v += sm[q * REGS * 64 + tid];
+        sm[tid] = v;        // its own column of the array: nobody else reads it before the barrier
+    }
+    __syncthreads();
+    // column c of the block, row m: tile and register of column (KB: c; else c / 2 of tile c % 2), lane 16 (column / 4) + m % 16
+    constexpr int COLS = KB ? 16 : 32;
+    if (tid < MT * 16 * COLS) {
+        const int m = tid / COLS, c = tid % COLS, i = m >> 4, t = KB ? c : c >> 1, j = KB ? 0 : c & 1;
+        const int at = ((i * NT + j) * 4 + (t & 3)) * 64 + (t >> 2) * 16 + (m & 15);
+        if ((size_t)m < g.M && n0 + c < g.N) emit1<T, EPI>(g, z, m, n0 + c, sm[at], EPI == EPI_GATE_FWD ? sm[at + 4 * 64] : 0.f);
+    }
+}
+
+template <typename T, bool KB, int EPI> void few(const Gemm<T>& g, int members, hipStream_t st) {
+    if (!g.M || !g.N) return;
+    const dim3 grid(cg_div_up(g.N, KB ? 16 : 32), members);
+    if (g.M <= 16) few_kernel<T, 1, KB, EPI><<<grid, FEW_WAVES * 64, 0, st>>>(g);
+    else few_kernel<T, 2, KB, EPI><<<grid, FEW_WAVES * 64, 0, st>>>(g);
+}
+
+// All parameter gradients of few rows in one launch: dW = P^T Q in tiles of 64 x 64 (4 waves of 16 x 64), db = column sums of P.
+template <typename T> struct FewGrads {
+    struct { const T *p, *q; T *dw, *db; int P, Q, tiles_q, first, add_w, add_b; } o[3];
+    int n, M;
+    size_t gs;
+};
+template <typename T> __global__ __launch_bounds__(256) void few_grads_kernel(FewGrads<T> g) {
+    int i = 0;
+    while (i + 1 < g.n && (int)blockIdx.x >= g.o[i + 1].first) ++i;
+    const auto& o = g.o[i];
+    const int tile = blockIdx.x - o.first, lane = threadIdx.x & 63, l16 = lane & 15, lk = lane >> 4;
+    const size_t z = blockIdx.y;
+    const int p0 = tile / o.tiles_q * 64 + (threadIdx.x >> 6) * 16, q0 = tile % o.tiles_q * 64;
+    const T *p = o.p + z * g.M * o.P, *q = o.q + z * g.M * o.Q;
+    const int pc = p0 + l16 < o.P ? p0 + l16 : o.P - 1;
+    int qc[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) qc[j] = q0 + j * 16 + l16 < o.Q ? q0 + j * 16 + l16 : o.Q - 1;
+    f32x4 acc[4] = {};
+    float sum = 0.f;
+    for (int m0 = 0; m0 < g.M; m0 += 8) {
+        float a[2], b[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int m = m0 + h * 4 + lk;
+            const bool in = m < g.M;
+            a[h] = in ? (float)p[(size_t)m * o.P + pc] : 0.f;
+            sum += a[h];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[h][j] = in ? (float)q[(size_t)m * o.Q + qc[j]] : 0.f;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[h], b[h][j], acc[j], 0, 0, 0);
+    }
+    if (o.dw) {
+        T* dw = o.dw + z * g.gs;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = p0 + 4 * lk + r;
+            if (row >= o.P) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int c = q0 + j * 16 + l16;
+                if (c >= o.Q) continue;
+                T* d = dw + (size_t)row * o.Q + c;
+                *d = (T)(o.add_w ? (float)*d + acc[j][r] : acc[j][r]);
+            }
+        }
+    }
+    if (o.db && tile % o.tiles_q == 0) {
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (lk == 0 && p0 + l16 < o.P) {
+            T* d = o.db + z * g.gs + p0 + l16;
+            *d = (T)(o.add_b ? (float)*d + sum : sum);
+        }
+    }
+}
+
 // da, dv from a stored gradient of h (no output projection)
 template <typename T> struct GateBwd { const T *dh, *a, *v; T *da, *dv; size_t n; int gate; };
 template <typename T> __global__ __launch_bounds__(256) void gate_bwd_kernel(GateBwd<T> g) {
@@ -803,13 +1049,16 @@ inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 // scratch of the forward and the backward pass: both use it for one product or sum after the other
 size_t fwd_part(const cg_gated_dims* d, const cg_group* grp) {
     const int nz = grp_n(grp), e = (int)esize(d->dtype);
-    const size_t M = d->rows / nz, p = part_bytes(M, 2 * (size_t)d->F, d->D, nz, 1, e, 2);
+    const size_t M = d->rows / nz;
+    if (M <= FEW_ROWS) return 0;
+    const size_t p = part_bytes(M, 2 * (size_t)d->F, d->D, nz, 1, e, 2);
     const size_t q = d->O ? part_bytes(M, d->O, d->F, nz, 1, e, 1) : 0;
     return p > q ? p : q;
 }
 size_t bwd_part(const cg_gated_dims* d, const cg_group* grp) {
     const int nz = grp_n(grp), e = (int)esize(d->dtype);
     const size_t M = d->rows / nz, F = d->F, D = d->D, O = d->O;
+    if (M <= FEW_ROWS) return 0;
     const size_t n[] = {O ? part_bytes(M, F, O, nz, 1, e, 1) : 0, part_bytes(M, D, 2 * F, nz, 1, e, 1), part_bytes(F, D, M, nz, 1, e, 1),
                         part_bytes(F, D, M, nz, 2, e, 1), O ? part_bytes(O, F, M, nz, 1, e, 1) : 0,
                         (size_t)2 * nz * strips_of(M) * (F > O ? F : O) * 4, (size_t)4 * nz * cg_div_up(M, 64) * F * 4};
@@ -830,7 +1079,9 @@ void fwd(const cg_gated_dims* d, const cg_group* grp, const T* x, const T* wg, c
     g.M = M, g.K = D, g.N = d->F, g.gate = d->gate;
     g.bias[0] = bg, g.bias[1] = bv, g.biasz = gs;
     g.o0 = h, g.o1 = a, g.o2 = v, g.oz = M * F;
-    gemm<T, true, true, EPI_GATE_FWD>(g, nz, part, st);
+    const bool small = M <= FEW_ROWS;
+    if (small) few<T, true, EPI_GATE_FWD>(g, nz, st);
+    else gemm<T, true, true, EPI_GATE_FWD>(g, nz, part, st);
     if (!d->O) return;
     Gemm<T> p = {};
     p.nseg = p.nsel = 1;
@@ -839,7 +1090,8 @@ void fwd(const cg_gated_dims* d, const cg_group* grp, const T* x, const T* wg, c
     p.M = M, p.K = F, p.N = d->O;
     p.bias[0] = bo, p.biasz = gs;
     p.c[0] = y, p.cz = M * d->O;
-    gemm<T, true, true, EPI_STORE>(p, nz, part, st);
+    if (small) few<T, true, EPI_STORE>(p, nz, st);
+    else gemm<T, true, true, EPI_STORE>(p, nz, part, st);
 }
 
 template <typename T>
@@ -848,6 +1100,7 @@ void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, c
          hipStream_t st) {
     const int nz = grp_n(grp);
     const size_t M = d->rows / nz, gs = grp_stride(grp), D = d->D, F = d->F, O = d->O;
+    const bool small = M <= FEW_ROWS;
     if (dx || dwg || dwv || dbg || dbv) {
         if (O) {
             Gemm<T> g = {};
@@ -856,8 +1109,9 @@ void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, c
             g.B[0] = wo, g.bz = gs, g.ldb = F;
             g.M = M, g.K = O, g.N = d->F, g.gate = d->gate;
             g.o0 = da, g.o1 = dv, g.i0 = a, g.i1 = v, g.oz = M * F;
-            if (dbg || dbv) g.sums = part;
-            gemm<T, true, false, EPI_GATE_BWD>(g, nz, part, st);
+            if ((dbg || dbv) && !small) g.sums = part;
+            if (small) few<T, false, EPI_GATE_BWD>(g, nz, st);
+            else gemm<T, true, false, EPI_GATE_BWD>(g, nz, part, st);
             if (g.sums && M) {
                 ColSum<T> c = {{da, dv}, {dbg, dbv}, M, gs, d->F, g.strips, acc >> 3 & 3, part};
                 colsum_join_kernel<T><<<dim3(cg_div_up(F, 32), 1, 2 * nz), 1024, 0, st>>>(c);
@@ -875,7 +1129,25 @@ void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, c
         g.B[0] = wg, g.B[1] = wv, g.bz = gs, g.ldb = D;
         g.M = M, g.K = F, g.N = d->D;
         g.c[0] = dx, g.cz = M * D;
-        gemm<T, true, false, EPI_STORE>(g, nz, part, st);
+        if (small) few<T, false, EPI_STORE>(g, nz, st);
+        else gemm<T, true, false, EPI_STORE>(g, nz, part, st);
+    }
+    if (small) {
+        FewGrads<T> g = {};
+        g.M = (int)M, g.gs = gs;
+        int first = 0;
+        auto add = [&](const T* p, size_t P, const T* q, size_t Q, T* dw, T* db, int bit) {
+            if (!dw && !db) return;
+            auto& o = g.o[g.n++];
+            o.p = p, o.q = q, o.dw = dw, o.db = db, o.P = (int)P, o.Q = (int)Q, o.tiles_q = dw ? (int)cg_div_up(Q, 64) : 1, o.first = first;
+            o.add_w = acc >> bit & 1, o.add_b = acc >> (bit + 3) & 1;
+            first += (int)cg_div_up(P, 64) * o.tiles_q;
+        };
+        add(da, F, x, D, dwg, dbg, 0);
+        add(dv, F, x, D, dwv, dbv, 1);
+        if (O) add(dy, O, h, F, dwo, dbo, 2);
+        if (g.n) few_grads_kernel<T><<<dim3(first, nz), 256, 0, st>>>(g);
+        return;
     }
     auto wgrad = [&](const T* p0, const T* p1, size_t P, const T* q, size_t Q, T* dw0, T* dw1, int accumulate) {
         if (!dw0 && !dw1) return;

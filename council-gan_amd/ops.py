@@ -1924,6 +1924,7 @@ def _rows_like(x, n, c):
 
 
 def _gated_fwd(x, wg, wv, wo, bg, bv, bo, gate, grp, keep):
+    """(y, h, the two projections in x's type: [2, rows, F], only if `keep`)"""
     F, D = wg.shape
     O = wo.shape[0] if wo is not None else 0
     rows = x.numel() // D
@@ -1931,12 +1932,14 @@ def _gated_fwd(x, wg, wv, wo, bg, bv, bo, gate, grp, keep):
     dims = _gated_geom(rows, D, F, O, hip.DT[x.dtype], gate)
     h = _rows_like(x, rows, F)
     y = _rows_like(x, rows, O) if O else None
-    a, v = (torch.empty((2, rows, F), dtype=x.dtype, device=x.device).unbind(0)) if keep else (None, None)
+    av = torch.empty((2, rows, F), dtype=x.dtype, device=x.device) if keep else None
+    a = av.data_ptr() if keep else None
     nws = lib.cg_gated_ff_fwd_workspace(dims, grp)
     ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
     check(lib.cg_gated_ff_fwd(dims, grp, x.data_ptr(), wg.data_ptr(), wv.data_ptr(), _addr(wo), _addr(bg), _addr(bv), _addr(bo),
-                              h.data_ptr(), _addr(a), _addr(v), _addr(y), _addr(ws), nws, _stream_handle()), "cg_gated_ff_fwd")
-    return y, h, a, v
+                              h.data_ptr(), a, a + rows * F * x.element_size() if keep else None, _addr(y), _addr(ws), nws,
+                              _stream_handle()), "cg_gated_ff_fwd")
+    return y, h, av
 
 
 class _GatedFeedForward(torch.autograd.Function):
@@ -1944,8 +1947,8 @@ class _GatedFeedForward(torch.autograd.Function):
     def forward(ctx, x, wg, wv, wo, bg, bv, bo, gate, grp, bufs):
         x = _dense(x)
         params = tuple(None if p is None else p.contiguous() for p in (wg, wv, wo, bg, bv, bo))
-        y, h, a, v = _gated_fwd(x, *params, gate, grp, True)
-        ctx.save_for_backward(x, *params[:3], h if y is not None else None, a, v)
+        y, h, av = _gated_fwd(x, *params, gate, grp, True)
+        ctx.save_for_backward(x, *params[:3], h if y is not None else None, av)
         ctx.biases = params[3:]
         ctx.gate, ctx.grp, ctx.bufs = gate, grp, bufs
         return h if y is None else y
@@ -1953,12 +1956,13 @@ class _GatedFeedForward(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         _once("gated_feed_forward")
-        x, wg, wv, wo, h, a, v = ctx.saved_tensors
+        x, wg, wv, wo, h, av = ctx.saved_tensors
         grp, need = ctx.grp, ctx.needs_input_grad
         F, D = wg.shape
         dy = _dense(dy)
         lib = _lib()
-        dims = _gated_geom(x.numel() // D, D, F, wo.shape[0] if wo is not None else 0, hip.DT[x.dtype], ctx.gate)
+        rows = x.numel() // D
+        dims = _gated_geom(rows, D, F, wo.shape[0] if wo is not None else 0, hip.DT[x.dtype], ctx.gate)
         dx = torch.empty_like(x) if need[0] else None
         outs, ret, acc = [], [], 0
         for i, p in enumerate((wg, wv, wo) + ctx.biases):
@@ -1966,19 +1970,36 @@ class _GatedFeedForward(torch.autograd.Function):
             acc |= on << i
             outs.append(_addr(t))
             ret.append(r)
-        ws = torch.empty(lib.cg_gated_ff_bwd_workspace(dims, grp), dtype=torch.uint8, device=x.device)
-        check(lib.cg_gated_ff_bwd(dims, grp, dy.data_ptr(), x.data_ptr(), wg.data_ptr(), wv.data_ptr(), _addr(wo), _addr(h),
-                                  a.data_ptr(), v.data_ptr(), _addr(dx), *outs, acc, ws.data_ptr(), ws.numel(), _stream_handle()),
+        nws = lib.cg_gated_ff_bwd_workspace(dims, grp)
+        ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
+        a = av.data_ptr()
+        check(lib.cg_gated_ff_bwd(dims, grp, dy.data_ptr(), x.data_ptr(), wg.data_ptr(), wv.data_ptr(), _addr(wo), _addr(h), a,
+                                  a + rows * F * x.element_size(), _addr(dx), *outs, acc, ws.data_ptr(), nws, _stream_handle()),
               "cg_gated_ff_bwd")
         return (dx, *ret, None, None, None)
 
 
-def gated_feed_forward(x, w_gate, w_value, w_out=None, b_gate=None, b_value=None, b_out=None, act="silu"):
-    """(act(x w_gate^T + b_gate) * (x w_value^T + b_value)) w_out^T + b_out over the rows of x; without w_out the gated hidden units
-    themselves.  w_gate / w_value [F, D], w_out [O, F] as nn.Linear keeps them, all in x's type; act: 'silu', 'gelu' (error function)
-    or 'sigmoid'.  Between the two products the hidden units (and, for the backward pass, both projections) are held in x's type.  Under
-    ops.members(n) (fp32) every member's rows take its own parameters."""
-    what = "gated_feed_forward"
+def _gated_args_ok(x, wg, wv, wo, bg, bv, bo, act):
+    """Every condition that _gated_explain names, in one go (a call of one token takes a few microseconds altogether)."""
+    try:
+        dt, dev, shape = x.dtype, x.device, wg.shape
+        F, D = shape
+        if (dt not in hip.DT or act not in hip.GATE or wg.dtype != dt or wv.dtype != dt or wv.shape != shape or wg.device != dev
+                or wv.device != dev or D < 1 or F < 1 or x.shape[1 if x.dim() == 4 else -1] != D):
+            return False
+        if wo is not None and (wo.dim() != 2 or wo.shape[1] != F or wo.shape[0] < 1 or wo.dtype != dt or wo.device != dev):
+            return False
+        if bo is not None and wo is None:
+            return False
+        for b, n in ((bg, F), (bv, F), (bo, wo.shape[0] if wo is not None else 0)):
+            if b is not None and (b.dim() != 1 or b.shape[0] != n or b.dtype != dt or b.device != dev):
+                return False
+        return True
+    except (AttributeError, ValueError, IndexError, TypeError):      # not tensors, or not of this many dimensions
+        return False
+
+
+def _gated_explain(what, x, w_gate, w_value, w_out, b_gate, b_value, b_out, act):
     D = _check_rows(what, x)
     if act not in hip.GATE:
         raise ValueError("%s: act must be one of %s" % (what, ", ".join(hip.GATE)))
@@ -1995,15 +2016,27 @@ def gated_feed_forward(x, w_gate, w_value, w_out=None, b_gate=None, b_value=None
     for name, p, shape in named:
         if p is not None or name == "w_value":
             _check_param(what, name, p, shape, x, (x.dtype,))
+    raise ValueError("%s: bad arguments" % what)
+
+
+def gated_feed_forward(x, w_gate, w_value, w_out=None, b_gate=None, b_value=None, b_out=None, act="silu"):
+    """(act(x w_gate^T + b_gate) * (x w_value^T + b_value)) w_out^T + b_out over the rows of x; without w_out the gated hidden units
+    themselves.  w_gate / w_value [F, D], w_out [O, F] as nn.Linear keeps them, all in x's type; act: 'silu', 'gelu' (error function)
+    or 'sigmoid'.  Between the two products the hidden units (and, for the backward pass, both projections) are held in x's type.  Under
+    ops.members(n) (fp32) every member's rows take its own parameters."""
+    what = "gated_feed_forward"
+    if not _gated_args_ok(x, w_gate, w_value, w_out, b_gate, b_value, b_out, act):
+        _gated_explain(what, x, w_gate, w_value, w_out, b_gate, b_value, b_out, act)
+    D = w_gate.shape[1]
     _check_gpu(what, x)
     params = (w_gate, w_value, w_out, b_gate, b_value, b_out)
     with _dev(x):
-        grp = _member_params(what, x.numel() // D, [p for p in params if p is not None])
+        grp = _member_params(what, x.numel() // D, [p for p in params if p is not None]) if _G.n > 1 else None
         if grp is not None and x.dtype != torch.float32:
             raise hip.HipError("member-batched gated_feed_forward: the pools hold fp32 parameters")
         if torch.is_grad_enabled() and (x.requires_grad or any(p is not None and p.requires_grad for p in params)):
-            return _GatedFeedForward.apply(x, *params, hip.GATE[act], grp, tuple(getattr(p, "_cg_grad", None) for p in params))
-        y, h, _, _ = _gated_fwd(_dense(x), *(None if p is None else p.contiguous() for p in params), hip.GATE[act], grp, False)
+            return _GatedFeedForward.apply(x, *params, hip.GATE[act], grp, tuple([getattr(p, "_cg_grad", None) for p in params]))
+        y, h, _ = _gated_fwd(_dense(x), *(None if p is None else p.contiguous() for p in params), hip.GATE[act], grp, False)
     return h if y is None else y
 
 
