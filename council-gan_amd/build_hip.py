@@ -1,4 +1,5 @@
-"""Builds the gfx950 shared library IN-TREE: council-gan_amd/lib/libcouncilgan_hip.so.
+"""Builds the gfx950 shared library IN-TREE: council-gan_amd/lib/libcouncilgan_hip.so, and the host extension cg_nodes.so beside it
+(autograd nodes of the channel-MLP operators: C++ against torch's headers, no device code).
 
     python council-gan_amd/build_hip.py [--force]
 
@@ -6,9 +7,11 @@ hipcc cross-compiles without a GPU; the .so is git-ignored but travels with gpur
 compiled to its own object (in parallel, cached by a digest of the file, the shared headers and the flags under lib/obj/) and
 the objects are linked: an edit to one kernel file recompiles that file only."""
 import hashlib
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -57,8 +60,37 @@ def _compile(hipcc, src, verbose):
     return obj
 
 
+NODES_SRC = os.path.join(CSRC, "nodes.cpp")
+NODES = os.path.join(OUT_DIR, "cg_nodes.so")
+
+
+def build_nodes(force=False, verbose=True):
+    torch_dir = list(importlib.util.find_spec("torch").submodule_search_locations)[0]      # located, not imported
+    inc, lib = os.path.join(torch_dir, "include"), os.path.join(torch_dir, "lib")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-I/opt/rocm/include", "-I" + inc,
+           "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + sysconfig.get_paths()["include"], NODES_SRC, "-o", NODES,
+           "-L" + lib, "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip"]
+    h = hashlib.sha256(" ".join(cmd).encode())
+    for p in (NODES_SRC, SHARED[-1], os.path.join(torch_dir, "version.py")):
+        h.update(open(p, "rb").read())
+    tag, dig = os.path.join(OBJ_DIR, "cg_nodes.so.stamp"), h.hexdigest()
+    if not force and os.path.exists(NODES) and os.path.exists(tag) and open(tag).read() == dig:
+        return NODES
+    if verbose:
+        print("[build_hip]", " ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    open(tag, "w").write(dig)
+    return NODES
+
+
 def build(force=False, verbose=True):
     os.makedirs(OBJ_DIR, exist_ok=True)
+    build_library(force, verbose)
+    build_nodes(force, verbose)
+    return OUT
+
+
+def build_library(force=False, verbose=True):
     dig = _digest()
     if not force and os.path.exists(OUT) and os.path.exists(STAMP) and open(STAMP).read() == dig:
         return OUT

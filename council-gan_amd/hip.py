@@ -3,6 +3,7 @@
 There is NO fallback: if the shared library is missing, or a kernel is called without a GPU,
 this raises.  The product path never routes through PyTorch compute ops or the oracle."""
 import ctypes
+import importlib.util
 import os
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int8, c_int32, c_int64, c_size_t, c_void_p
 
@@ -221,6 +222,27 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_nodes = None
+NODES_PATH = os.path.join(_HERE, "lib", "cg_nodes.so")
+_NODE_CALLS = ("cg_last_error", "cg_channel_norm_fwd", "cg_channel_norm_bwd_workspace", "cg_channel_norm_bwd", "cg_dropout",
+               "cg_gated_ff_fwd_workspace", "cg_gated_ff_fwd", "cg_gated_ff_bwd_workspace", "cg_gated_ff_bwd")
+
+
+def nodes():
+    """The host extension with the autograd nodes of the channel-MLP operators, bound to the loaded library."""
+    global _nodes
+    if _nodes is None:
+        if not os.path.exists(NODES_PATH):
+            raise HipLibraryMissing("%s not found -- build it with `python council-gan_amd/build_hip.py`" % NODES_PATH)
+        lib = load()
+        spec = importlib.util.spec_from_file_location("cg_nodes", NODES_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind({n: ctypes.cast(getattr(lib, n), c_void_p).value for n in _NODE_CALLS})
+        _nodes = mod
+    return _nodes
 
 
 class HipError(RuntimeError):

@@ -1698,32 +1698,9 @@ def l1_mean(a, b):
 # The channels of a row are dimension 1 of a 4-D tensor (logical NCHW, channels_last: a row is a pixel) and the last dimension of every
 # other tensor.  Inputs of any strides are taken (made dense first); outputs are dense, 4-D ones channels_last.  Sums, statistics and
 # accumulators are fp32, every stored value is rounded once.  Scratch memory comes from torch's caching allocator, per call: a captured
-# graph owns its own, and two graphs share none.  All of them run on the current stream of the tensors' device.
-_ctx_null = contextlib.nullcontext()
-_stream_handle = hip._stream_handle
-
-
-def _dev(t):
-    """Context that makes the tensor's device the current one (the launch, the stream and the scratch follow it)."""
-    if t.is_cuda and t.device.index != torch.cuda.current_device():
-        return torch.cuda.device(t.device)
-    return _ctx_null
-
-
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _dense(t):
-    return t.contiguous(memory_format=CL) if t.dim() == 4 else t.contiguous()
-
-
-def _once(what):
-    # autograd leaves recording on in a backward pass that is itself differentiated (create_graph=True)
-    if torch.is_grad_enabled():
-        raise hip.HipError("%s: the backward pass cannot be differentiated again" % what)
-
-
+# graph owns its own, and two graphs share none.  All of them run on the current stream of the tensors' device.  The calls and their
+# autograd nodes are C++ (csrc/nodes.cpp); a node declines arguments that do not fit, and the functions here say what is wrong with them.
+# Gradients of a parameter that carries `_cg_grad` are added to that buffer; the backward passes cannot be differentiated again.
 def _check_rows(what, x):
     if not isinstance(x, torch.Tensor) or x.dtype not in hip.DT:
         raise ValueError("%s: x must be a float32, float16 or bfloat16 tensor" % what)
@@ -1746,90 +1723,45 @@ def _check_gpu(what, x):
         raise hip.HipError("%s: tensor on %s: the operators run on the GPU only, there is no CPU fallback" % (what, x.device))
 
 
-def _member_params(what, rows, params):
-    """cg_group of the parameters under the current ops.members scope (None outside of one)."""
+def _member_group(what, x, params):
+    """(members, parameter stride) of a call under the current ops.members scope."""
     if _G.n <= 1:
-        return None
+        return 1, 0
     pool = getattr(params[0], '_cg_pool', None)
     if pool is None or any(getattr(p, '_cg_pool', None) is not pool for p in params) or not all(p.is_contiguous() for p in params):
         raise hip.HipError("member-batched %s: the parameters must live in one optim.ParamPool" % what)
+    if x.dtype != torch.float32:
+        raise hip.HipError("member-batched %s: the pools hold fp32 parameters" % what)
+    rows = x.numel() // max(1, _check_rows(what, x))
     if rows % _G.n:
         raise hip.HipError("member-batched %s: %d rows are not %d equal blocks" % (what, rows, _G.n))
-    return _grp(params[0])
-
-
-def _grad_target(p, buf, wanted, grp):
-    """(tensor the backward kernel writes or None, accumulate?, what the backward returns) for one parameter."""
-    if not wanted:
-        return None, 0, None
-    if buf is not None and buf.dtype == p.dtype and buf.is_contiguous():
-        buf._cg_touched = True
-        return buf, 1, None
-    if grp is not None:
-        raise hip.HipError("member-batched backward needs the pool's gradient buffers")
-    g = torch.empty_like(p, memory_format=torch.contiguous_format)
-    return g, 0, g
-
-
-def _channel_norm_fwd(x, w, b, eps, grp, stats):
-    C = w.numel()
-    rows = x.numel() // C
-    y = torch.empty_like(x)
-    st = torch.empty((2, rows), dtype=torch.float32, device=x.device) if stats else None
-    check(_lib().cg_channel_norm_fwd(grp, x.data_ptr(), w.data_ptr(), _addr(b), y.data_ptr(), _addr(st),
-                                     st.data_ptr() + 4 * rows if stats else None, rows, C, hip.DT[x.dtype], hip.DT[w.dtype], eps,
-                                     _stream_handle()), "cg_channel_norm_fwd")
-    return y, st
-
-
-class _ChannelNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w, b, eps, grp, bufs):
-        x, wc, bc = _dense(x), w.contiguous(), None if b is None else b.contiguous()
-        y, st = _channel_norm_fwd(x, wc, bc, eps, grp, True)
-        ctx.save_for_backward(x, wc, st)
-        ctx.grp, ctx.bufs, ctx.b = grp, bufs, bc
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        _once("channel_norm")
-        x, w, st = ctx.saved_tensors
-        need, lib, grp = ctx.needs_input_grad, _lib(), ctx.grp
-        C = w.numel()
-        rows = x.numel() // C
-        dt = hip.DT[x.dtype]
-        dy = _dense(dy)
-        dx = torch.empty_like(x) if need[0] else None
-        dw, aw, rw = _grad_target(w, ctx.bufs[0], need[1], grp)
-        db, ab, rb = _grad_target(ctx.b, ctx.bufs[1], need[2], grp)
-        nws = lib.cg_channel_norm_bwd_workspace(grp, rows, C, dt) if need[1] or need[2] else 0
-        ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
-        sp = st.data_ptr()
-        check(lib.cg_channel_norm_bwd(grp, dy.data_ptr(), x.data_ptr(), w.data_ptr(), sp, sp + 4 * rows, _addr(dx), _addr(dw), _addr(db),
-                                      aw | ab << 1, rows, C, dt, hip.DT[w.dtype], _addr(ws), nws, _stream_handle()),
-              "cg_channel_norm_bwd")
-        return dx, rw, rb, None, None, None
+    return _G.n, pool.stride
 
 
 def channel_norm(x, weight, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the channels of every row (biased variance; ops.layer_norm is the
     reference's norm over C*H*W of a sample).  weight / bias: [C], both in x's type or both fp32.  Under ops.members(n) every
     member's rows take its own parameters."""
-    C = _check_rows("channel_norm", x)
+    n, stride = _member_group("channel_norm", x, [weight] if bias is None else [weight, bias]) if _G.n > 1 else (1, 0)
+    try:
+        y = hip.nodes().channel_norm(x, weight, bias, eps, n, stride, getattr(weight, "_cg_grad", None), getattr(bias, "_cg_grad", None))
+    except TypeError:
+        y = None
+    return _norm_explain(x, weight, bias, eps) if y is None else y
+
+
+def _norm_explain(x, weight, bias, eps):
+    what = "channel_norm"
+    C = _check_rows(what, x)
     if C < 1:
-        raise ValueError("channel_norm: a row needs at least one channel")
+        raise ValueError("%s: a row needs at least one channel" % what)
     if not eps >= 0:
-        raise ValueError("channel_norm: eps must not be negative")
-    _check_param("channel_norm", "weight", weight, (C,), x, (x.dtype, torch.float32))
+        raise ValueError("%s: eps must not be negative" % what)
+    _check_param(what, "weight", weight, (C,), x, (x.dtype, torch.float32))
     if bias is not None:
-        _check_param("channel_norm", "bias", bias, (C,), x, (weight.dtype,))
-    _check_gpu("channel_norm", x)
-    with _dev(x):
-        grp = _member_params("channel_norm", x.numel() // C, [weight] if bias is None else [weight, bias])
-        if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-            return _ChannelNorm.apply(x, weight, bias, float(eps), grp, (getattr(weight, "_cg_grad", None), getattr(bias, "_cg_grad", None)))
-        return _channel_norm_fwd(_dense(x), weight.contiguous(), None if bias is None else bias.contiguous(), float(eps), grp, False)[0]
+        _check_param(what, "bias", bias, (C,), x, (weight.dtype,))
+    _check_gpu(what, x)
+    raise ValueError("%s: bad arguments" % what)
 
 
 def dropout_state(seed, device="cuda"):
@@ -1848,158 +1780,57 @@ def dropout_key(state):
     """The key of one dropout call: a copy of `state` taken on the device, whose step then advances -- captured into a graph, every
     replay draws a new mask."""
     _check_key("dropout_key", state)
-    with _dev(state):
+    with torch.cuda.device(state.device):
         key = torch.empty_like(state)
-        check(_lib().cg_dropout_key(state.data_ptr(), key.data_ptr(), _stream_handle()), "cg_dropout_key")
+        check(_lib().cg_dropout_key(state.data_ptr(), key.data_ptr(), hip._stream_handle()), "cg_dropout_key")
         torch.autograd.graph.increment_version(state)
     return key
-
-
-def _dropout_run(x, res, t, key):
-    y = torch.empty_like(x)
-    check(_lib().cg_dropout(x.data_ptr(), _addr(res), y.data_ptr(), x.numel(), t, key.data_ptr(), hip.DT[x.dtype], _stream_handle()),
-          "cg_dropout")
-    return y
-
-
-class _Dropout(torch.autograd.Function):
-    """The mask is not kept: the backward pass draws it again from the key."""
-
-    @staticmethod
-    def forward(ctx, x, res, t, key):
-        x = _dense(x)
-        ctx.save_for_backward(key)
-        ctx.t = t
-        return _dropout_run(x, None if res is None else _dense(res), t, key)
-
-    @staticmethod
-    def backward(ctx, dy):
-        _once("dropout")
-        (key,) = ctx.saved_tensors
-        dx = _dropout_run(_dense(dy), None, ctx.t, key) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None
 
 
 def dropout(x, p, key, residual=None):
     """residual + x * keep / (1 - p).  keep is drawn from `key` ({seed, step}, ops.dropout_key) and the position of the element alone
     (Philox4x32-10, 16 bits an element), so p counts in steps of 1/65536; a p that would round to 0 or to 1 is refused.  Positions
-    run over the dense form of x (channels_last for a 4-D tensor).  The same key on the same shape gives the same mask; a key must
-    stay unchanged until the backward pass has run."""
-    _check_rows("dropout", x)
+    run over the dense form of x (channels_last for a 4-D tensor).  The same key on the same shape gives the same mask, which the
+    backward pass draws again: a key must stay unchanged until then."""
     if not 0 <= p < 1:
         raise ValueError("dropout: p must be in [0, 1), got %r" % (p,))
     t = int(round(p * 65536))
     if (t == 0 and p > 0) or t > 65535:
         raise ValueError("dropout: p = %r is closer to %d than the step of 1/65536" % (p, 1 if t else 0))
+    try:
+        y = hip.nodes().dropout(x, residual, t, key)
+    except TypeError:
+        y = None
+    return _dropout_explain(x, residual, key) if y is None else y
+
+
+def _dropout_explain(x, residual, key):
+    _check_rows("dropout", x)
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError("dropout: residual must have the shape, type and device of x")
     _check_gpu("dropout", x)
     _check_key("dropout", key)
-    if key.device != x.device:
-        raise ValueError("dropout: key is on %s, x on %s" % (key.device, x.device))
-    with _dev(x):
-        if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-            return _Dropout.apply(x, residual, t, key)
-        return _dropout_run(_dense(x), None if residual is None else _dense(residual), t, key)
+    raise ValueError("dropout: key is on %s, x on %s" % (key.device, x.device))
 
 
-_gated_dims = {}
-
-
-def _gated_geom(rows, D, F, O, dtype, gate):
-    key = (rows, D, F, O, dtype, gate)
-    g = _gated_dims.get(key)
-    if g is None:
-        if len(_gated_dims) > 4096:
-            _gated_dims.clear()
-        g = _gated_dims[key] = byref(hip.GatedDims(rows, D, F, O, dtype, gate, 0))
-    return g
-
-
-def _rows_like(x, n, c):
-    """Dense output of x's rows with c channels."""
-    if x.dim() == 4:
-        return torch.empty((x.shape[0], c, x.shape[2], x.shape[3]), dtype=x.dtype, device=x.device, memory_format=CL)
-    return torch.empty(tuple(x.shape[:-1]) + (c,), dtype=x.dtype, device=x.device)
-
-
-def _gated_fwd(x, wg, wv, wo, bg, bv, bo, gate, grp, keep):
-    """(y, h, the two projections in x's type: [2, rows, F], only if `keep`)"""
-    F, D = wg.shape
-    O = wo.shape[0] if wo is not None else 0
-    rows = x.numel() // D
-    lib = _lib()
-    dims = _gated_geom(rows, D, F, O, hip.DT[x.dtype], gate)
-    h = _rows_like(x, rows, F)
-    y = _rows_like(x, rows, O) if O else None
-    av = torch.empty((2, rows, F), dtype=x.dtype, device=x.device) if keep else None
-    a = av.data_ptr() if keep else None
-    nws = lib.cg_gated_ff_fwd_workspace(dims, grp)
-    ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
-    check(lib.cg_gated_ff_fwd(dims, grp, x.data_ptr(), wg.data_ptr(), wv.data_ptr(), _addr(wo), _addr(bg), _addr(bv), _addr(bo),
-                              h.data_ptr(), a, a + rows * F * x.element_size() if keep else None, _addr(y), _addr(ws), nws,
-                              _stream_handle()), "cg_gated_ff_fwd")
-    return y, h, av
-
-
-class _GatedFeedForward(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, wg, wv, wo, bg, bv, bo, gate, grp, bufs):
-        x = _dense(x)
-        params = tuple(None if p is None else p.contiguous() for p in (wg, wv, wo, bg, bv, bo))
-        y, h, av = _gated_fwd(x, *params, gate, grp, True)
-        ctx.save_for_backward(x, *params[:3], h if y is not None else None, av)
-        ctx.biases = params[3:]
-        ctx.gate, ctx.grp, ctx.bufs = gate, grp, bufs
-        return h if y is None else y
-
-    @staticmethod
-    def backward(ctx, dy):
-        _once("gated_feed_forward")
-        x, wg, wv, wo, h, av = ctx.saved_tensors
-        grp, need = ctx.grp, ctx.needs_input_grad
-        F, D = wg.shape
-        dy = _dense(dy)
-        lib = _lib()
-        rows = x.numel() // D
-        dims = _gated_geom(rows, D, F, wo.shape[0] if wo is not None else 0, hip.DT[x.dtype], ctx.gate)
-        dx = torch.empty_like(x) if need[0] else None
-        outs, ret, acc = [], [], 0
-        for i, p in enumerate((wg, wv, wo) + ctx.biases):
-            t, on, r = _grad_target(p, ctx.bufs[i], p is not None and need[1 + i], grp)
-            acc |= on << i
-            outs.append(_addr(t))
-            ret.append(r)
-        nws = lib.cg_gated_ff_bwd_workspace(dims, grp)
-        ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
-        a = av.data_ptr()
-        check(lib.cg_gated_ff_bwd(dims, grp, dy.data_ptr(), x.data_ptr(), wg.data_ptr(), wv.data_ptr(), _addr(wo), _addr(h), a,
-                                  a + rows * F * x.element_size(), _addr(dx), *outs, acc, ws.data_ptr(), nws, _stream_handle()),
-              "cg_gated_ff_bwd")
-        return (dx, *ret, None, None, None)
-
-
-def _gated_args_ok(x, wg, wv, wo, bg, bv, bo, act):
-    """Every condition that _gated_explain names, in one go (a call of one token takes a few microseconds altogether)."""
+def gated_feed_forward(x, w_gate, w_value, w_out=None, b_gate=None, b_value=None, b_out=None, act="silu"):
+    """(act(x w_gate^T + b_gate) * (x w_value^T + b_value)) w_out^T + b_out over the rows of x; without w_out the gated hidden units
+    themselves.  w_gate / w_value [F, D], w_out [O, F] as nn.Linear keeps them, all in x's type; act: 'silu', 'gelu' (error function)
+    or 'sigmoid'.  Between the two products the hidden units (and, for the backward pass, both projections) are held in x's type.  fp32
+    products are six of three bfloat16 parts of either operand (as exact as an fp32 product; an infinite operand gives NaN).  Under
+    ops.members(n) (fp32) every member's rows take its own parameters."""
+    params = (w_gate, w_value, w_out, b_gate, b_value, b_out)
+    n, stride = _member_group("gated_feed_forward", x, [p for p in params if p is not None]) if _G.n > 1 else (1, 0)
+    bufs = tuple([getattr(p, "_cg_grad", None) for p in params])
     try:
-        dt, dev, shape = x.dtype, x.device, wg.shape
-        F, D = shape
-        if (dt not in hip.DT or act not in hip.GATE or wg.dtype != dt or wv.dtype != dt or wv.shape != shape or wg.device != dev
-                or wv.device != dev or D < 1 or F < 1 or x.shape[1 if x.dim() == 4 else -1] != D):
-            return False
-        if wo is not None and (wo.dim() != 2 or wo.shape[1] != F or wo.shape[0] < 1 or wo.dtype != dt or wo.device != dev):
-            return False
-        if bo is not None and wo is None:
-            return False
-        for b, n in ((bg, F), (bv, F), (bo, wo.shape[0] if wo is not None else 0)):
-            if b is not None and (b.dim() != 1 or b.shape[0] != n or b.dtype != dt or b.device != dev):
-                return False
-        return True
-    except (AttributeError, ValueError, IndexError, TypeError):      # not tensors, or not of this many dimensions
-        return False
+        y = hip.nodes().gated(x, *params, hip.GATE.get(act, -1), n, stride, bufs if any([b is not None for b in bufs]) else None)
+    except TypeError:
+        y = None
+    return _gated_explain(x, *params, act) if y is None else y
 
 
-def _gated_explain(what, x, w_gate, w_value, w_out, b_gate, b_value, b_out, act):
+def _gated_explain(x, w_gate, w_value, w_out, b_gate, b_value, b_out, act):
+    what = "gated_feed_forward"
     D = _check_rows(what, x)
     if act not in hip.GATE:
         raise ValueError("%s: act must be one of %s" % (what, ", ".join(hip.GATE)))
@@ -2016,28 +1847,8 @@ def _gated_explain(what, x, w_gate, w_value, w_out, b_gate, b_value, b_out, act)
     for name, p, shape in named:
         if p is not None or name == "w_value":
             _check_param(what, name, p, shape, x, (x.dtype,))
-    raise ValueError("%s: bad arguments" % what)
-
-
-def gated_feed_forward(x, w_gate, w_value, w_out=None, b_gate=None, b_value=None, b_out=None, act="silu"):
-    """(act(x w_gate^T + b_gate) * (x w_value^T + b_value)) w_out^T + b_out over the rows of x; without w_out the gated hidden units
-    themselves.  w_gate / w_value [F, D], w_out [O, F] as nn.Linear keeps them, all in x's type; act: 'silu', 'gelu' (error function)
-    or 'sigmoid'.  Between the two products the hidden units (and, for the backward pass, both projections) are held in x's type.  Under
-    ops.members(n) (fp32) every member's rows take its own parameters."""
-    what = "gated_feed_forward"
-    if not _gated_args_ok(x, w_gate, w_value, w_out, b_gate, b_value, b_out, act):
-        _gated_explain(what, x, w_gate, w_value, w_out, b_gate, b_value, b_out, act)
-    D = w_gate.shape[1]
     _check_gpu(what, x)
-    params = (w_gate, w_value, w_out, b_gate, b_value, b_out)
-    with _dev(x):
-        grp = _member_params(what, x.numel() // D, [p for p in params if p is not None]) if _G.n > 1 else None
-        if grp is not None and x.dtype != torch.float32:
-            raise hip.HipError("member-batched gated_feed_forward: the pools hold fp32 parameters")
-        if torch.is_grad_enabled() and (x.requires_grad or any(p is not None and p.requires_grad for p in params)):
-            return _GatedFeedForward.apply(x, *params, hip.GATE[act], grp, tuple([getattr(p, "_cg_grad", None) for p in params]))
-        y, h, _ = _gated_fwd(_dense(x), *(None if p is None else p.contiguous() for p in params), hip.GATE[act], grp, False)
-    return h if y is None else y
+    raise ValueError("%s: bad arguments" % what)
 
 
 # ------------------------------------------------------------------------------------------

@@ -511,5 +511,5 @@ def test_backward_passes_are_not_differentiated_again(cga):
     for f in (lambda t: cga.ops.channel_norm(t, w), lambda t: cga.ops.dropout(t, 0.5, key_of(1, 2)),
               lambda t: cga.ops.gated_feed_forward(t, *ps)):
         xl = x.detach().requires_grad_(True)
-        with pytest.raises(cga.hip.HipError, match="cannot be differentiated again"):
+        with pytest.raises(RuntimeError, match="cannot be differentiated again"):
             torch.autograd.grad(f(xl), xl, dy, create_graph=True)
