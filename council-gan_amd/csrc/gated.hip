@@ -168,46 +168,68 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
     static constexpr int BYTES = P * PLANE;
     static_assert(CH >= 1 && ((KC ? ROWS : BK) * CPR) % NT == 0, "every thread has the same number of chunks");
 
-    size_t off[CH];
-    Raw raw[CH];
-    int tid;
+    struct Regs { Raw q[CH]; };
+    size_t off[CH];      // K-contiguous: the row's start
+    int tid, col, shift; // row-contiguous: first row of the thread's chunk, and how far it was moved back to end with the operand
 
     static __device__ __forceinline__ int lrow(int tid, int i) { return (tid + i * NT) / CPR; }
     static __device__ __forceinline__ int lch(int tid) { return tid % CPR; }
     static_assert(NT % CPR == 0, "a thread keeps its chunk column");
 
-    // rows past the end are read from a row that exists: what they give is never stored
+    // Every chunk is loaded whole from inside the operand (of at least W in the contiguous direction), without a branch: rows past the end
+    // come from a row that exists (what they give is never stored), a chunk that would cross the end is moved back, and `store` puts that
+    // right where it matters -- so the loads of two steps stay in flight together.
     __device__ __forceinline__ void init(int t, size_t row0, size_t rows, size_t ld) {
         tid = t;
+        if (KC) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            if (KC) {
+            for (int i = 0; i < CH; ++i) {
                 int j = lrow(tid, i);
                 if (GATE) j = (j >> 6) * 32 + (j & 31);
                 const size_t r = row0 + j;
-                off[i] = (r < rows ? r : rows - 1) * ld + lch(tid) * W;
-            } else {
-                const size_t r = row0 + lch(tid) * W;
-                off[i] = lrow(tid, i) * ld + (r < rows ? r : 0);
+                off[i] = (r < rows ? r : rows - 1) * ld;
+            }
+        } else {
+            const long long r = (long long)row0 + lch(tid) * W, most = (long long)rows - W;
+            col = (int)(r < most ? r : most);
+            shift = (int)(r - col < W ? r - col : 0);
+        }
+    }
+    __device__ __forceinline__ void load(Regs& raw, const T* p0, const T* p1, int k0, int K, size_t ld) const {
+        if (KC) {
+            const int k = k0 + lch(tid) * W, kc = k < K - W ? k : K - W;
+#pragma unroll
+            for (int i = 0; i < CH; ++i) raw.q[i] = *(const Raw*)((GATE && (lrow(tid, i) >> 5 & 1) ? p1 : p0) + off[i] + kc);
+        } else {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const int k = k0 + lrow(tid, i), kc = k < K ? k : K - 1;
+                raw.q[i] = *(const Raw*)(p0 + (size_t)kc * ld + col);
             }
         }
     }
-    // `last`: the operand's last K-step -- everything past K reads as zero, nothing past the tensor is touched.  Elsewhere a chunk may
-    // run over the end of a row into the next one (a row-contiguous operand of at least W rows has it): rows that are never stored.
-    __device__ __forceinline__ void load(const T* p0, const T* p1, size_t k0, size_t K, size_t ld, size_t row0, size_t rows, bool last) {
-        const size_t step = KC ? k0 : k0 * ld;
-        if ((last && (K % BK != 0 || (!KC && rows % W != 0))) || (!KC && rows < W)) {
+    // the elements of a chunk moved down by s, zeros behind (s >= W: all zero)
+    static __device__ __forceinline__ Raw moved(Raw v, int s) {
+        typedef unsigned U4 __attribute__((ext_vector_type(4)));
+        U4 u = __builtin_bit_cast(U4, v);
+        const int h = sizeof(T) == 2 ? s : 2 * s;       // in 16-bit units
+        if (h & 4) u = U4{u[2], u[3], 0, 0};
+        if (h & 2) u = U4{u[1], u[2], u[3], 0};
+        if (h & 1) u = U4{u[0] >> 16 | u[1] << 16, u[1] >> 16 | u[2] << 16, u[2] >> 16 | u[3] << 16, u[3] >> 16};
+        if (h >= 8) u = U4{0, 0, 0, 0};
+        return __builtin_bit_cast(Raw, u);
+    }
+    // what step k0 loaded, with zeros past K
+    __device__ __forceinline__ void fix(Regs& raw, int k0, int K, size_t row0, size_t rows) const {
+        const bool tail = k0 + BK > K;
+        if (KC && tail) {
+            const int k = k0 + lch(tid) * W, s = k - (K - W) > 0 ? k - (K - W) : 0;
 #pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const T* p = (GATE && (lrow(tid, i) >> 5 & 1) ? p1 : p0) + step + off[i];
-                const size_t k = k0 + (KC ? lch(tid) * W : lrow(tid, i));
-                const size_t r = row0 + lch(tid) * W;
+            for (int i = 0; i < CH; ++i) raw.q[i] = moved(raw.q[i], s);
+        }
+        if (!KC && (tail || (rows % W && row0 + ROWS > rows))) {
 #pragma unroll
-                for (int e = 0; e < W; ++e) raw[i][e] = (KC ? k + e < K : k < K && r + e < rows) ? p[e] : (T)0.f;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < CH; ++i) raw[i] = *(const Raw*)((GATE && (lrow(tid, i) >> 5 & 1) ? p1 : p0) + step + off[i]);
+            for (int i = 0; i < CH; ++i) raw.q[i] = moved(raw.q[i], k0 + lrow(tid, i) < K ? shift : W);
         }
     }
     // where 16-byte chunk `chunk` of LDS row `row` lies in it (a row-contiguous operand's LDS rows are its depths)
@@ -215,17 +237,17 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
         if (!KC) return (unsigned)(chunk ^ (ROWS >= 128 ? (row & 3) << 2 : (row >> 1 & 1) << 2));
         return BK == 64 ? (unsigned)(chunk ^ ((row >> 1) & 7)) : (unsigned)(chunk ^ ((row >> 2) & 3));
     }
-    __device__ __forceinline__ void store(char* lds) const {
+    __device__ __forceinline__ void store(char* lds, const Regs& raw) const {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int r = lrow(tid, i), c = lch(tid);
             if constexpr (P == 1) {
-                *(Frag*)(lds + r * PITCH + swz(r, c) * 16) = __builtin_bit_cast(Frag, raw[i]);
+                *(Frag*)(lds + r * PITCH + swz(r, c) * 16) = __builtin_bit_cast(Frag, raw.q[i]);
             } else {
                 typedef E E4 __attribute__((ext_vector_type(4)));
                 float x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = raw[i][e];
+                for (int e = 0; e < 4; ++e) x[e] = raw.q[i][e];
                 char* d = lds + r * PITCH + swz(r, c >> 1) * 16 + (c & 1) * 8;
 #pragma unroll
                 for (int p = 0; p < 3; ++p) {
@@ -341,13 +363,16 @@ __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)
     }
 }
 
+// Loads run two K-steps ahead, in registers: with one block or two on a CU a step of products (a quarter of a microsecond) hides little of
+// a load's latency.  16-bit tiles have two LDS buffers (one barrier a step); the three planes of an fp32 tile leave room for one if two or
+// three blocks are to share a CU.
 template <typename T, int BM, int BN, int WM, int WN, bool KA, bool KB, int EPI>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && sizeof(T) == 4 && KA && KB ? 3 : 2) void gemm_kernel(Gemm<T> g) {
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void gemm_kernel(Gemm<T> g) {
     constexpr int NW = (BM / WM) * (BN / WN), NT = NW * 64, TM = WM / 32, TN = WN / 32;
     typedef Operand<T, BM, NT, KA, false> OA;
     typedef Operand<T, BN, NT, KB, EPI == EPI_GATE_FWD> OB;
-    constexpr int P = OA::P, BK = OA::BK, EP = WN + 4;
-    constexpr int SMEM = OA::BYTES + OB::BYTES > NW * 32 * EP * 4 ? OA::BYTES + OB::BYTES : NW * 32 * EP * 4;
+    constexpr int P = OA::P, BK = OA::BK, EP = WN + 4, BUF = OA::BYTES + OB::BYTES, NBUF = P == 1 ? 2 : 1;
+    constexpr int SMEM = NBUF * BUF > NW * 32 * EP * 4 ? NBUF * BUF : NW * 32 * EP * 4;
     __shared__ __attribute__((aligned(16))) char smem[SMEM];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
 
@@ -365,28 +390,33 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && sizeof(T) 
     OB b;
     a.init(tid, m0, g.M, g.lda);
     b.init(tid, n0, g.N, g.ldb);
-    auto load = [&](int step) {
-        const int s = step >= kt ? 1 : 0, k = step - s * kt;
-        a.load(g.A[g.nseg == 2 ? s : sel] + z * g.az, nullptr, (size_t)k * BK, g.K, g.lda, m0, g.M, k == kt - 1);
-        b.load(g.B[g.nseg == 2 ? s : 0] + z * g.bz, EPI == EPI_GATE_FWD ? g.B[1] + z * g.bz : nullptr, (size_t)k * BK, g.K, g.ldb, n0,
-               g.N, k == kt - 1);
+    typename OA::Regs ra[2];
+    typename OB::Regs rb[2];
+    auto load = [&](int u, int step) {      // behind the end: the last step again
+        step = step < k_end ? step : k_end - 1;
+        const int s = g.nseg == 2 && step >= kt ? 1 : 0, k = step - s * kt;
+        const T* pa = g.nseg == 2 ? (s ? g.A[1] : g.A[0]) : (sel ? g.A[1] : g.A[0]);
+        const T* pb = s ? g.B[1] : g.B[0];
+        a.load(ra[u], pa + z * g.az, nullptr, k * BK, (int)g.K, g.lda);
+        b.load(rb[u], pb + z * g.bz, EPI == EPI_GATE_FWD ? g.B[1] + z * g.bz : nullptr, k * BK, (int)g.K, g.ldb);
     };
-    if (k_begin < k_end) load(k_begin);
-    for (int step = k_begin; step < k_end; ++step) {
-        __syncthreads();
-        a.store(smem);
-        b.store(smem + OA::BYTES);
-        __syncthreads();
-        if (step + 1 < k_end) load(step + 1);
+    auto store = [&](int u, int step, char* to) {
+        const int k0 = (g.nseg == 2 && step >= kt ? step - kt : step) * BK;
+        a.fix(ra[u], k0, (int)g.K, m0, g.M);
+        b.fix(rb[u], k0, (int)g.K, n0, g.N);
+        a.store(to, ra[u]);
+        b.store(to + OA::BYTES, rb[u]);
+    };
+    auto compute = [&](const char* from) {
 #pragma unroll
         for (int ks = 0; ks < BK / 16; ++ks) {
             typename OA::Frag fa[TM][P], fb[TN][P];
 #pragma unroll
             for (int p = 0; p < P; ++p) {
 #pragma unroll
-                for (int i = 0; i < TM; ++i) fa[i][p] = OA::frag(smem, lane, wm + i * 32, ks, p);
+                for (int i = 0; i < TM; ++i) fa[i][p] = OA::frag(from, lane, wm + i * 32, ks, p);
 #pragma unroll
-                for (int j = 0; j < TN; ++j) fb[j][p] = OB::frag(smem + OA::BYTES, lane, wn + j * 32, ks, p);
+                for (int j = 0; j < TN; ++j) fb[j][p] = OB::frag(from + OA::BYTES, lane, wn + j * 32, ks, p);
             }
             // the smaller terms first
 #pragma unroll
@@ -398,8 +428,35 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && sizeof(T) 
 #pragma unroll
                         for (int j = 0; j < TN; ++j) acc[i][j] = mfma(fa[i][p], fb[j][d - p], acc[i][j]);
         }
+    };
+    if (k_begin < k_end) {
+        load(0, k_begin);
+        load(1, k_begin + 1);
+        if constexpr (NBUF == 2) {
+            store(0, k_begin, smem);
+            __syncthreads();
+        }
+        for (int step = k_begin; step < k_end; step += 2) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (step + u >= k_end) break;
+                if constexpr (NBUF == 2) {
+                    load(u, step + u + 2);
+                    compute(smem + u * BUF);
+                    store(u ^ 1, step + u + 1, smem + (u ^ 1) * BUF);
+                    __syncthreads();
+                } else {
+                    __syncthreads();
+                    store(u, step + u, smem);
+                    __syncthreads();
+                    load(u, step + u + 2);
+                    compute(smem);
+                }
+            }
+        }
     }
 
+    // the accumulators leave through LDS
     __syncthreads();
     store_tile<T, EPI, TM, TN>(g, acc, (float*)smem + wid * 32 * EP, lane, m0 + wm, n0 + (EPI == EPI_GATE_FWD ? wn / 2 : wn), z, sel,
                                split, zs);
@@ -659,65 +716,55 @@ template <typename T, int EPI> __global__ __launch_bounds__(256) void join_kerne
     }
 }
 
-// Tile and number of K splits.  `wide` (both operands 16 bit, rows on 16 bytes): 256 x 256 tiles wherever they can fill the chip, split
-// or not; then 128 x 128 tiles (4 waves of 64 x 64), then 64 x 64 (2 waves).  A split takes at least 4 K-steps.  Wide tiles run one a CU
-// in rounds of 256: the number of splits is the one with the least rounds + join (a K-step of a tile takes about 1 us; the partial
-// sums are written and read at about 5 TB/s).  Smaller tiles are split until there are two blocks for every CU.  The number of members
-// is left out: a member's results do not depend on how many run beside it.
-struct Plan { int tile, splits; };
-Plan plan(size_t M, size_t N, size_t K, int nsel, int esz, bool wide) {
-    const size_t bk = esz == 4 ? 32 : 64, steps = (K + bk - 1) / bk, most = steps / 4 > 1 ? steps / 4 : 1;
-    auto tiles = [&](size_t t) { return (size_t)cg_div_up(M, t) * cg_div_up(N, t) * nsel; };
-    if (!M || !N) return {64, 1};
-    if (wide && tiles(256) * most >= 192) {
-        Plan p = {256, 1};
-        double best = 0;
-        for (size_t s = 1; s <= most && s <= 16; ++s) {
-            const double t = (double)((tiles(256) * s + 255) / 256) * (double)((steps + s - 1) / s) + 4 +
-                             (s > 1 ? 2.0 * 4 * s * M * N * nsel / 5e6 + 4 : 0);
-            if (s == 1 || t < best) best = t, p.splits = (int)s;
-        }
-        return p;
-    }
-    const int tile = tiles(128) * most >= 192 ? 128 : 64;
-    const size_t t = tiles(tile), want = (512 + t - 1) / t;
-    return {tile, t >= 256 ? 1 : (int)(want < most ? want : most)};
-}
-size_t part_bytes(size_t M, size_t N, size_t K, int members, int nsel, int esz, int np) {      // N: columns of the product
-    size_t most = 0;
-    for (int wide = 0; wide < (esz == 2 ? 2 : 1); ++wide) {
-        const Plan p = plan(M, N, K, nsel, esz, wide);
-        const size_t n = p.splits > 1 ? (size_t)p.splits * members * nsel * M * np * pad8((int)(N / np)) * 4 : 0;
-        most = n > most ? n : most;
-    }
-    return most;
-}
-
-template <typename T, bool KA, bool KB, int EPI> void gemm(Gemm<T>& g, int members, float* part, hipStream_t st) {
-    if (!g.M || !g.N) return;
-    const int nz = members * g.nsel;
-    const size_t N = (size_t)g.N * planes<EPI>();
-    bool wide = false;
-    if constexpr (sizeof(T) == 2) {
-        wide = g.lda % 8 == 0 && g.ldb % 8 == 0 && g.lda <= 1 << 20 && g.ldb <= 1 << 20 && (!KA || g.K % 8 == 0) && members == 1;
-        for (int i = 0; i < 2; ++i) wide = wide && ((uintptr_t)g.A[i] | (uintptr_t)g.B[i]) % 16 == 0;
-    }
-    const Plan p = plan(g.M, N, g.K * g.nseg, g.nsel, sizeof(T), wide);
-    g.part = part, g.splits = p.splits;
-    g.tiles_m = cg_div_up(g.M, p.tile), g.tiles_n = cg_div_up(N, p.tile);
-    g.strips = 2 * g.tiles_m;
-    if (p.splits > 1) g.sums = nullptr;
-    const dim3 grid((unsigned)g.tiles_m * g.tiles_n, 1, nz * p.splits);
-    if (p.tile == 256) {
-        if constexpr (sizeof(T) == 2) gemm_wide_kernel<T, KA, KB, EPI><<<grid, 512, 0, st>>>(g);
-    } else if (p.tile == 128) {
-        gemm_kernel<T, 128, 128, 64, 64, KA, KB, EPI><<<grid, 256, 0, st>>>(g);
+// Operands narrower than one 16-byte chunk (fewer than 4 or 8 channels or hidden units): one output per thread, or per block where K is long.
+template <typename T, int EPI> __device__ __forceinline__ void emit1(const Gemm<T>& g, size_t z, int sel, size_t m, int n, float v, float w) {
+    float u, du;
+    const size_t o = z * g.oz + m * g.N + n;
+    if (EPI == EPI_STORE) {
+        T* c = g.c[sel] + z * g.cz + m * g.N + n;
+        v += g.bias[0] ? (float)g.bias[0][z * g.biasz + n] : 0.f;
+        *c = (T)(g.accumulate >> sel & 1 ? (float)*c + v : v);
+    } else if (EPI == EPI_GATE_FWD) {
+        v = (float)(T)(v + (g.bias[0] ? (float)g.bias[0][z * g.biasz + n] : 0.f));
+        w = (float)(T)(w + (g.bias[1] ? (float)g.bias[1][z * g.biasz + n] : 0.f));
+        gate_fn(v, g.gate, u, du);
+        g.o0[o] = (T)(u * w);
+        if (g.o1) g.o1[o] = (T)v, g.o2[o] = (T)w;
     } else {
-        gemm_kernel<T, 64, 64, 32, 64, KA, KB, EPI><<<grid, 128, 0, st>>>(g);
+        gate_fn((float)g.i0[o], g.gate, u, du);
+        g.o0[o] = (T)(v * (float)g.i1[o] * du);
+        g.o1[o] = (T)(v * u);
     }
-    if (p.splits > 1) {
-        const size_t nb = (g.M * (pad8(g.N) / 8) * nz + 255) / 256;
-        join_kernel<T, EPI><<<(unsigned)(nb < 4096 ? nb : 4096), 256, 0, st>>>(g, nz);
+}
+template <typename T, bool KA, bool KB, int EPI, bool BLOCK> __global__ __launch_bounds__(256) void narrow_kernel(Gemm<T> g) {
+    __shared__ float sm[2][4];
+    const int sel = blockIdx.z % g.nsel;
+    const size_t z = blockIdx.z / g.nsel, total = g.M * g.N, per = BLOCK ? 1 : 256;
+    for (size_t o0 = blockIdx.x * per; o0 < total; o0 += gridDim.x * per) {
+        const size_t o = BLOCK ? o0 : o0 + threadIdx.x, m = o / g.N;
+        const int n = (int)(o % g.N);
+        float v = 0.f, w = 0.f;
+        if (o < total)
+            for (int s = 0; s < g.nseg; ++s) {
+                const T* a = (g.nseg == 2 ? g.A[s] : g.A[sel]) + z * g.az + (KA ? m * g.lda : m);
+                const T* b = g.B[EPI == EPI_GATE_FWD ? 0 : s] + z * g.bz + (KB ? n * g.ldb : n);
+                const T* b1 = g.B[1] + z * g.bz + n * g.ldb;
+                for (size_t k = BLOCK ? threadIdx.x : 0; k < g.K; k += BLOCK ? 256 : 1) {
+                    const float x = (float)a[KA ? k : k * g.lda];
+                    v += x * (float)b[KB ? k : k * g.ldb];
+                    if (EPI == EPI_GATE_FWD) w += x * (float)b1[k];
+                }
+            }
+        if (BLOCK) {
+            v = wave_sum(v);
+            w = wave_sum(w);
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) sm[0][threadIdx.x >> 6] = v, sm[1][threadIdx.x >> 6] = w;
+            __syncthreads();
+            v = sm[0][0] + sm[0][1] + sm[0][2] + sm[0][3];
+            w = sm[1][0] + sm[1][1] + sm[1][2] + sm[1][3];
+        }
+        if (o < total && (!BLOCK || threadIdx.x == 0)) emit1<T, EPI>(g, z, sel, m, n, v, w);
     }
 }
 
@@ -737,24 +784,6 @@ __device__ __forceinline__ f32x4 mfma16(typename V8<cg_h16>::V a, typename V8<cg
 }
 __device__ __forceinline__ f32x4 mfma16(typename V8<cg_b16>::V a, typename V8<cg_b16>::V b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
-template <typename T, int EPI> __device__ __forceinline__ void emit1(const Gemm<T>& g, size_t z, size_t m, int n, float v, float w) {
-    float u, du;
-    const size_t o = z * g.oz + m * g.N + n;
-    if (EPI == EPI_STORE) {
-        g.c[0][z * g.cz + m * g.N + n] = (T)(v + (g.bias[0] ? (float)g.bias[0][z * g.biasz + n] : 0.f));
-    } else if (EPI == EPI_GATE_FWD) {
-        v = (float)(T)(v + (g.bias[0] ? (float)g.bias[0][z * g.biasz + n] : 0.f));
-        w = (float)(T)(w + (g.bias[1] ? (float)g.bias[1][z * g.biasz + n] : 0.f));
-        gate_fn(v, g.gate, u, du);
-        g.o0[o] = (T)(u * w);
-        if (g.o1) g.o1[o] = (T)v, g.o2[o] = (T)w;
-    } else {
-        gate_fn((float)g.i0[o], g.gate, u, du);
-        g.o0[o] = (T)(v * (float)g.i1[o] * du);
-        g.o1[o] = (T)(v * u);
-    }
 }
 
 // MT: blocks of 16 rows; KB: the weights are K-contiguous
@@ -890,7 +919,7 @@ template <typename T, int MT, bool KB, int EPI> __global__ __launch_bounds__(FEW
     if (tid < MT * 16 * COLS) {
         const int m = tid / COLS, c = tid % COLS, i = m >> 4, t = KB ? c : c >> 1, j = KB ? 0 : c & 1;
         const int at = ((i * NT + j) * 4 + (t & 3)) * 64 + (t >> 2) * 16 + (m & 15);
-        if ((size_t)m < g.M && n0 + c < g.N) emit1<T, EPI>(g, z, m, n0 + c, sm[at], EPI == EPI_GATE_FWD ? sm[at + 4 * 64] : 0.f);
+        if ((size_t)m < g.M && n0 + c < g.N) emit1<T, EPI>(g, z, 0, m, n0 + c, sm[at], EPI == EPI_GATE_FWD ? sm[at + 4 * 64] : 0.f);
     }
 }
 
@@ -962,6 +991,74 @@ template <typename T> __global__ __launch_bounds__(256) void few_grads_kernel(Fe
     }
 }
 
+// Tile and number of K splits.  `wide` (both operands 16 bit, rows on 16 bytes): 256 x 256 tiles wherever they can fill the chip, split
+// or not; then 128 x 128 tiles (4 waves of 64 x 64), then 64 x 64 (2 waves).  A split takes at least 4 K-steps.  The number of splits is
+// the one with the least time by this account: tiles run in rounds of as many as fit the chip (256 wide ones, 512 of the others), a K-step
+// takes about 1 us in a wide tile, 0.6 us in another (more where two share a CU, which the rounds do not show), and joining costs a
+// launch, the lost fusions of the epilogue, and the partial sums' way out and back at about 5 TB/s.  The number of members is left out: a
+// member's results do not depend on how many run beside it.
+struct Plan { int tile, splits; };
+Plan plan(size_t M, size_t N, size_t K, int nsel, int esz, bool wide) {
+    const size_t bk = esz == 4 ? 32 : 64, steps = (K + bk - 1) / bk, most = steps / 4 > 1 ? steps / 4 : 1;
+    auto tiles = [&](size_t t) { return (size_t)cg_div_up(M, t) * cg_div_up(N, t) * nsel; };
+    if (!M || !N) return {64, 1};
+    const int tile = wide && tiles(256) * most >= 192 ? 256 : tiles(128) * most >= 192 ? 128 : 64;
+    const size_t t = tiles(tile), slots = tile == 256 ? 256 : 512;
+    const double step_us = tile == 256 ? 1.0 : tile == 128 ? 0.6 : 0.4;
+    Plan p = {tile, 1};
+    double best = 0;
+    for (size_t s = 1; s <= most && s <= 64; ++s) {
+        const double us = (double)((t * s + slots - 1) / slots) * (double)((steps + s - 1) / s) * step_us +
+                          (s > 1 ? 8.0 + 2.0 * 4 * s * M * N * nsel / 5e6 : 0);
+        if (s == 1 || us < best) best = us, p.splits = (int)s;
+    }
+    return p;
+}
+size_t part_bytes(size_t M, size_t N, size_t K, int members, int nsel, int esz, int np) {      // N: columns of the product
+    size_t most = 0;
+    for (int wide = 0; wide < (esz == 2 ? 2 : 1); ++wide) {
+        const Plan p = plan(M, N, K, nsel, esz, wide);
+        const size_t n = p.splits > 1 ? (size_t)p.splits * members * nsel * M * np * pad8((int)(N / np)) * 4 : 0;
+        most = n > most ? n : most;
+    }
+    return most;
+}
+
+template <typename T, bool KA, bool KB, int EPI> void gemm(Gemm<T>& g, int members, float* part, hipStream_t st) {
+    if (!g.M || !g.N) return;
+    const int nz = members * g.nsel;
+    const size_t N = (size_t)g.N * planes<EPI>();
+    constexpr size_t W = CgT<T>::N;
+    if ((KA ? g.K : g.M) < W || (KB ? g.K : (size_t)g.N) < W) {
+        g.sums = nullptr;
+        if (!g.K || g.K > 64) narrow_kernel<T, KA, KB, EPI, true><<<dim3((unsigned)(g.M * g.N < 65536 ? g.M * g.N : 65536), 1, nz), 256, 0, st>>>(g);
+        else narrow_kernel<T, KA, KB, EPI, false><<<dim3((unsigned)(g.M * g.N < 1 << 24 ? (g.M * g.N + 255) / 256 : 65536), 1, nz), 256, 0, st>>>(g);
+        return;
+    }
+    bool wide = false;
+    if constexpr (sizeof(T) == 2) {
+        wide = g.lda % 8 == 0 && g.ldb % 8 == 0 && g.lda <= 1 << 20 && g.ldb <= 1 << 20 && (!KA || g.K % 8 == 0) && members == 1;
+        for (int i = 0; i < 2; ++i) wide = wide && ((uintptr_t)g.A[i] | (uintptr_t)g.B[i]) % 16 == 0;
+    }
+    const Plan p = plan(g.M, N, g.K * g.nseg, g.nsel, sizeof(T), wide);
+    g.part = part, g.splits = p.splits;
+    g.tiles_m = cg_div_up(g.M, p.tile), g.tiles_n = cg_div_up(N, p.tile);
+    g.strips = 2 * g.tiles_m;
+    if (p.splits > 1) g.sums = nullptr;
+    const dim3 grid((unsigned)g.tiles_m * g.tiles_n, 1, nz * p.splits);
+    if (p.tile == 256) {
+        if constexpr (sizeof(T) == 2) gemm_wide_kernel<T, KA, KB, EPI><<<grid, 512, 0, st>>>(g);
+    } else if (p.tile == 128) {
+        gemm_kernel<T, 128, 128, 64, 64, KA, KB, EPI><<<grid, 256, 0, st>>>(g);
+    } else {
+        gemm_kernel<T, 64, 64, 32, 64, KA, KB, EPI><<<grid, 128, 0, st>>>(g);
+    }
+    if (p.splits > 1) {
+        const size_t nb = (g.M * (pad8(g.N) / 8) * nz + 255) / 256;
+        join_kernel<T, EPI><<<(unsigned)(nb < 4096 ? nb : 4096), 256, 0, st>>>(g, nz);
+    }
+}
+
 // da, dv from a stored gradient of h (no output projection)
 template <typename T> struct GateBwd { const T *dh, *a, *v; T *da, *dv; size_t n; int gate; };
 template <typename T> __global__ __launch_bounds__(256) void gate_bwd_kernel(GateBwd<T> g) {
@@ -984,7 +1081,7 @@ template <typename T> __global__ __launch_bounds__(256) void gate_bwd_kernel(Gat
 }
 
 // Column sums of one or two [rows][C] tensors (bias gradients): strips of rows, then the strips in turn.
-constexpr int STRIP_ROWS = 128, MAX_STRIPS = 256;
+constexpr int STRIP_ROWS = 32, MAX_STRIPS = 512;
 inline int strips_of(size_t rows) {
     const size_t s = (rows + STRIP_ROWS - 1) / STRIP_ROWS;
     return (int)(s < 1 ? 1 : s > MAX_STRIPS ? MAX_STRIPS : s);
@@ -1000,6 +1097,7 @@ template <typename T> __global__ __launch_bounds__(256) void colsum_part_kernel(
     const T* p = g.p[blockIdx.z & 1];
     float s[N] = {}, v[N];
     if (p && c < g.C)
+#pragma unroll 8
         for (size_t r = r0 + w; r < r1; r += 4) {
             cg_load<T>(p + (z * g.rows + r) * g.C + c, g.C - c, v);
 #pragma unroll
@@ -1038,7 +1136,7 @@ template <typename T> __global__ __launch_bounds__(1024) void colsum_join_kernel
 }
 
 bool dims_ok(const cg_gated_dims* d, const cg_group* grp) {
-    return d && d->rows >= 0 && d->rows % grp_n(grp) == 0 && d->D > 0 && d->F > 0 && d->O >= 0 &&
+    return d && d->rows >= 0 && d->rows < INT32_MAX && d->rows % grp_n(grp) == 0 && d->D > 0 && d->F > 0 && d->O >= 0 &&
            (d->dtype == CG_DT_F32 || d->dtype == CG_DT_F16 || d->dtype == CG_DT_BF16) && d->gate >= 0 && d->gate <= CG_GATE_SIGMOID &&
            (grp_n(grp) == 1 || d->dtype == CG_DT_F32);
 }

@@ -222,7 +222,8 @@ def test_dropout_refuses_a_key_that_changed_before_the_backward_pass(cga):
 GATED_SIZES = [(1, 1, 1, 1, True), (1, 8, 32, 8, False), (1, 256, 704, 256, False), (2, 64, 96, 32, True), (3, 5, 7, 9, True), (16, 256, 1024, 256, True),
                (17, 33, 65, 31, True), (48, 128, 200, 128, False), (64, 64, 64, 64, True), (65, 100, 130, 70, False),
                (127, 257, 129, 255, True), (130, 96, 352, 0, True), (200, 72, 40, 0, False), (300, 512, 384, 512, True),
-               (1000, 40, 24, 16, True), (517, 320, 264, 328, False), (2300, 128, 256, 128, True)]
+               (1000, 40, 24, 16, True), (90, 3, 200, 5, True), (90, 200, 3, 70, True), (70, 65, 70, 2, False), (300, 1, 2, 0, True),
+               (517, 320, 264, 328, False), (2300, 128, 256, 128, True)]
 
 
 def gated_inputs(g, rows, D, F, O, bias, dtype):
