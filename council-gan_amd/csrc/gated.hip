@@ -36,13 +36,44 @@ template <typename T> struct Gemm {
     int splits, tiles_m, tiles_n;
 };
 
-__device__ __forceinline__ void gate_fn(float a, int gate, float& u, float& du) {
+// u = act(a), du = act'(a).  The epilogues evaluate this for every hidden unit, where the library's expf, division and erfcf took 16 of the
+// 39 us of a 777 x 2816 gate product: exponentials are one v_exp_f32 (of 2^x), reciprocals one v_rcp_f32, each good to an ulp.
+//   fp32: the argument's product with log2 e is carried in two parts (its rounding alone would cost |a| half ulps of the result);
+//   16 bit: one part -- the error stays below 2^-17 for every |a| that does not end in 0 or 1.
+// gelu, 16 bit: erfc(z) = t exp(-z^2 + P(t)), t = 1 / (1 + z / 2), with the degree-9 Chebyshev fit of Press et al., Numerical Recipes,
+// section 6.2 (relative error 1.2e-7 everywhere); fp32: the library's erfcf.
+template <bool FP32> __device__ __forceinline__ float exp_neg(float a) {       // exp(-a)
+    constexpr float L = 1.44269504f, L_LO = 1.92596299e-8f;                     // log2 e
+    if (!FP32) return __builtin_amdgcn_exp2f(-a * L);
+    const float c = __builtin_amdgcn_fmed3f(a, -104.f, 104.f), h = -c * L, l = -(__builtin_fmaf(c, L, h) + c * L_LO);
+    const float e = __builtin_amdgcn_exp2f(h);
+    return __builtin_fmaf(e, l * 0.69314718f, e);
+}
+template <bool FP32> __device__ __forceinline__ void gate_fn(float a, int gate, float& u, float& du) {
     if (gate == CG_GATE_GELU) {
-        const float cdf = 0.5f * erfcf(-a * 0.70710678118654752f);
-        u = a * cdf;
-        du = cdf + a * expf(-0.5f * a * a) * 0.39894228040143268f;
+        if (FP32) {
+            const float cdf = 0.5f * erfcf(-a * 0.70710678f);
+            u = a * cdf;
+            du = cdf + a * exp_neg<true>(0.5f * a * a) * 0.39894228f;
+        } else {
+            const float z = fabsf(a) * 0.70710678f, t = __builtin_amdgcn_rcpf(1.f + 0.5f * z), g = exp_neg<false>(0.5f * a * a);
+            float q = 0.17087277f;
+            q = __builtin_fmaf(q, t, -0.82215223f);
+            q = __builtin_fmaf(q, t, 1.48851587f);
+            q = __builtin_fmaf(q, t, -1.13520398f);
+            q = __builtin_fmaf(q, t, 0.27886807f);
+            q = __builtin_fmaf(q, t, -0.18628806f);
+            q = __builtin_fmaf(q, t, 0.09678418f);
+            q = __builtin_fmaf(q, t, 0.37409196f);
+            q = __builtin_fmaf(q, t, 1.00002368f);
+            q = __builtin_fmaf(q, t, -1.26551223f);
+            const float tail = 0.5f * t * g * exp_neg<false>(-q), cdf = a > 0.f ? 1.f - tail : tail;      // 0.5 erfc(|z|)
+            u = a * cdf;
+            du = cdf + a * g * 0.39894228f;
+        }
     } else {
-        const float s = 1.f / (1.f + expf(-a));
+        float s = __builtin_amdgcn_rcpf(1.f + exp_neg<FP32>(a));
+        if (FP32) s = a != a ? a : s;       // the clamped exponential hides a NaN
         u = gate == CG_GATE_SILU ? a * s : s;
         du = gate == CG_GATE_SILU ? s + u * (1.f - s) : s * (1.f - s);
     }
@@ -104,7 +135,7 @@ __device__ __forceinline__ void emit(const Gemm<T>& g, size_t z, int sel, size_t
             // act(a) v is formed from the rounded a, v: the values the backward pass differentiates
             v[i] = (float)(T)(v[i] + b.x[i]);
             w[i] = (float)(T)(w[i] + b.y[i]);
-            gate_fn(v[i], g.gate, u, du);
+            gate_fn<sizeof(T) == 4>(v[i], g.gate, u, du);
             h[i] = u * w[i];
         }
         cg_store<T, 8>(g.o0 + o, left, h);
@@ -115,7 +146,7 @@ __device__ __forceinline__ void emit(const Gemm<T>& g, size_t z, int sel, size_t
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            gate_fn((float)row.x.q[i / W][i % W], g.gate, u, du);
+            gate_fn<sizeof(T) == 4>((float)row.x.q[i / W][i % W], g.gate, u, du);
             w[i] = v[i] * u;
             v[i] = v[i] * (float)row.y.q[i / W][i % W] * du;
             sx[i] += v[i];
@@ -363,11 +394,12 @@ __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)
     }
 }
 
-// Loads run two K-steps ahead, in registers: with one block or two on a CU a step of products (a quarter of a microsecond) hides little of
-// a load's latency.  16-bit tiles have two LDS buffers (one barrier a step); the three planes of an fp32 tile leave room for one if two or
-// three blocks are to share a CU.
+// 16-bit tiles: loads run two K-steps ahead, in registers, and there are two LDS buffers (one barrier a step) -- with one block or two on a
+// CU a step of products, a quarter of a microsecond, hides little of a load's latency.  An fp32 step has six times the products and three
+// planes to hold: one buffer, one step ahead, and three blocks on a CU where the registers allow it (K-contiguous operands: 510 us instead
+// of 577 for the gate product of 65536 x 256 x 1024 with two).
 template <typename T, int BM, int BN, int WM, int WN, bool KA, bool KB, int EPI>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void gemm_kernel(Gemm<T> g) {
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && sizeof(T) == 4 && KA && KB ? 3 : 2) void gemm_kernel(Gemm<T> g) {
     constexpr int NW = (BM / WM) * (BN / WN), NT = NW * 64, TM = WM / 32, TN = WN / 32;
     typedef Operand<T, BM, NT, KA, false> OA;
     typedef Operand<T, BN, NT, KB, EPI == EPI_GATE_FWD> OB;
@@ -390,8 +422,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void gemm_kernel(Gem
     OB b;
     a.init(tid, m0, g.M, g.lda);
     b.init(tid, n0, g.N, g.ldb);
-    typename OA::Regs ra[2];
-    typename OB::Regs rb[2];
+    typename OA::Regs ra[NBUF];
+    typename OB::Regs rb[NBUF];
     auto load = [&](int u, int step) {      // behind the end: the last step again
         step = step < k_end ? step : k_end - 1;
         const int s = g.nseg == 2 && step >= kt ? 1 : 0, k = step - s * kt;
@@ -431,27 +463,27 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void gemm_kernel(Gem
     };
     if (k_begin < k_end) {
         load(0, k_begin);
-        load(1, k_begin + 1);
         if constexpr (NBUF == 2) {
+            load(1, k_begin + 1);
             store(0, k_begin, smem);
             __syncthreads();
-        }
-        for (int step = k_begin; step < k_end; step += 2) {
+            for (int step = k_begin; step < k_end; step += 2) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (step + u >= k_end) break;
-                if constexpr (NBUF == 2) {
+                for (int u = 0; u < 2; ++u) {
+                    if (step + u >= k_end) break;
                     load(u, step + u + 2);
                     compute(smem + u * BUF);
                     store(u ^ 1, step + u + 1, smem + (u ^ 1) * BUF);
                     __syncthreads();
-                } else {
-                    __syncthreads();
-                    store(u, step + u, smem);
-                    __syncthreads();
-                    load(u, step + u + 2);
-                    compute(smem);
                 }
+            }
+        } else {
+            for (int step = k_begin; step < k_end; ++step) {
+                __syncthreads();
+                store(0, step, smem);
+                __syncthreads();
+                load(0, step + 1);
+                compute(smem);
             }
         }
     }
@@ -727,11 +759,11 @@ template <typename T, int EPI> __device__ __forceinline__ void emit1(const Gemm<
     } else if (EPI == EPI_GATE_FWD) {
         v = (float)(T)(v + (g.bias[0] ? (float)g.bias[0][z * g.biasz + n] : 0.f));
         w = (float)(T)(w + (g.bias[1] ? (float)g.bias[1][z * g.biasz + n] : 0.f));
-        gate_fn(v, g.gate, u, du);
+        gate_fn<sizeof(T) == 4>(v, g.gate, u, du);
         g.o0[o] = (T)(u * w);
         if (g.o1) g.o1[o] = (T)v, g.o2[o] = (T)w;
     } else {
-        gate_fn((float)g.i0[o], g.gate, u, du);
+        gate_fn<sizeof(T) == 4>((float)g.i0[o], g.gate, u, du);
         g.o0[o] = (T)(v * (float)g.i1[o] * du);
         g.o1[o] = (T)(v * u);
     }
@@ -1071,7 +1103,7 @@ template <typename T> __global__ __launch_bounds__(256) void gate_bwd_kernel(Gat
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float u, du;
-            gate_fn(a[e], g.gate, u, du);
+            gate_fn<sizeof(T) == 4>(a[e], g.gate, u, du);
             a[e] = d[e] * v[e] * du;
             v[e] = d[e] * u;
         }
