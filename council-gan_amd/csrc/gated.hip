@@ -29,7 +29,7 @@ template <typename T> struct Gemm {
     int gate;
     T *o0, *o1, *o2;          // EPI_GATE_FWD: h, a, v; EPI_GATE_BWD: da, dv
     const T *i0, *i1;         // EPI_GATE_BWD: a, v
-    size_t oz;
+    int ld0, ldf;             // pitch of h; of a, v, da, dv.  A pitch beyond N is a multiple of 8 and its columns get zeros
     float* sums;              // EPI_GATE_BWD, or NULL: column sums of da and dv over a wave's rows, [member][2][strips][N]
     int strips;
     float* part;              // splits > 1: partial sums [split][member * nsel + sel][M][planes][NP]
@@ -99,9 +99,9 @@ template <typename T, int EPI> __device__ __forceinline__ void fetch_row(const G
     const int left = m < g.M ? g.N - n : 0;
     if (EPI == EPI_STORE && (g.accumulate >> sel & 1)) get<T>(r.x, g.c[sel] + z * g.cz + m * g.N + n, left);
     if (EPI == EPI_GATE_BWD) {
-        const size_t o = z * g.oz + m * g.N + n;
-        get<T>(r.x, g.i0 + o, left);
-        get<T>(r.y, g.i1 + o, left);
+        const size_t o = (z * g.M + m) * g.ldf + n;
+        get<T>(r.x, g.i0 + o, m < g.M ? g.ldf - n : 0);
+        get<T>(r.y, g.i1 + o, m < g.M ? g.ldf - n : 0);
     }
 }
 struct Bias { float x[8], y[8]; };
@@ -126,7 +126,7 @@ __device__ __forceinline__ void emit(const Gemm<T>& g, size_t z, int sel, size_t
         cg_store<T, 8>(g.c[sel] + z * g.cz + m * g.N + n, left, v);
         return;
     }
-    const size_t o = z * g.oz + m * g.N + n;
+    const size_t of = (z * g.M + m) * g.ldf + n;
     float u, du;
     if (EPI == EPI_GATE_FWD) {
         float h[8];
@@ -136,24 +136,24 @@ __device__ __forceinline__ void emit(const Gemm<T>& g, size_t z, int sel, size_t
             v[i] = (float)(T)(v[i] + b.x[i]);
             w[i] = (float)(T)(w[i] + b.y[i]);
             gate_fn<sizeof(T) == 4>(v[i], g.gate, u, du);
-            h[i] = u * w[i];
+            h[i] = i < left ? u * w[i] : 0.f;
         }
-        cg_store<T, 8>(g.o0 + o, left, h);
+        cg_store<T, 8>(g.o0 + (z * g.M + m) * g.ld0 + n, g.ld0 - n, h);
         if (g.o1) {
-            cg_store<T, 8>(g.o1 + o, left, v);
-            cg_store<T, 8>(g.o2 + o, left, w);
+            cg_store<T, 8>(g.o1 + of, g.ldf - n, v);
+            cg_store<T, 8>(g.o2 + of, g.ldf - n, w);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             gate_fn<sizeof(T) == 4>((float)row.x.q[i / W][i % W], g.gate, u, du);
-            w[i] = v[i] * u;
-            v[i] = v[i] * (float)row.y.q[i / W][i % W] * du;
+            w[i] = i < left ? v[i] * u : 0.f;
+            v[i] = i < left ? v[i] * (float)row.y.q[i / W][i % W] * du : 0.f;
             sx[i] += v[i];
             sy[i] += w[i];
         }
-        cg_store<T, 8>(g.o0 + o, left, v);
-        cg_store<T, 8>(g.o1 + o, left, w);
+        cg_store<T, 8>(g.o0 + of, g.ldf - n, v);
+        cg_store<T, 8>(g.o1 + of, g.ldf - n, w);
     }
 }
 
@@ -200,7 +200,7 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
     static_assert(CH >= 1 && ((KC ? ROWS : BK) * CPR) % NT == 0, "every thread has the same number of chunks");
 
     struct Regs { Raw q[CH]; };
-    size_t off[CH];      // K-contiguous: the row's start
+    size_t off[CH];      // the row's start (K-contiguous), the chunk of K-step 0 (row-contiguous)
     int tid, col, shift; // row-contiguous: first row of the thread's chunk, and how far it was moved back to end with the operand
 
     static __device__ __forceinline__ int lrow(int tid, int i) { return (tid + i * NT) / CPR; }
@@ -224,6 +224,8 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
             const long long r = (long long)row0 + lch(tid) * W, most = (long long)rows - W;
             col = (int)(r < most ? r : most);
             shift = (int)(r - col < W ? r - col : 0);
+#pragma unroll
+            for (int i = 0; i < CH; ++i) off[i] = lrow(tid, i) * ld + col;
         }
     }
     __device__ __forceinline__ void load(Regs& raw, const T* p0, const T* p1, int k0, int K, size_t ld) const {
@@ -232,11 +234,17 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
 #pragma unroll
             for (int i = 0; i < CH; ++i) raw.q[i] = *(const Raw*)((GATE && (lrow(tid, i) >> 5 & 1) ? p1 : p0) + off[i] + kc);
         } else {
+            const T* p[CH];
 #pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const int k = k0 + lrow(tid, i), kc = k < K ? k : K - 1;
-                raw.q[i] = *(const Raw*)(p0 + (size_t)kc * ld + col);
-            }
+            for (int i = 0; i < CH; ++i) p[i] = p0 + (size_t)k0 * ld + off[i];
+            if (k0 + BK > K)
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    const int k = k0 + lrow(tid, i);
+                    p[i] = p0 + (size_t)(k < K ? k : K - 1) * ld + col;
+                }
+#pragma unroll
+            for (int i = 0; i < CH; ++i) raw.q[i] = *(const Raw*)p[i];
         }
     }
     // the elements of a chunk moved down by s, zeros behind (s >= W: all zero)
@@ -394,17 +402,15 @@ __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)
     }
 }
 
-// 16-bit tiles: loads run two K-steps ahead, in registers, and there are two LDS buffers (one barrier a step) -- with one block or two on a
-// CU a step of products, a quarter of a microsecond, hides little of a load's latency.  An fp32 step has six times the products and three
-// planes to hold: one buffer, one step ahead, and three blocks on a CU where the registers allow it (K-contiguous operands: 510 us instead
-// of 577 for the gate product of 65536 x 256 x 1024 with two).
+// One LDS buffer, loads one K-step ahead in registers, and three blocks on a CU where the registers allow it (K-contiguous operands: 510 us
+// instead of 577 for the gate product of 65536 x 256 x 1024 with two blocks and two steps ahead).
 template <typename T, int BM, int BN, int WM, int WN, bool KA, bool KB, int EPI>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && sizeof(T) == 4 && KA && KB ? 3 : 2) void gemm_kernel(Gemm<T> g) {
     constexpr int NW = (BM / WM) * (BN / WN), NT = NW * 64, TM = WM / 32, TN = WN / 32;
     typedef Operand<T, BM, NT, KA, false> OA;
     typedef Operand<T, BN, NT, KB, EPI == EPI_GATE_FWD> OB;
-    constexpr int P = OA::P, BK = OA::BK, EP = WN + 4, BUF = OA::BYTES + OB::BYTES, NBUF = P == 1 ? 2 : 1;
-    constexpr int SMEM = NBUF * BUF > NW * 32 * EP * 4 ? NBUF * BUF : NW * 32 * EP * 4;
+    constexpr int P = OA::P, BK = OA::BK, EP = WN + 4, BUF = OA::BYTES + OB::BYTES;
+    constexpr int SMEM = BUF > NW * 32 * EP * 4 ? BUF : NW * 32 * EP * 4;
     __shared__ __attribute__((aligned(16))) char smem[SMEM];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
 
@@ -422,22 +428,22 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && sizeof(T) 
     OB b;
     a.init(tid, m0, g.M, g.lda);
     b.init(tid, n0, g.N, g.ldb);
-    typename OA::Regs ra[NBUF];
-    typename OB::Regs rb[NBUF];
-    auto load = [&](int u, int step) {      // behind the end: the last step again
+    typename OA::Regs ra;
+    typename OB::Regs rb;
+    auto load = [&](int step) {      // behind the end: the last step again
         step = step < k_end ? step : k_end - 1;
         const int s = g.nseg == 2 && step >= kt ? 1 : 0, k = step - s * kt;
         const T* pa = g.nseg == 2 ? (s ? g.A[1] : g.A[0]) : (sel ? g.A[1] : g.A[0]);
         const T* pb = s ? g.B[1] : g.B[0];
-        a.load(ra[u], pa + z * g.az, nullptr, k * BK, (int)g.K, g.lda);
-        b.load(rb[u], pb + z * g.bz, EPI == EPI_GATE_FWD ? g.B[1] + z * g.bz : nullptr, k * BK, (int)g.K, g.ldb);
+        a.load(ra, pa + z * g.az, nullptr, k * BK, (int)g.K, g.lda);
+        b.load(rb, pb + z * g.bz, EPI == EPI_GATE_FWD ? g.B[1] + z * g.bz : nullptr, k * BK, (int)g.K, g.ldb);
     };
-    auto store = [&](int u, int step, char* to) {
+    auto store = [&](int step) {
         const int k0 = (g.nseg == 2 && step >= kt ? step - kt : step) * BK;
-        a.fix(ra[u], k0, (int)g.K, m0, g.M);
-        b.fix(rb[u], k0, (int)g.K, n0, g.N);
-        a.store(to, ra[u]);
-        b.store(to + OA::BYTES, rb[u]);
+        a.fix(ra, k0, (int)g.K, m0, g.M);
+        b.fix(rb, k0, (int)g.K, n0, g.N);
+        a.store(smem, ra);
+        b.store(smem + OA::BYTES, rb);
     };
     auto compute = [&](const char* from) {
 #pragma unroll
@@ -462,29 +468,13 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && sizeof(T) 
         }
     };
     if (k_begin < k_end) {
-        load(0, k_begin);
-        if constexpr (NBUF == 2) {
-            load(1, k_begin + 1);
-            store(0, k_begin, smem);
+        load(k_begin);
+        for (int step = k_begin; step < k_end; ++step) {
             __syncthreads();
-            for (int step = k_begin; step < k_end; step += 2) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    if (step + u >= k_end) break;
-                    load(u, step + u + 2);
-                    compute(smem + u * BUF);
-                    store(u ^ 1, step + u + 1, smem + (u ^ 1) * BUF);
-                    __syncthreads();
-                }
-            }
-        } else {
-            for (int step = k_begin; step < k_end; ++step) {
-                __syncthreads();
-                store(0, step, smem);
-                __syncthreads();
-                load(0, step + 1);
-                compute(smem);
-            }
+            store(step);
+            __syncthreads();
+            load(step + 1);
+            compute(smem);
         }
     }
 
@@ -495,7 +485,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && sizeof(T) 
 }
 
 // ------------------------------------------------------------------------------------------
-// The same product of 16-bit operands in 256 x 256 tiles, for operands whose rows start on 16 bytes: 8 waves of 128 x 64, one block a CU.
+// The same product of 16-bit operands, whose rows start on 16 bytes and end in zeros where they are longer than K: 256 x 256 tiles, 8 waves
+// of 128 x 64, one block a CU; 128 x 128 tiles, 4 waves of 64 x 64, two blocks a CU.
 //
 // The tiles come straight from memory into LDS (buffer_load_dwordx4 ... lds: 64 lanes x 16 bytes to consecutive LDS addresses, no
 // registers on the way), so the swizzle is in the address that each lane fetches: chunk c of row r of a K-contiguous tile lies at
@@ -518,9 +509,10 @@ __device__ __forceinline__ void dma16(rsrc4 rsrc, unsigned lds, unsigned off) {
 
 constexpr unsigned OUTSIDE = 0x80000000u, MOST = 0x7fffff00u;      // an offset past every bound; the largest bound
 
-template <typename T, bool KC> struct WideOperand {
+template <typename T, int ROWS, bool KC> struct WideOperand {
     typedef typename V8<T>::V Frag;
-    static constexpr int ROWS = 256, BK = 64, PIECES = 4, BYTES = ROWS * BK * 2;
+    static constexpr int BK = 64, PIECES = 4, BYTES = ROWS * BK * 2;      // ROWS / 32 waves
+    static constexpr int PITCH = ROWS * 2, LANES = ROWS / 8;               // row-contiguous: bytes and lanes of a depth
     unsigned off[PIECES];
     int k_of[2];     // K-contiguous: first k of the lane's chunk in even and odd pieces
     // the tile to fill next: its address, the bytes and the K-steps from there to the operand's end, the bytes to the next tile
@@ -528,7 +520,7 @@ template <typename T, bool KC> struct WideOperand {
     long long left, step;
     int room;
 
-    // wave w fills LDS rows w * 32 + 8 i .. (K-contiguous) or depths w * 8 + 2 i .. (row-contiguous)
+    // wave w fills LDS rows w * 32 + 8 i .. (K-contiguous) or its share of the 64 depths, 64 / LANES at a time (row-contiguous)
     __device__ __forceinline__ void init(int w, int lane, size_t ld) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
@@ -537,7 +529,7 @@ template <typename T, bool KC> struct WideOperand {
                 k_of[i & 1] = c * 8;
                 off[i] = (unsigned)((w * 32 + i * 8 + row) * ld * 2) + c * 16;
             } else {
-                const int k = w * 8 + i * 2 + (lane >> 5), c = (lane & 31) ^ ((k & 3) << 2);
+                const int k = (w * PIECES + i) * (64 / LANES) + lane / LANES, c = lane % LANES ^ ((k & 3) << 2);
                 off[i] = (unsigned)(k * ld * 2) + c * 16;
             }
         }
@@ -577,7 +569,7 @@ template <typename T, bool KC> struct WideOperand {
     static __device__ __forceinline__ unsigned addr(int lane, int r0, int j) {
         if (KC) return (r0 + j * 32 + (lane & 31)) * 128 + (((lane >> 5) ^ ((lane >> 1) & 7)) << 4);
         const int sl = lane & 15, c = (r0 + j * 32) / 8 + ((lane >> 4) & 1) * 2 + ((sl & 3) >> 1);
-        return ((lane >> 5) * 8 + (sl >> 2)) * 512 + ((c ^ ((sl >> 2) << 2)) << 4) + (sl & 1) * 8;
+        return ((lane >> 5) * 8 + (sl >> 2)) * PITCH + ((c ^ ((sl >> 2) << 2)) << 4) + (sl & 1) * 8;
     }
     static __device__ __forceinline__ Frag frag(unsigned base, unsigned a, int ks) {
         if constexpr (KC) {
@@ -585,26 +577,26 @@ template <typename T, bool KC> struct WideOperand {
         } else {
             typedef __attribute__((address_space(3))) s16x4* Q;
             struct { s16x4 a, b; } f;
-            f.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Q)(size_t)(base + a + ks * 8192));
-            f.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Q)(size_t)(base + a + ks * 8192 + 2048));
+            f.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Q)(size_t)(base + a + ks * 16 * PITCH));
+            f.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Q)(size_t)(base + a + ks * 16 * PITCH + 4 * PITCH));
             return __builtin_bit_cast(Frag, f);
         }
     }
 };
 
-template <typename T, bool KA, bool KB, int EPI> __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(Gemm<T> g) {
-    typedef WideOperand<T, KA> OA;
-    typedef WideOperand<T, KB> OB;
-    constexpr int TM = 4, TN = 2, BK = OA::BK, A_BUFS = 3, LDS_B = A_BUFS * OA::BYTES;
+template <typename T, int TILE, bool KA, bool KB, int EPI> __global__ __launch_bounds__(TILE * 2, 2) void gemm_wide_kernel(Gemm<T> g) {
+    typedef WideOperand<T, TILE, KA> OA;
+    typedef WideOperand<T, TILE, KB> OB;
+    constexpr int TM = TILE / 64, TN = 2, WN = TILE / 64, BK = OA::BK, A_BUFS = 3, LDS_B = A_BUFS * OA::BYTES;
     __shared__ __attribute__((aligned(1024))) char smem[A_BUFS * OA::BYTES + 2 * OB::BYTES];
     const unsigned lds = (unsigned)(size_t)(__attribute__((address_space(3))) char*)smem;
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     size_t m0;
     int n0;
-    tile_origin<256, EPI == EPI_GATE_FWD ? 128 : 256>(g.tiles_m, g.tiles_n, m0, n0);
+    tile_origin<TILE, EPI == EPI_GATE_FWD ? TILE / 2 : TILE>(g.tiles_m, g.tiles_n, m0, n0);
     const int split = blockIdx.z % g.splits, zs = blockIdx.z / g.splits, sel = zs % g.nsel;
     const size_t z = zs / g.nsel;
-    const int wm = (wid >> 2) * 128, wn = (wid & 3) * 64;
+    const int wm = wid / WN * (TILE / 2), wn = wid % WN * 64;
 
     f32x16 acc[TM][TN] = {};
     const int kt = (int)((g.K + BK - 1) / BK), all = kt * g.nseg;
@@ -650,16 +642,16 @@ template <typename T, bool KA, bool KB, int EPI> __global__ __launch_bounds__(51
 #pragma unroll
         for (int i = 0; i < TM; ++i) fa[f][i] = OA::frag(la, aa[i], ks);
     };
-    auto multiply = [&](int f, int i0) {       // two of the four row blocks
+    auto multiply = [&](int f, int half) {       // half of the row blocks
 #pragma unroll
-        for (int i = i0; i < i0 + 2; ++i)
+        for (int i = half * TM / 2; i < (half + 1) * TM / 2; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[i][j] = mfma(fa[f][i], fb[f][j], acc[i][j]);
     };
-    constexpr int READS = TM * (KA ? 1 : 2) + TN * (KB ? 1 : 2), PER = (READS + 3) / 4;
-    auto interleave = [&]() {       // the reads of the next step spread between the first four products of this one
+    constexpr int READS = TM * (KA ? 1 : 2) + TN * (KB ? 1 : 2), PER = (READS + TM - 1) / TM;
+    auto interleave = [&]() {       // the reads of the next step spread between the first TM (half the) products of this one
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < TM; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
         }
@@ -694,13 +686,13 @@ template <typename T, bool KA, bool KB, int EPI> __global__ __launch_bounds__(51
             const rsrc4 ra = a.window(), rb = b.window();
             read(a0, b0, 1, 1), multiply(0, 0), interleave();
             fill_a(ra, 0, a2);
-            multiply(0, 2);
+            multiply(0, 1);
             fill_a(ra, 1, a2);
             read(a0, b0, 2, 0), multiply(1, 0), interleave();
             fill_a(ra, 2, a2);
-            multiply(1, 2);
+            multiply(1, 1);
             fill_a(ra, 3, a2);
-            read(a0, b0, 3, 1), multiply(0, 0), interleave(), multiply(0, 2);
+            read(a0, b0, 3, 1), multiply(0, 0), interleave(), multiply(0, 1);
             // all but the newest four loads (A of the step after the next) have landed
             asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
@@ -710,7 +702,7 @@ template <typename T, bool KA, bool KB, int EPI> __global__ __launch_bounds__(51
             read(a1, b1, 0, 0), multiply(1, 0), interleave();
             b.fill(rb, 2, b0, wid);
             b.fill(rb, 3, b0, wid);
-            multiply(1, 2);
+            multiply(1, 1);
             const unsigned ta = a0, tb = b0;
             a0 = a1, a1 = a2, a2 = ta, b0 = b1, b1 = tb;
         }
@@ -751,7 +743,7 @@ template <typename T, int EPI> __global__ __launch_bounds__(256) void join_kerne
 // Operands narrower than one 16-byte chunk (fewer than 4 or 8 channels or hidden units): one output per thread, or per block where K is long.
 template <typename T, int EPI> __device__ __forceinline__ void emit1(const Gemm<T>& g, size_t z, int sel, size_t m, int n, float v, float w) {
     float u, du;
-    const size_t o = z * g.oz + m * g.N + n;
+    const size_t o = (z * g.M + m) * g.ldf + n;
     if (EPI == EPI_STORE) {
         T* c = g.c[sel] + z * g.cz + m * g.N + n;
         v += g.bias[0] ? (float)g.bias[0][z * g.biasz + n] : 0.f;
@@ -760,7 +752,7 @@ template <typename T, int EPI> __device__ __forceinline__ void emit1(const Gemm<
         v = (float)(T)(v + (g.bias[0] ? (float)g.bias[0][z * g.biasz + n] : 0.f));
         w = (float)(T)(w + (g.bias[1] ? (float)g.bias[1][z * g.biasz + n] : 0.f));
         gate_fn<sizeof(T) == 4>(v, g.gate, u, du);
-        g.o0[o] = (T)(u * w);
+        g.o0[(z * g.M + m) * g.ld0 + n] = (T)(u * w);
         if (g.o1) g.o1[o] = (T)v, g.o2[o] = (T)w;
     } else {
         gate_fn<sizeof(T) == 4>((float)g.i0[o], g.gate, u, du);
@@ -964,7 +956,7 @@ template <typename T, bool KB, int EPI> void few(const Gemm<T>& g, int members, 
 
 // All parameter gradients of few rows in one launch: dW = P^T Q in tiles of 64 x 64 (4 waves of 16 x 64), db = column sums of P.
 template <typename T> struct FewGrads {
-    struct { const T *p, *q; T *dw, *db; int P, Q, tiles_q, first, add_w, add_b; } o[3];
+    struct { const T *p, *q; T *dw, *db; int P, Q, ldp, ldq, tiles_q, first, add_w, add_b; } o[3];
     int n, M;
     size_t gs;
 };
@@ -975,7 +967,7 @@ template <typename T> __global__ __launch_bounds__(256) void few_grads_kernel(Fe
     const int tile = blockIdx.x - o.first, lane = threadIdx.x & 63, l16 = lane & 15, lk = lane >> 4;
     const size_t z = blockIdx.y;
     const int p0 = tile / o.tiles_q * 64 + (threadIdx.x >> 6) * 16, q0 = tile % o.tiles_q * 64;
-    const T *p = o.p + z * g.M * o.P, *q = o.q + z * g.M * o.Q;
+    const T *p = o.p + z * g.M * o.ldp, *q = o.q + z * g.M * o.ldq;
     const int pc = p0 + l16 < o.P ? p0 + l16 : o.P - 1;
     int qc[4];
 #pragma unroll
@@ -988,10 +980,10 @@ template <typename T> __global__ __launch_bounds__(256) void few_grads_kernel(Fe
         for (int h = 0; h < 2; ++h) {
             const int m = m0 + h * 4 + lk;
             const bool in = m < g.M;
-            a[h] = in ? (float)p[(size_t)m * o.P + pc] : 0.f;
+            a[h] = in ? (float)p[(size_t)m * o.ldp + pc] : 0.f;
             sum += a[h];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[h][j] = in ? (float)q[(size_t)m * o.Q + qc[j]] : 0.f;
+            for (int j = 0; j < 4; ++j) b[h][j] = in ? (float)q[(size_t)m * o.ldq + qc[j]] : 0.f;
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -1023,18 +1015,17 @@ template <typename T> __global__ __launch_bounds__(256) void few_grads_kernel(Fe
     }
 }
 
-// Tile and number of K splits.  `wide` (both operands 16 bit, rows on 16 bytes): 256 x 256 tiles wherever they can fill the chip, split
-// or not; then 128 x 128 tiles (4 waves of 64 x 64), then 64 x 64 (2 waves).  A split takes at least 4 K-steps.  The number of splits is
-// the one with the least time by this account: tiles run in rounds of as many as fit the chip (256 wide ones, 512 of the others), a K-step
-// takes about 1 us in a wide tile, 0.6 us in another (more where two share a CU, which the rounds do not show), and joining costs a
-// launch, the lost fusions of the epilogue, and the partial sums' way out and back at about 5 TB/s.  The number of members is left out: a
-// member's results do not depend on how many run beside it.
+// Tile and number of K splits.  16 bit: 256 x 256 tiles wherever they can fill the chip, split or not, then 128 x 128; fp32: 128 x 128 (4
+// waves of 64 x 64), then 64 x 64 (2 waves).  A split takes at least 4 K-steps.  The number of splits is the one with the least time by this
+// account: tiles run in rounds of as many as fit the chip (256 of the largest, 512 of the others), a K-step takes about 1 us in a 256 x 256
+// tile, 0.6 and 0.4 us in the others, and joining costs a launch, the lost fusions of the epilogue, and the partial sums' way out and
+// back at about 5 TB/s.  The number of members is left out: a member's results do not depend on how many run beside it.
 struct Plan { int tile, splits; };
-Plan plan(size_t M, size_t N, size_t K, int nsel, int esz, bool wide) {
+Plan plan(size_t M, size_t N, size_t K, int nsel, int esz) {
     const size_t bk = esz == 4 ? 32 : 64, steps = (K + bk - 1) / bk, most = steps / 4 > 1 ? steps / 4 : 1;
     auto tiles = [&](size_t t) { return (size_t)cg_div_up(M, t) * cg_div_up(N, t) * nsel; };
-    if (!M || !N) return {64, 1};
-    const int tile = wide && tiles(256) * most >= 192 ? 256 : tiles(128) * most >= 192 ? 128 : 64;
+    if (!M || !N) return {128, 1};
+    const int tile = esz == 2 ? (tiles(256) * most >= 192 ? 256 : 128) : (tiles(128) * most >= 192 ? 128 : 64);
     const size_t t = tiles(tile), slots = tile == 256 ? 256 : 512;
     const double step_us = tile == 256 ? 1.0 : tile == 128 ? 0.6 : 0.4;
     Plan p = {tile, 1};
@@ -1047,43 +1038,35 @@ Plan plan(size_t M, size_t N, size_t K, int nsel, int esz, bool wide) {
     return p;
 }
 size_t part_bytes(size_t M, size_t N, size_t K, int members, int nsel, int esz, int np) {      // N: columns of the product
-    size_t most = 0;
-    for (int wide = 0; wide < (esz == 2 ? 2 : 1); ++wide) {
-        const Plan p = plan(M, N, K, nsel, esz, wide);
-        const size_t n = p.splits > 1 ? (size_t)p.splits * members * nsel * M * np * pad8((int)(N / np)) * 4 : 0;
-        most = n > most ? n : most;
-    }
-    return most;
+    const Plan p = plan(M, N, K, nsel, esz);
+    return p.splits > 1 ? (size_t)p.splits * members * nsel * M * np * pad8((int)(N / np)) * 4 : 0;
 }
 
 template <typename T, bool KA, bool KB, int EPI> void gemm(Gemm<T>& g, int members, float* part, hipStream_t st) {
     if (!g.M || !g.N) return;
     const int nz = members * g.nsel;
     const size_t N = (size_t)g.N * planes<EPI>();
-    constexpr size_t W = CgT<T>::N;
-    if ((KA ? g.K : g.M) < W || (KB ? g.K : (size_t)g.N) < W) {
-        g.sums = nullptr;
-        if (!g.K || g.K > 64) narrow_kernel<T, KA, KB, EPI, true><<<dim3((unsigned)(g.M * g.N < 65536 ? g.M * g.N : 65536), 1, nz), 256, 0, st>>>(g);
-        else narrow_kernel<T, KA, KB, EPI, false><<<dim3((unsigned)(g.M * g.N < 1 << 24 ? (g.M * g.N + 255) / 256 : 65536), 1, nz), 256, 0, st>>>(g);
-        return;
+    if constexpr (sizeof(T) == 4) {
+        constexpr size_t W = CgT<T>::N;
+        if ((KA ? g.K : g.M) < W || (KB ? g.K : (size_t)g.N) < W) {
+            g.sums = nullptr;
+            if (!g.K || g.K > 64) narrow_kernel<T, KA, KB, EPI, true><<<dim3((unsigned)(g.M * g.N < 65536 ? g.M * g.N : 65536), 1, nz), 256, 0, st>>>(g);
+            else narrow_kernel<T, KA, KB, EPI, false><<<dim3((unsigned)(g.M * g.N < 1 << 24 ? (g.M * g.N + 255) / 256 : 65536), 1, nz), 256, 0, st>>>(g);
+            return;
+        }
     }
-    bool wide = false;
-    if constexpr (sizeof(T) == 2) {
-        wide = g.lda % 8 == 0 && g.ldb % 8 == 0 && g.lda <= 1 << 20 && g.ldb <= 1 << 20 && (!KA || g.K % 8 == 0) && members == 1;
-        for (int i = 0; i < 2; ++i) wide = wide && ((uintptr_t)g.A[i] | (uintptr_t)g.B[i]) % 16 == 0;
-    }
-    const Plan p = plan(g.M, N, g.K * g.nseg, g.nsel, sizeof(T), wide);
+    const Plan p = plan(g.M, N, g.K * g.nseg, g.nsel, sizeof(T));
     g.part = part, g.splits = p.splits;
     g.tiles_m = cg_div_up(g.M, p.tile), g.tiles_n = cg_div_up(N, p.tile);
     g.strips = 2 * g.tiles_m;
     if (p.splits > 1) g.sums = nullptr;
     const dim3 grid((unsigned)g.tiles_m * g.tiles_n, 1, nz * p.splits);
-    if (p.tile == 256) {
-        if constexpr (sizeof(T) == 2) gemm_wide_kernel<T, KA, KB, EPI><<<grid, 512, 0, st>>>(g);
-    } else if (p.tile == 128) {
-        gemm_kernel<T, 128, 128, 64, 64, KA, KB, EPI><<<grid, 256, 0, st>>>(g);
+    if constexpr (sizeof(T) == 2) {
+        if (p.tile == 256) gemm_wide_kernel<T, 256, KA, KB, EPI><<<grid, 512, 0, st>>>(g);
+        else gemm_wide_kernel<T, 128, KA, KB, EPI><<<grid, 256, 0, st>>>(g);
     } else {
-        gemm_kernel<T, 64, 64, 32, 64, KA, KB, EPI><<<grid, 128, 0, st>>>(g);
+        if (p.tile == 128) gemm_kernel<T, 128, 128, 64, 64, KA, KB, EPI><<<grid, 256, 0, st>>>(g);
+        else gemm_kernel<T, 64, 64, 32, 64, KA, KB, EPI><<<grid, 128, 0, st>>>(g);
     }
     if (p.splits > 1) {
         const size_t nb = (g.M * (pad8(g.N) / 8) * nz + 255) / 256;
@@ -1092,14 +1075,16 @@ template <typename T, bool KA, bool KB, int EPI> void gemm(Gemm<T>& g, int membe
 }
 
 // da, dv from a stored gradient of h (no output projection)
-template <typename T> struct GateBwd { const T *dh, *a, *v; T *da, *dv; size_t n; int gate; };
+template <typename T> struct GateBwd { const T *dh, *a, *v; T *da, *dv; size_t rows; int F, ldf, gate; };
 template <typename T> __global__ __launch_bounds__(256) void gate_bwd_kernel(GateBwd<T> g) {
-    for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 8; i < g.n; i += (size_t)gridDim.x * 2048) {
-        const int left = g.n - i < 8 ? (int)(g.n - i) : 8;
+    const size_t per = g.ldf / 8;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < g.rows * per; i += (size_t)gridDim.x * 256) {
+        const size_t m = i / per;
+        const int n = (int)(i % per) * 8;
         float d[8], a[8], v[8];
-        cg_load<T, 8>(g.dh + i, left, d);
-        cg_load<T, 8>(g.a + i, left, a);
-        cg_load<T, 8>(g.v + i, left, v);
+        cg_load<T, 8>(g.dh + m * g.F + n, g.F - n, d);       // zeros behind F: da and dv end in zeros
+        cg_load<T, 8>(g.a + m * g.ldf + n, g.F - n, a);
+        cg_load<T, 8>(g.v + m * g.ldf + n, g.F - n, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float u, du;
@@ -1107,8 +1092,8 @@ template <typename T> __global__ __launch_bounds__(256) void gate_bwd_kernel(Gat
             a[e] = d[e] * v[e] * du;
             v[e] = d[e] * u;
         }
-        cg_store<T, 8>(g.da + i, left, a);
-        cg_store<T, 8>(g.dv + i, left, v);
+        cg_store<T, 8>(g.da + m * g.ldf + n, 8, a);
+        cg_store<T, 8>(g.dv + m * g.ldf + n, 8, v);
     }
 }
 
@@ -1118,7 +1103,7 @@ inline int strips_of(size_t rows) {
     const size_t s = (rows + STRIP_ROWS - 1) / STRIP_ROWS;
     return (int)(s < 1 ? 1 : s > MAX_STRIPS ? MAX_STRIPS : s);
 }
-template <typename T> struct ColSum { const T* p[2]; T* out[2]; size_t rows, zs; int C, strips, accumulate; float* part; };
+template <typename T> struct ColSum { const T* p[2]; T* out[2]; size_t rows, zs; int C, ld, strips, accumulate; float* part; };
 
 template <typename T> __global__ __launch_bounds__(256) void colsum_part_kernel(ColSum<T> g) {
     constexpr int N = CgT<T>::N;
@@ -1131,7 +1116,7 @@ template <typename T> __global__ __launch_bounds__(256) void colsum_part_kernel(
     if (p && c < g.C)
 #pragma unroll 8
         for (size_t r = r0 + w; r < r1; r += 4) {
-            cg_load<T>(p + (z * g.rows + r) * g.C + c, g.C - c, v);
+            cg_load<T>(p + (z * g.rows + r) * g.ld + c, g.C - c, v);
 #pragma unroll
             for (int i = 0; i < N; ++i) s[i] += v[i];
         }
@@ -1167,14 +1152,75 @@ template <typename T> __global__ __launch_bounds__(1024) void colsum_join_kernel
     *o = (T)(g.accumulate >> sel & 1 ? (float)*o + s : s);
 }
 
+constexpr int MAX_WIDTH = 1 << 21;
 bool dims_ok(const cg_gated_dims* d, const cg_group* grp) {
     return d && d->rows >= 0 && d->rows < INT32_MAX && d->rows % grp_n(grp) == 0 && d->D > 0 && d->F > 0 && d->O >= 0 &&
+           d->D <= MAX_WIDTH && d->F <= MAX_WIDTH && d->O <= MAX_WIDTH &&      // a tile's offsets stay below 2^31 bytes
            (d->dtype == CG_DT_F32 || d->dtype == CG_DT_F16 || d->dtype == CG_DT_BF16) && d->gate >= 0 && d->gate <= CG_GATE_SIGMOID &&
            (grp_n(grp) == 1 || d->dtype == CG_DT_F32);
 }
 
 inline size_t esize(int dt) { return dt == CG_DT_F32 ? 4 : 2; }
 inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Copies of 16-bit operands whose rows do not start on 16 bytes (an odd width, a shifted tensor): rows of a multiple of 8 elements that end
+// in zeros.  The tiles are fetched 16 bytes at a time straight into LDS; a copy reads and writes an operand once, where the product
+// reads it once for every 256 rows or columns of the result.
+template <typename T> struct Pack {
+    struct { const T* src; T* dst; size_t first, end; int cols, chunks; } o[4];      // chunks [first, end) of the launch, `chunks` a row
+    int n;
+};
+template <typename T> __global__ __launch_bounds__(256) void pack_kernel(Pack<T> g) {
+    const size_t total = g.o[g.n - 1].end;
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
+        int j = 0;
+        while (i >= g.o[j].end) ++j;
+        const size_t c = i - g.o[j].first, r = c / g.o[j].chunks;
+        const int k = (int)(c % g.o[j].chunks) * 8;
+        float v[8];
+        cg_load<T, 8>(g.o[j].src + r * g.o[j].cols + k, g.o[j].cols - k, v);
+        cg_store<T, 8>(g.o[j].dst + c * 8, 8, v);
+    }
+}
+
+// Operands as the products read them: pointer and pitch, packed or in place
+template <typename T> struct Operands { const T *x, *wg, *wv, *wo; size_t ldx, ldw, ldo; };
+bool packs(const cg_gated_dims* d, const cg_group* grp, const void* p, size_t cols) {
+    return d->dtype != CG_DT_F32 && (size_t)d->rows / grp_n(grp) > FEW_ROWS && (cols % 8 != 0 || (uintptr_t)p % 16 != 0);
+}
+size_t pack_bytes(const cg_gated_dims* d, const cg_group* grp, const void* x, const void* wg, const void* wv, const void* wo) {
+    size_t n = 0;
+    auto add = [&](const void* p, size_t rows, size_t cols) { n += packs(d, grp, p, cols) ? up256(rows * pad8((int)cols) * 2) : 0; };
+    add(x, d->rows, d->D);
+    // the two projections share a pitch
+    if (packs(d, grp, wg, d->D) || packs(d, grp, wv, d->D)) n += 2 * up256((size_t)d->F * pad8(d->D) * 2);
+    if (d->O) add(wo, d->O, d->F);
+    return n;
+}
+// where the operands are once `pack` is filled; run: fill it
+template <typename T>
+Operands<T> operands(const cg_gated_dims* d, const cg_group* grp, const T* x, const T* wg, const T* wv, const T* wo, void* pack, bool run,
+                     hipStream_t st) {
+    const size_t D = d->D, F = d->F, dp = pad8(d->D), fp = pad8(d->F);
+    Operands<T> r = {x, wg, wv, wo, D, D, F};
+    char* at = (char*)pack;
+    Pack<T> g = {};
+    auto add = [&](const T*& p, size_t rows, size_t cols, size_t pitch) {
+        const size_t first = g.n ? g.o[g.n - 1].end : 0;
+        auto& o = g.o[g.n++];
+        o.src = p, o.dst = (T*)at, o.first = first, o.end = first + rows * (pitch / 8), o.cols = (int)cols, o.chunks = (int)(pitch / 8);
+        p = (const T*)at;
+        at += up256(rows * pitch * 2);
+    };
+    if (packs(d, grp, x, D)) add(r.x, d->rows, D, dp), r.ldx = dp;
+    if (packs(d, grp, wg, D) || packs(d, grp, wv, D)) add(r.wg, F, D, dp), add(r.wv, F, D, dp), r.ldw = dp;
+    if (d->O && packs(d, grp, wo, F)) add(r.wo, d->O, F, fp), r.ldo = fp;
+    if (g.n && run) {
+        const size_t nb = (g.o[g.n - 1].end + 255) / 256;
+        pack_kernel<T><<<(unsigned)(nb < 8192 ? nb : 8192), 256, 0, st>>>(g);
+    }
+    return r;
+}
 
 // scratch of the forward and the backward pass: both use it for one product or sum after the other
 size_t fwd_part(const cg_gated_dims* d, const cg_group* grp) {
@@ -1197,27 +1243,31 @@ size_t bwd_part(const cg_gated_dims* d, const cg_group* grp) {
     return up256(most);
 }
 
+// pitch of a, v, da, dv, and of h where it is not the result: rows on 16 bytes
+inline int ldf_of(const cg_gated_dims* d) { return (int)pad8(d->F); }
+
 template <typename T>
 void fwd(const cg_gated_dims* d, const cg_group* grp, const T* x, const T* wg, const T* wv, const T* wo, const T* bg, const T* bv,
-         const T* bo, T* h, T* a, T* v, T* y, float* part, hipStream_t st) {
-    const int nz = grp_n(grp);
-    const size_t M = d->rows / nz, gs = grp_stride(grp), D = d->D, F = d->F;
+         const T* bo, T* h, T* a, T* v, T* y, void* pack, float* part, hipStream_t st) {
+    const int nz = grp_n(grp), ldf = ldf_of(d);
+    const size_t M = d->rows / nz, gs = grp_stride(grp);
+    const bool small = M <= FEW_ROWS;
+    const Operands<T> op = operands<T>(d, grp, x, wg, wv, wo, pack, true, st);
     Gemm<T> g = {};
     g.nseg = g.nsel = 1;
-    g.A[0] = x, g.az = M * D, g.lda = D;
-    g.B[0] = wg, g.B[1] = wv, g.bz = gs, g.ldb = D;
-    g.M = M, g.K = D, g.N = d->F, g.gate = d->gate;
+    g.A[0] = op.x, g.az = M * op.ldx, g.lda = op.ldx;
+    g.B[0] = op.wg, g.B[1] = op.wv, g.bz = gs, g.ldb = op.ldw;
+    g.M = M, g.K = d->D, g.N = d->F, g.gate = d->gate;
     g.bias[0] = bg, g.bias[1] = bv, g.biasz = gs;
-    g.o0 = h, g.o1 = a, g.o2 = v, g.oz = M * F;
-    const bool small = M <= FEW_ROWS;
+    g.o0 = h, g.o1 = a, g.o2 = v, g.ld0 = d->O ? ldf : d->F, g.ldf = ldf;
     if (small) few<T, true, EPI_GATE_FWD>(g, nz, st);
     else gemm<T, true, true, EPI_GATE_FWD>(g, nz, part, st);
     if (!d->O) return;
     Gemm<T> p = {};
     p.nseg = p.nsel = 1;
-    p.A[0] = h, p.az = M * F, p.lda = F;
-    p.B[0] = wo, p.bz = gs, p.ldb = F;
-    p.M = M, p.K = F, p.N = d->O;
+    p.A[0] = h, p.az = M * ldf, p.lda = ldf;
+    p.B[0] = op.wo, p.bz = gs, p.ldb = op.ldo;
+    p.M = M, p.K = d->F, p.N = d->O;
     p.bias[0] = bo, p.biasz = gs;
     p.c[0] = y, p.cz = M * d->O;
     if (small) few<T, true, EPI_STORE>(p, nz, st);
@@ -1226,37 +1276,47 @@ void fwd(const cg_gated_dims* d, const cg_group* grp, const T* x, const T* wg, c
 
 template <typename T>
 void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, const T* wg, const T* wv, const T* wo, const T* h,
-         const T* a, const T* v, T* dx, T* dwg, T* dwv, T* dwo, T* dbg, T* dbv, T* dbo, int acc, T* da, T* dv, float* part,
-         hipStream_t st) {
-    const int nz = grp_n(grp);
+         const T* a, const T* v, T* dx, T* dwg, T* dwv, T* dwo, T* dbg, T* dbv, T* dbo, int acc, void* pack, T* da, T* dv, T* dyp,
+         float* part, hipStream_t st) {
+    const int nz = grp_n(grp), ldf = ldf_of(d);
     const size_t M = d->rows / nz, gs = grp_stride(grp), D = d->D, F = d->F, O = d->O;
     const bool small = M <= FEW_ROWS;
+    const Operands<T> op = operands<T>(d, grp, x, wg, wv, wo, pack, false, st);
+    size_t ldy = O;
+    if (O && packs(d, grp, dy, O)) {
+        Pack<T> g = {};
+        g.n = 1, ldy = pad8(d->O);
+        g.o[0].src = dy, g.o[0].dst = dyp, g.o[0].end = d->rows * (ldy / 8), g.o[0].cols = d->O, g.o[0].chunks = (int)(ldy / 8);
+        const size_t nb = (g.o[0].end + 255) / 256;
+        pack_kernel<T><<<(unsigned)(nb < 8192 ? nb : 8192), 256, 0, st>>>(g);
+        dy = dyp;
+    }
     if (dx || dwg || dwv || dbg || dbv) {
         if (O) {
             Gemm<T> g = {};
             g.nseg = g.nsel = 1;
-            g.A[0] = dy, g.az = M * O, g.lda = O;
-            g.B[0] = wo, g.bz = gs, g.ldb = F;
+            g.A[0] = dy, g.az = M * ldy, g.lda = ldy;
+            g.B[0] = op.wo, g.bz = gs, g.ldb = op.ldo;
             g.M = M, g.K = O, g.N = d->F, g.gate = d->gate;
-            g.o0 = da, g.o1 = dv, g.i0 = a, g.i1 = v, g.oz = M * F;
+            g.o0 = da, g.o1 = dv, g.i0 = a, g.i1 = v, g.ldf = ldf;
             if ((dbg || dbv) && !small) g.sums = part;
             if (small) few<T, false, EPI_GATE_BWD>(g, nz, st);
             else gemm<T, true, false, EPI_GATE_BWD>(g, nz, part, st);
             if (g.sums && M) {
-                ColSum<T> c = {{da, dv}, {dbg, dbv}, M, gs, d->F, g.strips, acc >> 3 & 3, part};
+                ColSum<T> c = {{da, dv}, {dbg, dbv}, M, gs, d->F, ldf, g.strips, acc >> 3 & 3, part};
                 colsum_join_kernel<T><<<dim3(cg_div_up(F, 32), 1, 2 * nz), 1024, 0, st>>>(c);
                 dbg = dbv = nullptr;
             }
         } else if (M) {
-            const size_t n = (size_t)d->rows * F, nb = (n + 2047) / 2048;
-            gate_bwd_kernel<T><<<(unsigned)(nb < 16384 ? nb : 16384), 256, 0, st>>>(GateBwd<T>{dy, a, v, da, dv, n, d->gate});
+            const size_t nb = ((size_t)d->rows * (ldf / 8) + 255) / 256;
+            gate_bwd_kernel<T><<<(unsigned)(nb < 16384 ? nb : 16384), 256, 0, st>>>(GateBwd<T>{dy, a, v, da, dv, (size_t)d->rows, d->F, ldf, d->gate});
         }
     }
     if (dx) {
         Gemm<T> g = {};
         g.nseg = 2, g.nsel = 1;
-        g.A[0] = da, g.A[1] = dv, g.az = M * F, g.lda = F;
-        g.B[0] = wg, g.B[1] = wv, g.bz = gs, g.ldb = D;
+        g.A[0] = da, g.A[1] = dv, g.az = M * ldf, g.lda = ldf;
+        g.B[0] = op.wg, g.B[1] = op.wv, g.bz = gs, g.ldb = op.ldw;
         g.M = M, g.K = F, g.N = d->D;
         g.c[0] = dx, g.cz = M * D;
         if (small) few<T, false, EPI_STORE>(g, nz, st);
@@ -1266,79 +1326,88 @@ void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, c
         FewGrads<T> g = {};
         g.M = (int)M, g.gs = gs;
         int first = 0;
-        auto add = [&](const T* p, size_t P, const T* q, size_t Q, T* dw, T* db, int bit) {
+        auto add = [&](const T* p, size_t P, size_t ldp, const T* q, size_t Q, size_t ldq, T* dw, T* db, int bit) {
             if (!dw && !db) return;
             auto& o = g.o[g.n++];
-            o.p = p, o.q = q, o.dw = dw, o.db = db, o.P = (int)P, o.Q = (int)Q, o.tiles_q = dw ? (int)cg_div_up(Q, 64) : 1, o.first = first;
+            o.p = p, o.q = q, o.dw = dw, o.db = db, o.P = (int)P, o.Q = (int)Q, o.ldp = (int)ldp, o.ldq = (int)ldq;
+            o.tiles_q = dw ? (int)cg_div_up(Q, 64) : 1, o.first = first;
             o.add_w = acc >> bit & 1, o.add_b = acc >> (bit + 3) & 1;
             first += (int)cg_div_up(P, 64) * o.tiles_q;
         };
-        add(da, F, x, D, dwg, dbg, 0);
-        add(dv, F, x, D, dwv, dbv, 1);
-        if (O) add(dy, O, h, F, dwo, dbo, 2);
+        add(da, F, ldf, x, D, D, dwg, dbg, 0);
+        add(dv, F, ldf, x, D, D, dwv, dbv, 1);
+        if (O) add(dy, O, O, h, F, ldf, dwo, dbo, 2);
         if (g.n) few_grads_kernel<T><<<dim3(first, nz), 256, 0, st>>>(g);
         return;
     }
-    auto wgrad = [&](const T* p0, const T* p1, size_t P, const T* q, size_t Q, T* dw0, T* dw1, int accumulate) {
+    auto wgrad = [&](const T* p0, const T* p1, size_t P, size_t ldp, const T* q, size_t Q, size_t ldq, T* dw0, T* dw1, int accumulate) {
         if (!dw0 && !dw1) return;
         Gemm<T> g = {};
         g.nseg = 1, g.nsel = dw0 && dw1 ? 2 : 1;
-        g.A[0] = dw0 ? p0 : p1, g.A[1] = p1, g.az = M * P, g.lda = P;
-        g.B[0] = q, g.bz = M * Q, g.ldb = Q;
+        g.A[0] = dw0 ? p0 : p1, g.A[1] = p1, g.az = M * ldp, g.lda = ldp;
+        g.B[0] = q, g.bz = M * ldq, g.ldb = ldq;
         g.M = P, g.K = M, g.N = (int)Q;
         g.c[0] = dw0 ? dw0 : dw1, g.c[1] = dw1, g.cz = gs, g.accumulate = dw0 ? accumulate : accumulate >> 1;
         gemm<T, false, false, EPI_STORE>(g, nz, part, st);
     };
-    wgrad(da, dv, F, x, D, dwg, dwv, acc & 3);
-    if (O) wgrad(dy, nullptr, O, h, F, dwo, nullptr, acc >> 2 & 1);
-    auto bgrad = [&](const T* p0, const T* p1, int C, T* db0, T* db1, int accumulate) {
+    wgrad(da, dv, F, ldf, op.x, D, op.ldx, dwg, dwv, acc & 3);
+    if (O) wgrad(dy, nullptr, O, ldy, h, F, ldf, dwo, nullptr, acc >> 2 & 1);
+    auto bgrad = [&](const T* p0, const T* p1, int C, size_t ld, T* db0, T* db1, int accumulate) {
         if (!db0 && !db1) return;
-        ColSum<T> g = {{db0 ? p0 : nullptr, db1 ? p1 : nullptr}, {db0, db1}, M, gs, C, strips_of(M), accumulate, part};
+        ColSum<T> g = {{db0 ? p0 : nullptr, db1 ? p1 : nullptr}, {db0, db1}, M, gs, C, (int)ld, strips_of(M), accumulate, part};
         colsum_part_kernel<T><<<dim3(cg_div_up(C, 64 * CgT<T>::N), g.strips, 2 * nz), 256, 0, st>>>(g);
         colsum_join_kernel<T><<<dim3(cg_div_up(C, 32), 1, 2 * nz), 1024, 0, st>>>(g);
     };
-    bgrad(da, dv, d->F, dbg, dbv, acc >> 3 & 3);
-    if (O) bgrad(dy, nullptr, d->O, dbo, nullptr, acc >> 5 & 1);
+    bgrad(da, dv, d->F, ldf, dbg, dbv, acc >> 3 & 3);
+    if (O) bgrad(dy, nullptr, d->O, ldy, dbo, nullptr, acc >> 5 & 1);
 }
 
 }  // namespace
 
+extern "C" size_t cg_gated_ff_pack_bytes(const cg_gated_dims* d, const cg_group* grp, const void* x, const void* wg, const void* wv,
+                                         const void* wo) {
+    return dims_ok(d, grp) ? pack_bytes(d, grp, x, wg, wv, wo) : 0;
+}
+
 extern "C" size_t cg_gated_ff_fwd_workspace(const cg_gated_dims* d, const cg_group* grp) { return dims_ok(d, grp) ? fwd_part(d, grp) : 0; }
 
 extern "C" int cg_gated_ff_fwd(const cg_gated_dims* d, const cg_group* grp, const void* x, const void* wg, const void* wv, const void* wo,
-                               const void* bg, const void* bv, const void* bo, void* h, void* a, void* v, void* y, void* ws,
+                               const void* bg, const void* bv, const void* bo, void* h, void* a, void* v, void* y, void* pack, void* ws,
                                size_t ws_bytes, cg_stream_t stream) {
     CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && !a == !v && (!d->O || wo) && (!d->rows || (x && h && (!d->O || y))),
                  "cg_gated_ff_fwd: bad args");
     const size_t need = fwd_part(d, grp);
-    if (ws_bytes < need || (!ws && need)) return cg_set_error(CG_ERR_WORKSPACE, "cg_gated_ff_fwd: workspace too small");
+    if (ws_bytes < need || (!ws && need) || (!pack && pack_bytes(d, grp, x, wg, wv, wo)))
+        return cg_set_error(CG_ERR_WORKSPACE, "cg_gated_ff_fwd: workspace too small");
     if (!d->rows) return CG_OK;
     CG_DISPATCH_DT(d->dtype, T, (fwd<T>(d, grp, (const T*)x, (const T*)wg, (const T*)wv, (const T*)wo, (const T*)bg, (const T*)bv,
-                                        (const T*)bo, (T*)h, (T*)a, (T*)v, (T*)y, (float*)ws, cg_s(stream))));
+                                        (const T*)bo, (T*)h, (T*)a, (T*)v, (T*)y, pack, (float*)ws, cg_s(stream))));
     CG_LAUNCH_CHECK("cg_gated_ff_fwd");
     return CG_OK;
 }
 
-static size_t bwd_hidden(const cg_gated_dims* d) { return up256((size_t)d->rows * d->F * esize(d->dtype)); }
+static size_t bwd_hidden(const cg_gated_dims* d) { return up256((size_t)d->rows * ldf_of(d) * esize(d->dtype)); }
+static size_t bwd_dy(const cg_gated_dims* d) { return d->dtype == CG_DT_F32 ? 0 : up256((size_t)d->rows * pad8(d->O) * 2); }
 
 extern "C" size_t cg_gated_ff_bwd_workspace(const cg_gated_dims* d, const cg_group* grp) {
-    return dims_ok(d, grp) ? 2 * bwd_hidden(d) + bwd_part(d, grp) : 0;
+    return dims_ok(d, grp) ? 2 * bwd_hidden(d) + bwd_dy(d) + bwd_part(d, grp) : 0;
 }
 
 extern "C" int cg_gated_ff_bwd(const cg_gated_dims* d, const cg_group* grp, const void* dy, const void* x, const void* wg,
                                const void* wv, const void* wo, const void* h, const void* a, const void* v, void* dx, void* dwg,
-                               void* dwv, void* dwo, void* dbg, void* dbv, void* dbo, int accumulate, void* ws, size_t ws_bytes,
-                               cg_stream_t stream) {
+                               void* dwv, void* dwo, void* dbg, void* dbv, void* dbo, int accumulate, const void* pack, void* ws,
+                               size_t ws_bytes, cg_stream_t stream) {
     CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && (!d->O || wo) && (!d->rows || (dy && x && a && v && (!d->O || h))),
                  "cg_gated_ff_bwd: bad args");
     const size_t need = cg_gated_ff_bwd_workspace(d, grp);
-    if (ws_bytes < need || (!ws && need)) return cg_set_error(CG_ERR_WORKSPACE, "cg_gated_ff_bwd: workspace too small");
+    if (ws_bytes < need || (!ws && need) || (!pack && pack_bytes(d, grp, x, wg, wv, wo)))
+        return cg_set_error(CG_ERR_WORKSPACE, "cg_gated_ff_bwd: workspace too small");
     CG_DISPATCH_DT(d->dtype, T, {
-        T* da = (T*)ws;
-        T* dv = (T*)((char*)ws + bwd_hidden(d));
-        float* part = (float*)((char*)ws + 2 * bwd_hidden(d));
+        char* w = (char*)ws;
+        T *da = (T*)w, *dv = (T*)(w + bwd_hidden(d)), *dyp = (T*)(w + 2 * bwd_hidden(d));
+        float* part = (float*)(w + 2 * bwd_hidden(d) + bwd_dy(d));
         bwd<T>(d, grp, (const T*)dy, (const T*)x, (const T*)wg, (const T*)wv, (const T*)wo, (const T*)h, (const T*)a, (const T*)v, (T*)dx,
-               (T*)dwg, (T*)dwv, (T*)dwo, (T*)dbg, (T*)dbv, (T*)dbo, accumulate, da, dv, part, cg_s(stream));
+               (T*)dwg, (T*)dwv, (T*)dwo, (T*)dbg, (T*)dbv, (T*)dbo, accumulate, (void*)pack, da, dv, dyp, part, cg_s(stream));
     });
     CG_LAUNCH_CHECK("cg_gated_ff_bwd");
     return CG_OK;

@@ -35,6 +35,7 @@ struct Api {
     decltype(&cg_channel_norm_bwd_workspace) norm_bwd_ws = nullptr;
     decltype(&cg_channel_norm_bwd) norm_bwd = nullptr;
     decltype(&cg_dropout) dropout = nullptr;
+    decltype(&cg_gated_ff_pack_bytes) gated_pack = nullptr;
     decltype(&cg_gated_ff_fwd_workspace) gated_fwd_ws = nullptr;
     decltype(&cg_gated_ff_fwd) gated_fwd = nullptr;
     decltype(&cg_gated_ff_bwd_workspace) gated_bwd_ws = nullptr;
@@ -244,10 +245,12 @@ py::object dropout(const Tensor& x, const std::optional<Tensor>& residual, int t
     return py::cast(y);
 }
 
+constexpr int64_t MAX_WIDTH = 1 << 21;       // as the library has it
+
 // -- gated_feed_forward --------------------------------------------------------------------------------
 struct Gated : public torch::autograd::Node {
     SavedVariable x_, wg_, wv_, wo_;
-    Tensor h_, av_;
+    Tensor h_, av_, pack_;      // av_: both projections; pack_: the forward pass's copies of operands that are not on 16 bytes
     std::array<Tensor, 3> biases;
     cg_gated_dims dims{};
     Members members;
@@ -261,6 +264,7 @@ struct Gated : public torch::autograd::Node {
         wo_.reset_data();
         h_.reset();
         av_.reset();
+        pack_.reset();
     }
     variable_list apply(variable_list&& grads) override {
         once("gated_feed_forward");
@@ -282,9 +286,9 @@ struct Gated : public torch::autograd::Node {
         const size_t nws = api.gated_bwd_ws(&dims, members.get());
         const Tensor ws = scratch(nws, x);
         char* a = (char*)av_.data_ptr();
-        char* v = a + (size_t)dims.rows * dims.F * av_.element_size();
+        char* v = a + av_.nbytes() / 2;
         check(api.gated_bwd(&dims, members.get(), ptr(dy), ptr(x), ptr(p[0]), ptr(p[1]), ptr(p[2]), ptr(h_), a, v, ptr(dx), to[0], to[1], to[2],
-                            to[3], to[4], to[5], add, ptr(ws), nws, stream_of(x)),
+                            to[3], to[4], to[5], add, ptr(pack_), ptr(ws), nws, stream_of(x)),
               "cg_gated_ff_bwd");
         return out;
     }
@@ -299,10 +303,10 @@ py::object gated(const Tensor& x, const Tensor& wg, const Tensor& wv, const std:
     const int dt = dt_of(x.scalar_type());
     auto like = [&](const Tensor& t) { return t.scalar_type() == x.scalar_type() && t.device() == x.device(); };
     if (!x.is_cuda() || dt < 0 || gate < 0 || wg.dim() != 2 || wv.dim() != 2 || wg.sizes() != wv.sizes() || !like(wg) || !like(wv) ||
-        channels(x) != wg.size(1) || wg.size(0) < 1 || wg.size(1) < 1 || wg.size(0) > INT32_MAX || wg.size(1) > INT32_MAX)
+        channels(x) != wg.size(1) || wg.size(0) < 1 || wg.size(1) < 1 || wg.size(0) > MAX_WIDTH || wg.size(1) > MAX_WIDTH || x.numel() / wg.size(1) >= INT32_MAX)
         return py::none();
     const int64_t F = wg.size(0), D = wg.size(1);
-    if (wo.defined() && (wo.dim() != 2 || wo.size(1) != F || wo.size(0) < 1 || wo.size(0) > INT32_MAX || !like(wo))) return py::none();
+    if (wo.defined() && (wo.dim() != 2 || wo.size(1) != F || wo.size(0) < 1 || wo.size(0) > MAX_WIDTH || !like(wo))) return py::none();
     const int64_t O = wo.defined() ? wo.size(0) : 0;
     for (int i = 0; i < 3; ++i)
         if (b[i].defined() && (b[i].dim() != 1 || b[i].size(0) != (i < 2 ? F : O) || !like(b[i]) || (i == 2 && !O))) return py::none();
@@ -321,7 +325,7 @@ py::object gated(const Tensor& x, const Tensor& wg, const Tensor& wv, const std:
         py::gil_scoped_release unlock;
         const c10::DeviceGuard device(x.device());
         Members members{{n, 0, stride}};
-        Tensor xd, h, av;
+        Tensor xd, h, av, pack;
         std::array<Tensor, 6> p{wg, wv, wo, b[0], b[1], b[2]};
         const int64_t rows = x.numel() / D;
         cg_gated_dims dims{rows, (int32_t)D, (int32_t)F, (int32_t)O, dt, gate, 0};
@@ -335,14 +339,16 @@ py::object gated(const Tensor& x, const Tensor& wg, const Tensor& wv, const std:
                 s[x.dim() == 4 ? 1 : x.dim() - 1] = c;
                 return x.dim() == 4 ? at::empty(s, x.options(), at::MemoryFormat::ChannelsLast) : at::empty(s, x.options());
             };
-            h = rows_like(F);
+            const int64_t pitch = (F + 7) & ~(int64_t)7;
+            h = O ? at::empty({rows, pitch}, x.options()) : rows_like(F);
             if (O) y = rows_like(O);
-            if (record) av = at::empty({2, rows, F}, x.options());
+            if (record) av = at::empty({2, rows, pitch}, x.options());
             char* a = record ? (char*)av.data_ptr() : nullptr;
+            pack = scratch(api.gated_pack(&dims, members.get(), ptr(xd), ptr(p[0]), ptr(p[1]), ptr(p[2])), x);
             const size_t nws = api.gated_fwd_ws(&dims, members.get());
             const Tensor ws = scratch(nws, x);
             check(api.gated_fwd(&dims, members.get(), ptr(xd), ptr(p[0]), ptr(p[1]), ptr(p[2]), ptr(p[3]), ptr(p[4]), ptr(p[5]), ptr(h), a,
-                                record ? a + (size_t)rows * F * av.element_size() : nullptr, ptr(y), ptr(ws), nws, stream_of(x)),
+                                record ? a + av.nbytes() / 2 : nullptr, ptr(y), ptr(pack), ptr(ws), nws, stream_of(x)),
                   "cg_gated_ff_fwd");
         }
         if (record) {
@@ -357,6 +363,7 @@ py::object gated(const Tensor& x, const Tensor& wg, const Tensor& wv, const std:
             for (int i = 0; i < 3; ++i)
                 if (p[3 + i].defined()) node->biases[i] = p[3 + i].detach();
             node->av_ = av;
+            node->pack_ = pack;
             node->dims = dims;
             node->members = members;
             if (!O) y = h;
@@ -376,6 +383,7 @@ void bind(const py::dict& d) {
     CG_BIND(norm_bwd_ws, cg_channel_norm_bwd_workspace);
     CG_BIND(norm_bwd, cg_channel_norm_bwd);
     CG_BIND(dropout, cg_dropout);
+    CG_BIND(gated_pack, cg_gated_ff_pack_bytes);
     CG_BIND(gated_fwd_ws, cg_gated_ff_fwd_workspace);
     CG_BIND(gated_fwd, cg_gated_ff_fwd);
     CG_BIND(gated_bwd_ws, cg_gated_ff_bwd_workspace);

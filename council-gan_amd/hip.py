@@ -163,9 +163,10 @@ _SIGS = {
     "cg_dropout_key": (c_int, [_P, _P, _P]),
     "cg_dropout": (c_int, [_P, _P, _P, c_size_t, c_int, _P, c_int, _P]),
     "cg_gated_ff_fwd_workspace": (c_size_t, [POINTER(GatedDims), POINTER(Group)]),
-    "cg_gated_ff_fwd": (c_int, [POINTER(GatedDims), POINTER(Group)] + [_P] * 12 + [c_size_t, _P]),
+    "cg_gated_ff_pack_bytes": (c_size_t, [POINTER(GatedDims), POINTER(Group), _P, _P, _P, _P]),
+    "cg_gated_ff_fwd": (c_int, [POINTER(GatedDims), POINTER(Group)] + [_P] * 13 + [c_size_t, _P]),
     "cg_gated_ff_bwd_workspace": (c_size_t, [POINTER(GatedDims), POINTER(Group)]),
-    "cg_gated_ff_bwd": (c_int, [POINTER(GatedDims), POINTER(Group)] + [_P] * 15 + [c_int, _P, c_size_t, _P]),
+    "cg_gated_ff_bwd": (c_int, [POINTER(GatedDims), POINTER(Group)] + [_P] * 15 + [c_int, _P, _P, c_size_t, _P]),
     "cg_avgpool3s2_fwd": (c_int, [_P, _P, c_int, c_int, c_int, c_int, _P]),
     "cg_avgpool3s2_bwd": (c_int, [_P, _P, c_int, c_int, c_int, c_int, _P]),
     "cg_upsample2x_fwd": (c_int, [_P, _P, c_int, c_int, c_int, c_int, _P]),
@@ -227,7 +228,7 @@ def load():
 _nodes = None
 NODES_PATH = os.path.join(_HERE, "lib", "cg_nodes.so")
 _NODE_CALLS = ("cg_last_error", "cg_channel_norm_fwd", "cg_channel_norm_bwd_workspace", "cg_channel_norm_bwd", "cg_dropout",
-               "cg_gated_ff_fwd_workspace", "cg_gated_ff_fwd", "cg_gated_ff_bwd_workspace", "cg_gated_ff_bwd")
+               "cg_gated_ff_pack_bytes", "cg_gated_ff_fwd_workspace", "cg_gated_ff_fwd", "cg_gated_ff_bwd_workspace", "cg_gated_ff_bwd")
 
 
 def nodes():

@@ -1847,6 +1847,8 @@ def _gated_explain(x, w_gate, w_value, w_out, b_gate, b_value, b_out, act):
     for name, p, shape in named:
         if p is not None or name == "w_value":
             _check_param(what, name, p, shape, x, (x.dtype,))
+    if max(D, F, w_out.shape[0] if w_out is not None else 0) > 1 << 21 or x.numel() // D >= (1 << 31) - 1:
+        raise ValueError("%s: at most 2^21 channels or hidden units and 2^31 - 2 rows" % what)
     _check_gpu(what, x)
     raise ValueError("%s: bad arguments" % what)
 

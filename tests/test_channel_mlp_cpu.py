@@ -45,6 +45,7 @@ REFUSED = [
     ("gated_bias", lambda: ops.gated_feed_forward(t(2, 4), t(6, 4), t(6, 4), b_gate=t(4)), "b_gate must be"),
     ("gated_bias_out", lambda: ops.gated_feed_forward(t(2, 4), t(6, 4), t(6, 4), b_out=t(4)), "b_out without w_out"),
     ("gated_mixed", lambda: ops.gated_feed_forward(t(2, 4, dtype=torch.bfloat16), t(6, 4), t(6, 4)), "w_gate is"),
+    ("gated_wide", lambda: ops.gated_feed_forward(t(0, (1 << 21) + 1), t(1, (1 << 21) + 1), t(1, (1 << 21) + 1)), "at most 2"),
     ("gated_empty", lambda: ops.gated_feed_forward(t(2, 4), t(0, 4), t(0, 4)), "at least 1"),
 ]
 
@@ -75,12 +76,17 @@ def test_library_refuses_bad_arguments_before_any_launch():
     assert lib.cg_dropout(p, None, p, 4, 1, p, 3, None) == -1
     assert lib.cg_dropout_key(p, p, None) == -1
     d = hip.GatedDims(4, 8, 16, 8, 1, 0, 0)
-    args = [p] * 12
+    args = [p] * 13
     assert lib.cg_gated_ff_fwd(ctypes.byref(hip.GatedDims(4, 8, 16, 8, 1, 3, 0)), None, *args, 0, None) == -1
     assert lib.cg_gated_ff_fwd(ctypes.byref(d), ctypes.byref(hip.Group(2, 0, 32)), *args, 0, None) == -1   # members hold fp32
-    assert lib.cg_gated_ff_fwd(ctypes.byref(d), None, p, p, p, None, None, None, None, p, p, p, p, None, 0, None) == -1
-    assert lib.cg_gated_ff_bwd(ctypes.byref(d), None, *([p] * 15), 0, p, 0, None) == -3
+    assert lib.cg_gated_ff_fwd(ctypes.byref(d), None, p, p, p, None, None, None, None, p, p, p, p, None, None, 0, None) == -1
+    assert lib.cg_gated_ff_bwd(ctypes.byref(d), None, *([p] * 15), 0, p, p, 0, None) == -3
     assert b"workspace" in lib.cg_last_error()
+    odd = hip.GatedDims(64, 9, 16, 8, 1, 0, 0)      # rows of 9 halves do not start on 16 bytes: the copies need memory
+    assert lib.cg_gated_ff_pack_bytes(ctypes.byref(odd), None, p, p, p, p) >= (64 + 2 * 16) * 16 * 2
+    assert lib.cg_gated_ff_fwd(ctypes.byref(odd), None, p, p, p, p, None, None, None, p, p, p, p, None, p, 1 << 30, None) == -3
+    assert lib.cg_gated_ff_pack_bytes(ctypes.byref(hip.GatedDims(64, 8, 16, 8, 1, 0, 0)), None, p, p, p, p) == 0
+    assert lib.cg_gated_ff_pack_bytes(ctypes.byref(hip.GatedDims(64, 8, 16, 8, 1, 0, 0)), None, ctypes.c_void_p(258), p, p, p) > 0
 
 
 def test_workspaces_of_any_size_are_finite():
@@ -93,7 +99,7 @@ def test_workspaces_of_any_size_are_finite():
                 d, grp = ctypes.byref(hip.GatedDims(rows, 264, 520, 72, dt, 0, 0)), ctypes.byref(hip.Group(n, 0, 1 << 20))
                 assert lib.cg_gated_ff_fwd_workspace(d, grp) < 1 << 33
                 hidden = rows * 520 * (4 if dt == 0 else 2)
-                assert 2 * hidden <= lib.cg_gated_ff_bwd_workspace(d, grp) < 2 * hidden + (1 << 33)
+                assert 2 * hidden <= lib.cg_gated_ff_bwd_workspace(d, grp) < 2 * hidden + rows * 144 + (1 << 33)
         assert lib.cg_channel_norm_bwd_workspace(None, rows, 264, 0) < 1 << 33
 
 
