@@ -200,7 +200,7 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
     static_assert(CH >= 1 && ((KC ? ROWS : BK) * CPR) % NT == 0, "every thread has the same number of chunks");
 
     struct Regs { Raw q[CH]; };
-    size_t off[CH];      // the row's start (K-contiguous), the chunk of K-step 0 (row-contiguous)
+    unsigned off[CH];    // bytes from the tile's origin: of the row (K-contiguous), of the chunk (row-contiguous); below 2^31 (MAX_WIDTH)
     int tid, col, shift; // row-contiguous: first row of the thread's chunk, and how far it was moved back to end with the operand
 
     static __device__ __forceinline__ int lrow(int tid, int i) { return (tid + i * NT) / CPR; }
@@ -218,33 +218,39 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
                 int j = lrow(tid, i);
                 if (GATE) j = (j >> 6) * 32 + (j & 31);
                 const size_t r = row0 + j;
-                off[i] = (r < rows ? r : rows - 1) * ld;
+                off[i] = (unsigned)(((r < rows ? r : rows - 1) - row0) * ld * sizeof(T));
             }
         } else {
             const long long r = (long long)row0 + lch(tid) * W, most = (long long)rows - W;
             col = (int)(r < most ? r : most);
             shift = (int)(r - col < W ? r - col : 0);
 #pragma unroll
-            for (int i = 0; i < CH; ++i) off[i] = lrow(tid, i) * ld + col;
+            for (int i = 0; i < CH; ++i) off[i] = (unsigned)((lrow(tid, i) * ld + col) * sizeof(T));
         }
     }
+    // p0, p1: the operands (K-contiguous: from the tile's first row on)
     __device__ __forceinline__ void load(Regs& raw, const T* p0, const T* p1, int k0, int K, size_t ld) const {
+        auto at = [](const T* p, unsigned o) { return (const Raw*)((const char*)p + o); };
         if (KC) {
-            const int k = k0 + lch(tid) * W, kc = k < K - W ? k : K - W;
+            const int k = k0 + lch(tid) * W;
+            const unsigned kc = (unsigned)(k < K - W ? k : K - W) * (unsigned)sizeof(T);
 #pragma unroll
-            for (int i = 0; i < CH; ++i) raw.q[i] = *(const Raw*)((GATE && (lrow(tid, i) >> 5 & 1) ? p1 : p0) + off[i] + kc);
+            for (int i = 0; i < CH; ++i) {
+                const bool second = GATE && (i * (NT / CPR) >> 5 & 1);       // rows 32 .. 63 of 64; a thread's first row is below 32
+                raw.q[i] = *at(second ? p1 : p0, off[i] + kc);
+            }
         } else {
-            const T* p[CH];
+            unsigned o[CH];
 #pragma unroll
-            for (int i = 0; i < CH; ++i) p[i] = p0 + (size_t)k0 * ld + off[i];
+            for (int i = 0; i < CH; ++i) o[i] = off[i];
             if (k0 + BK > K)
 #pragma unroll
                 for (int i = 0; i < CH; ++i) {
-                    const int k = k0 + lrow(tid, i);
-                    p[i] = p0 + (size_t)(k < K ? k : K - 1) * ld + col;
+                    const int r = lrow(tid, i), last = K - 1 - k0;
+                    o[i] = (unsigned)(((r < last ? r : last) * ld + col) * sizeof(T));
                 }
 #pragma unroll
-            for (int i = 0; i < CH; ++i) raw.q[i] = *(const Raw*)p[i];
+            for (int i = 0; i < CH; ++i) raw.q[i] = *at(p0 + (size_t)k0 * ld, o[i]);
         }
     }
     // the elements of a chunk moved down by s, zeros behind (s >= W: all zero)
@@ -402,10 +408,10 @@ __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)
     }
 }
 
-// One LDS buffer, loads one K-step ahead in registers, and three blocks on a CU where the registers allow it (K-contiguous operands: 510 us
-// instead of 577 for the gate product of 65536 x 256 x 1024 with two blocks and two steps ahead).
+// One LDS buffer, loads one K-step ahead in registers, and three blocks on a CU where the registers allow it (not with the operands of the
+// gate's backward epilogue): 510 us instead of 577 for the gate product of 65536 x 256 x 1024 with two blocks and two steps ahead.
 template <typename T, int BM, int BN, int WM, int WN, bool KA, bool KB, int EPI>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && sizeof(T) == 4 && KA && KB ? 3 : 2) void gemm_kernel(Gemm<T> g) {
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && EPI != EPI_GATE_BWD ? 3 : 2) void gemm_kernel(Gemm<T> g) {
     constexpr int NW = (BM / WM) * (BN / WN), NT = NW * 64, TM = WM / 32, TN = WN / 32;
     typedef Operand<T, BM, NT, KA, false> OA;
     typedef Operand<T, BN, NT, KB, EPI == EPI_GATE_FWD> OB;
@@ -435,8 +441,9 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && sizeof(T) 
         const int s = g.nseg == 2 && step >= kt ? 1 : 0, k = step - s * kt;
         const T* pa = g.nseg == 2 ? (s ? g.A[1] : g.A[0]) : (sel ? g.A[1] : g.A[0]);
         const T* pb = s ? g.B[1] : g.B[0];
-        a.load(ra, pa + z * g.az, nullptr, k * BK, (int)g.K, g.lda);
-        b.load(rb, pb + z * g.bz, EPI == EPI_GATE_FWD ? g.B[1] + z * g.bz : nullptr, k * BK, (int)g.K, g.ldb);
+        a.load(ra, pa + z * g.az + (KA ? m0 * g.lda : 0), nullptr, k * BK, (int)g.K, g.lda);
+        const size_t ob = z * g.bz + (KB ? n0 * g.ldb : 0);
+        b.load(rb, pb + ob, EPI == EPI_GATE_FWD ? g.B[1] + ob : nullptr, k * BK, (int)g.K, g.ldb);
     };
     auto store = [&](int step) {
         const int k0 = (g.nseg == 2 && step >= kt ? step - kt : step) * BK;
@@ -1015,25 +1022,32 @@ template <typename T> __global__ __launch_bounds__(256) void few_grads_kernel(Fe
     }
 }
 
-// Tile and number of K splits.  16 bit: 256 x 256 tiles wherever they can fill the chip, split or not, then 128 x 128; fp32: 128 x 128 (4
-// waves of 64 x 64), then 64 x 64 (2 waves).  A split takes at least 4 K-steps.  The number of splits is the one with the least time by this
-// account: tiles run in rounds of as many as fit the chip (256 of the largest, 512 of the others), a K-step takes about 1 us in a 256 x 256
-// tile, 0.6 and 0.4 us in the others, and joining costs a launch, the lost fusions of the epilogue, and the partial sums' way out and
-// back at about 5 TB/s.  The number of members is left out: a member's results do not depend on how many run beside it.
+// Tile and number of K splits: 256 x 256 or 128 x 128 (16 bit), 128 x 128 or 64 x 64 (fp32; 4 waves of 64 x 64, 2 of 32 x 64).  The pair with
+// the least time by this account is taken: tiles run in rounds of as many as fit the chip; a tile takes its K-steps, longer where tiles
+// share a CU, and its epilogue; joining splits costs a launch, the lost fusions of the epilogue, and the partial sums' way out and back at
+// about 5 TB/s.  A split takes at least 4 K-steps.  The figures below are measured (us).  The number of members is left out: a member's
+// results do not depend on how many run beside it.
 struct Plan { int tile, splits; };
 Plan plan(size_t M, size_t N, size_t K, int nsel, int esz) {
     const size_t bk = esz == 4 ? 32 : 64, steps = (K + bk - 1) / bk, most = steps / 4 > 1 ? steps / 4 : 1;
-    auto tiles = [&](size_t t) { return (size_t)cg_div_up(M, t) * cg_div_up(N, t) * nsel; };
-    if (!M || !N) return {128, 1};
-    const int tile = esz == 2 ? (tiles(256) * most >= 192 ? 256 : 128) : (tiles(128) * most >= 192 ? 128 : 64);
-    const size_t t = tiles(tile), slots = tile == 256 ? 256 : 512;
-    const double step_us = tile == 256 ? 1.0 : tile == 128 ? 0.6 : 0.4;
-    Plan p = {tile, 1};
-    double best = 0;
-    for (size_t s = 1; s <= most && s <= 64; ++s) {
-        const double us = (double)((t * s + slots - 1) / slots) * (double)((steps + s - 1) / s) * step_us +
-                          (s > 1 ? 8.0 + 2.0 * 4 * s * M * N * nsel / 5e6 : 0);
-        if (s == 1 || us < best) best = us, p.splits = (int)s;
+    Plan p = {128, 1};
+    if (!M || !N) return p;
+    double best = 1e30;
+    for (int c = 0; c < 2; ++c) {
+        const int tile = esz == 2 ? 256 >> c : 128 >> c;
+        const size_t t = (size_t)cg_div_up(M, tile) * cg_div_up(N, tile) * nsel;
+        for (size_t s = 1; s <= most && s <= 64; ++s) {
+            const size_t n = t * s;
+            double step, epilogue;
+            size_t slots;
+            if (tile == 256) step = 1.0, epilogue = 8, slots = 256;
+            else if (esz == 2) step = n > 256 ? 0.9 : 0.7, epilogue = 4, slots = 512;
+            else if (tile == 128) step = n > 512 ? 2.2 : n > 256 ? 1.6 : 1.4, epilogue = 5, slots = 768;
+            else step = 1.4, epilogue = 2, slots = 1024;
+            const double us = (double)((t * s + slots - 1) / slots) * ((double)((steps + s - 1) / s) * step + epilogue) +
+                              (s > 1 ? 8.0 + 2.0 * 4 * s * M * N * nsel / 5e6 : 0);
+            if (us < best) best = us, p = {tile, (int)s};
+        }
     }
     return p;
 }
