@@ -4,8 +4,8 @@ Public surface = the reference's: `Council_Trainer` (trainer_council.py) and the
 (networks.py), plus the host helpers its constructor uses.  Importing the package needs neither a
 GPU nor the built library; running anything on the hot path needs both and fails loudly otherwise."""
 from . import hip, ops  # noqa: F401
-from .networks import (AdaINGen, AdaptiveInstanceNorm2d, Conv2dBlock, ContentEncoder, Decoder_V2_atten,  # noqa: F401
-                       LayerNorm, LinearBlock, MLP, MsImageDis, MsImageDisCouncil, ResBlock, ResBlocks,
+from .networks import (AdaINGen, AdaptiveInstanceNorm2d, ChannelNorm, Conv2dBlock, ContentEncoder, Decoder_V2_atten,  # noqa: F401
+                       Dropout, GatedBlock, LayerNorm, LinearBlock, MLP, MsImageDis, MsImageDisCouncil, ResBlock, ResBlocks,
                        StyleEncoder)
 from .input import DeviceInput  # noqa: F401
 from .optim import FlatAdam  # noqa: F401

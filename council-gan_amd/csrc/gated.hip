@@ -12,6 +12,9 @@ namespace {
 inline int grp_n(const cg_group* g) { return g && g->n > 1 ? g->n : 1; }
 inline size_t grp_stride(const cg_group* g) { return g && g->n > 1 ? (size_t)g->stride : 0; }
 
+constexpr int MAX_ROWS = 1 << 30;       // a step past the last row is still an int
+constexpr int MAX_WIDTH = 1 << 21;      // a tile's offsets stay below 2^31 bytes
+
 enum { EPI_STORE = 0, EPI_GATE_FWD = 1, EPI_GATE_BWD = 2 };
 
 // C[m, n] = sum_k A(m, k) B(n, k).  Operands are "K-contiguous" (A(m, k) = A[m * ld + k]) or "row-contiguous" (A(m, k) = A[k * ld + m]).
@@ -27,9 +30,9 @@ template <typename T> struct Gemm {
     const T* bias[2];
     size_t biasz;
     int gate;
-    T *o0, *o1, *o2;          // EPI_GATE_FWD: h, a, v; EPI_GATE_BWD: da, dv
-    const T *i0, *i1;         // EPI_GATE_BWD: a, v
-    int ld0, ldf;             // pitch of h; of a, v, da, dv.  A pitch beyond N is a multiple of 8 and its columns get zeros
+    T *o0, *o1, *o2;          // EPI_GATE_FWD: h and, for the backward pass, u = act(a) and p = v act'(a); EPI_GATE_BWD: da, dv
+    const T *i0, *i1;         // EPI_GATE_BWD: u, p
+    int ld0, ldf;             // pitch of h; of u, p, da, dv.  A pitch beyond N is a multiple of 8 and its columns get zeros
     float* sums;              // EPI_GATE_BWD, or NULL: column sums of da and dv over a wave's rows, [member][2][strips][N]
     int strips;
     float* part;              // splits > 1: partial sums [split][member * nsel + sel][M][planes][NP]
@@ -127,16 +130,17 @@ __device__ __forceinline__ void emit(const Gemm<T>& g, size_t z, int sel, size_t
         return;
     }
     const size_t of = (z * g.M + m) * g.ldf + n;
-    float u, du;
     if (EPI == EPI_GATE_FWD) {
-        float h[8];
+        float h[8], u, du;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            // act(a) v is formed from the rounded a, v: the values the backward pass differentiates
-            v[i] = (float)(T)(v[i] + b.x[i]);
-            w[i] = (float)(T)(w[i] + b.y[i]);
-            gate_fn<sizeof(T) == 4>(v[i], g.gate, u, du);
+            // h, and what the backward pass needs, are formed in fp32 from the sums and rounded once (16 bit: h, da and dv are operands of
+            // further 16-bit products; with u and p, and not a and v, in memory no rounding goes through the gate)
+            w[i] += b.y[i];
+            gate_fn<sizeof(T) == 4>(v[i] + b.x[i], g.gate, u, du);
             h[i] = i < left ? u * w[i] : 0.f;
+            v[i] = u;
+            w[i] *= du;
         }
         cg_store<T, 8>(g.o0 + (z * g.M + m) * g.ld0 + n, g.ld0 - n, h);
         if (g.o1) {
@@ -146,9 +150,8 @@ __device__ __forceinline__ void emit(const Gemm<T>& g, size_t z, int sel, size_t
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            gate_fn<sizeof(T) == 4>((float)row.x.q[i / W][i % W], g.gate, u, du);
-            w[i] = i < left ? v[i] * u : 0.f;
-            v[i] = i < left ? v[i] * (float)row.y.q[i / W][i % W] * du : 0.f;
+            w[i] = i < left ? v[i] * (float)row.x.q[i / W][i % W] : 0.f;
+            v[i] = i < left ? v[i] * (float)row.y.q[i / W][i % W] : 0.f;
             sx[i] += v[i];
             sy[i] += w[i];
         }
@@ -161,9 +164,9 @@ template <int EPI> constexpr int planes() { return EPI == EPI_GATE_FWD ? 2 : 1; 
 __host__ __device__ __forceinline__ size_t pad8(int n) { return (size_t)((n + 7) & ~7); }
 
 // ------------------------------------------------------------------------------------------
-// tile kernel on v_mfma_f32_32x32x16 (fp16 / bf16).
+// Products of fp32 operands on v_mfma_f32_32x32x16_bf16: 128 x 128 tiles, 4 waves of 64 x 64; 64 x 64 tiles, 2 waves of 32 x 64.
 //
-// fp32 operands are split exactly into three bf16 values on their way to LDS, x = h + m + l (round to nearest even, 8 + 8 + 8
+// The operands are split exactly into three bf16 values on their way to LDS, x = h + m + l (round to nearest even, 8 + 8 + 8
 // significant bits), and a product is the six terms hh, hm, mh, hl, mm, lh: what is left out is below 2^-23 of |x y|, half a
 // rounding of an fp32 product.  Six products on the 16-bit matrix pipe take less than half the time of one fp32 product on the fp32 one.
 //
@@ -173,10 +176,8 @@ __host__ __device__ __forceinline__ size_t pad8(int n) { return (size_t)((n + 7)
 // i gets X[4 j + i / 4][i % 4]; the four depths that they gather lie 64 bytes apart).
 // ------------------------------------------------------------------------------------------
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((__vector_size__(4 * sizeof(short))));
-
-template <typename T> struct Mx { typedef T E; static constexpr int P = 1, BK = 64; };
-template <> struct Mx<float> { typedef cg_b16 E; static constexpr int P = 3, BK = 32; };
 
 template <typename E> struct V8 { typedef E V __attribute__((ext_vector_type(8))); };
 __device__ __forceinline__ f32x16 mfma(typename V8<cg_h16>::V a, typename V8<cg_h16>::V b, f32x16 c) {
@@ -187,11 +188,12 @@ __device__ __forceinline__ f32x16 mfma(typename V8<cg_b16>::V a, typename V8<cg_
 }
 
 // One operand of a tile: global -> registers -> LDS, and the fragments of one 16-deep step
-template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
-    typedef typename Mx<T>::E E;
-    typedef typename V8<E>::V Frag;
-    typedef typename CgT<T>::V Raw;
-    static constexpr int P = Mx<T>::P, BK = Mx<T>::BK, W = CgT<T>::N;
+template <int ROWS, int NT, bool KC, bool GATE> struct Operand {
+    typedef float T;
+    typedef cg_b16 E;
+    typedef V8<E>::V Frag;
+    typedef CgT<T>::V Raw;
+    static constexpr int P = 3, BK = 32, W = CgT<T>::N;
     static constexpr int CPR = KC ? BK / W : ROWS / W;             // chunks of W elements per LDS row
     static constexpr int CH = (KC ? ROWS : BK) * CPR / NT;
     static constexpr int PITCH = KC ? BK * 2 : ROWS * 2;           // bytes
@@ -255,14 +257,10 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
     }
     // the elements of a chunk moved down by s, zeros behind (s >= W: all zero)
     static __device__ __forceinline__ Raw moved(Raw v, int s) {
-        typedef unsigned U4 __attribute__((ext_vector_type(4)));
-        U4 u = __builtin_bit_cast(U4, v);
-        const int h = sizeof(T) == 2 ? s : 2 * s;       // in 16-bit units
-        if (h & 4) u = U4{u[2], u[3], 0, 0};
-        if (h & 2) u = U4{u[1], u[2], u[3], 0};
-        if (h & 1) u = U4{u[0] >> 16 | u[1] << 16, u[1] >> 16 | u[2] << 16, u[2] >> 16 | u[3] << 16, u[3] >> 16};
-        if (h >= 8) u = U4{0, 0, 0, 0};
-        return __builtin_bit_cast(Raw, u);
+        if (s & 2) v = Raw{v[2], v[3], 0, 0};
+        if (s & 1) v = Raw{v[1], v[2], v[3], 0};
+        if (s >= W) v = Raw{0, 0, 0, 0};
+        return v;
     }
     // what step k0 loaded, with zeros past K
     __device__ __forceinline__ void fix(Regs& raw, int k0, int K, size_t row0, size_t rows) const {
@@ -280,30 +278,26 @@ template <typename T, int ROWS, int NT, bool KC, bool GATE> struct Operand {
     // where 16-byte chunk `chunk` of LDS row `row` lies in it (a row-contiguous operand's LDS rows are its depths)
     static __device__ __forceinline__ unsigned swz(int row, int chunk) {
         if (!KC) return (unsigned)(chunk ^ (ROWS >= 128 ? (row & 3) << 2 : (row >> 1 & 1) << 2));
-        return BK == 64 ? (unsigned)(chunk ^ ((row >> 1) & 7)) : (unsigned)(chunk ^ ((row >> 2) & 3));
+        return (unsigned)(chunk ^ ((row >> 2) & 3));
     }
     __device__ __forceinline__ void store(char* lds, const Regs& raw) const {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
+            typedef E E4 __attribute__((ext_vector_type(4)));
             const int r = lrow(tid, i), c = lch(tid);
-            if constexpr (P == 1) {
-                *(Frag*)(lds + r * PITCH + swz(r, c) * 16) = __builtin_bit_cast(Frag, raw.q[i]);
-            } else {
-                typedef E E4 __attribute__((ext_vector_type(4)));
-                float x[4];
+            float x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = raw.q[i][e];
-                char* d = lds + r * PITCH + swz(r, c >> 1) * 16 + (c & 1) * 8;
+            for (int e = 0; e < 4; ++e) x[e] = raw.q[i][e];
+            char* d = lds + r * PITCH + swz(r, c >> 1) * 16 + (c & 1) * 8;
 #pragma unroll
-                for (int p = 0; p < 3; ++p) {
-                    E4 h;
+            for (int p = 0; p < P; ++p) {
+                E4 h;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        h[e] = (E)x[e];
-                        x[e] -= (float)h[e];
-                    }
-                    *(E4*)(d + p * PLANE) = h;
+                for (int e = 0; e < 4; ++e) {
+                    h[e] = (E)x[e];
+                    x[e] -= (float)h[e];
                 }
+                *(E4*)(d + p * PLANE) = h;
             }
         }
     }
@@ -410,11 +404,12 @@ __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)
 
 // One LDS buffer, loads one K-step ahead in registers, and three blocks on a CU where the registers allow it (not with the operands of the
 // gate's backward epilogue): 510 us instead of 577 for the gate product of 65536 x 256 x 1024 with two blocks and two steps ahead.
-template <typename T, int BM, int BN, int WM, int WN, bool KA, bool KB, int EPI>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && EPI != EPI_GATE_BWD ? 3 : 2) void gemm_kernel(Gemm<T> g) {
+template <int BM, int BN, int WM, int WN, bool KA, bool KB, int EPI>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && EPI != EPI_GATE_BWD ? 3 : 2) void gemm_kernel(Gemm<float> g) {
+    typedef float T;
     constexpr int NW = (BM / WM) * (BN / WN), NT = NW * 64, TM = WM / 32, TN = WN / 32;
-    typedef Operand<T, BM, NT, KA, false> OA;
-    typedef Operand<T, BN, NT, KB, EPI == EPI_GATE_FWD> OB;
+    typedef Operand<BM, NT, KA, false> OA;
+    typedef Operand<BN, NT, KB, EPI == EPI_GATE_FWD> OB;
     constexpr int P = OA::P, BK = OA::BK, EP = WN + 4, BUF = OA::BYTES + OB::BYTES;
     constexpr int SMEM = BUF > NW * 32 * EP * 4 ? BUF : NW * 32 * EP * 4;
     __shared__ __attribute__((aligned(16))) char smem[SMEM];
@@ -749,22 +744,20 @@ template <typename T, int EPI> __global__ __launch_bounds__(256) void join_kerne
 
 // Operands narrower than one 16-byte chunk (fewer than 4 or 8 channels or hidden units): one output per thread, or per block where K is long.
 template <typename T, int EPI> __device__ __forceinline__ void emit1(const Gemm<T>& g, size_t z, int sel, size_t m, int n, float v, float w) {
-    float u, du;
     const size_t o = (z * g.M + m) * g.ldf + n;
     if (EPI == EPI_STORE) {
         T* c = g.c[sel] + z * g.cz + m * g.N + n;
         v += g.bias[0] ? (float)g.bias[0][z * g.biasz + n] : 0.f;
         *c = (T)(g.accumulate >> sel & 1 ? (float)*c + v : v);
     } else if (EPI == EPI_GATE_FWD) {
-        v = (float)(T)(v + (g.bias[0] ? (float)g.bias[0][z * g.biasz + n] : 0.f));
-        w = (float)(T)(w + (g.bias[1] ? (float)g.bias[1][z * g.biasz + n] : 0.f));
-        gate_fn<sizeof(T) == 4>(v, g.gate, u, du);
+        float u, du;
+        w += g.bias[1] ? (float)g.bias[1][z * g.biasz + n] : 0.f;
+        gate_fn<sizeof(T) == 4>(v + (g.bias[0] ? (float)g.bias[0][z * g.biasz + n] : 0.f), g.gate, u, du);
         g.o0[(z * g.M + m) * g.ld0 + n] = (T)(u * w);
-        if (g.o1) g.o1[o] = (T)v, g.o2[o] = (T)w;
+        if (g.o1) g.o1[o] = (T)u, g.o2[o] = (T)(w * du);
     } else {
-        gate_fn<sizeof(T) == 4>((float)g.i0[o], g.gate, u, du);
-        g.o0[o] = (T)(v * (float)g.i1[o] * du);
-        g.o1[o] = (T)(v * u);
+        g.o0[o] = (T)(v * (float)g.i1[o]);
+        g.o1[o] = (T)(v * (float)g.i0[o]);
     }
 }
 template <typename T, bool KA, bool KB, int EPI, bool BLOCK> __global__ __launch_bounds__(256) void narrow_kernel(Gemm<T> g) {
@@ -808,7 +801,6 @@ template <typename T, bool KA, bool KB, int EPI, bool BLOCK> __global__ __launch
 // multiplied in fp32 (16-bit K-contiguous operands on v_mfma_f32_16x16x32, which takes the 16 bytes as they are).
 // ------------------------------------------------------------------------------------------
 constexpr int FEW_ROWS = 32, FEW_WAVES = 16;
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ f32x4 mfma16(typename V8<cg_h16>::V a, typename V8<cg_h16>::V b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -1079,8 +1071,8 @@ template <typename T, bool KA, bool KB, int EPI> void gemm(Gemm<T>& g, int membe
         if (p.tile == 256) gemm_wide_kernel<T, 256, KA, KB, EPI><<<grid, 512, 0, st>>>(g);
         else gemm_wide_kernel<T, 128, KA, KB, EPI><<<grid, 256, 0, st>>>(g);
     } else {
-        if (p.tile == 128) gemm_kernel<T, 128, 128, 64, 64, KA, KB, EPI><<<grid, 256, 0, st>>>(g);
-        else gemm_kernel<T, 64, 64, 32, 64, KA, KB, EPI><<<grid, 128, 0, st>>>(g);
+        if (p.tile == 128) gemm_kernel<128, 128, 64, 64, KA, KB, EPI><<<grid, 256, 0, st>>>(g);
+        else gemm_kernel<64, 64, 32, 64, KA, KB, EPI><<<grid, 128, 0, st>>>(g);
     }
     if (p.splits > 1) {
         const size_t nb = (g.M * (pad8(g.N) / 8) * nz + 255) / 256;
@@ -1089,25 +1081,20 @@ template <typename T, bool KA, bool KB, int EPI> void gemm(Gemm<T>& g, int membe
 }
 
 // da, dv from a stored gradient of h (no output projection)
-template <typename T> struct GateBwd { const T *dh, *a, *v; T *da, *dv; size_t rows; int F, ldf, gate; };
+template <typename T> struct GateBwd { const T *dh, *u, *p; T *da, *dv; size_t rows; int F, ldf; };
 template <typename T> __global__ __launch_bounds__(256) void gate_bwd_kernel(GateBwd<T> g) {
     const size_t per = g.ldf / 8;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < g.rows * per; i += (size_t)gridDim.x * 256) {
         const size_t m = i / per;
         const int n = (int)(i % per) * 8;
-        float d[8], a[8], v[8];
+        float d[8], u[8], p[8];
         cg_load<T, 8>(g.dh + m * g.F + n, g.F - n, d);       // zeros behind F: da and dv end in zeros
-        cg_load<T, 8>(g.a + m * g.ldf + n, g.F - n, a);
-        cg_load<T, 8>(g.v + m * g.ldf + n, g.F - n, v);
+        cg_load<T, 8>(g.u + m * g.ldf + n, g.F - n, u);
+        cg_load<T, 8>(g.p + m * g.ldf + n, g.F - n, p);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float u, du;
-            gate_fn<sizeof(T) == 4>(a[e], g.gate, u, du);
-            a[e] = d[e] * v[e] * du;
-            v[e] = d[e] * u;
-        }
-        cg_store<T, 8>(g.da + m * g.ldf + n, 8, a);
-        cg_store<T, 8>(g.dv + m * g.ldf + n, 8, v);
+        for (int e = 0; e < 8; ++e) p[e] *= d[e], u[e] *= d[e];
+        cg_store<T, 8>(g.da + m * g.ldf + n, 8, p);
+        cg_store<T, 8>(g.dv + m * g.ldf + n, 8, u);
     }
 }
 
@@ -1166,10 +1153,9 @@ template <typename T> __global__ __launch_bounds__(1024) void colsum_join_kernel
     *o = (T)(g.accumulate >> sel & 1 ? (float)*o + s : s);
 }
 
-constexpr int MAX_WIDTH = 1 << 21;
 bool dims_ok(const cg_gated_dims* d, const cg_group* grp) {
-    return d && d->rows >= 0 && d->rows < INT32_MAX && d->rows % grp_n(grp) == 0 && d->D > 0 && d->F > 0 && d->O >= 0 &&
-           d->D <= MAX_WIDTH && d->F <= MAX_WIDTH && d->O <= MAX_WIDTH &&      // a tile's offsets stay below 2^31 bytes
+    return d && d->rows >= 0 && d->rows <= MAX_ROWS && d->rows % grp_n(grp) == 0 && d->D > 0 && d->F > 0 && d->O >= 0 &&
+           d->D <= MAX_WIDTH && d->F <= MAX_WIDTH && d->O <= MAX_WIDTH &&
            (d->dtype == CG_DT_F32 || d->dtype == CG_DT_F16 || d->dtype == CG_DT_BF16) && d->gate >= 0 && d->gate <= CG_GATE_SIGMOID &&
            (grp_n(grp) == 1 || d->dtype == CG_DT_F32);
 }
@@ -1257,12 +1243,12 @@ size_t bwd_part(const cg_gated_dims* d, const cg_group* grp) {
     return up256(most);
 }
 
-// pitch of a, v, da, dv, and of h where it is not the result: rows on 16 bytes
+// pitch of u, p, da, dv, and of h where it is not the result: rows on 16 bytes
 inline int ldf_of(const cg_gated_dims* d) { return (int)pad8(d->F); }
 
 template <typename T>
 void fwd(const cg_gated_dims* d, const cg_group* grp, const T* x, const T* wg, const T* wv, const T* wo, const T* bg, const T* bv,
-         const T* bo, T* h, T* a, T* v, T* y, void* pack, float* part, hipStream_t st) {
+         const T* bo, T* h, T* u, T* p, T* y, void* pack, float* part, hipStream_t st) {
     const int nz = grp_n(grp), ldf = ldf_of(d);
     const size_t M = d->rows / nz, gs = grp_stride(grp);
     const bool small = M <= FEW_ROWS;
@@ -1273,24 +1259,24 @@ void fwd(const cg_gated_dims* d, const cg_group* grp, const T* x, const T* wg, c
     g.B[0] = op.wg, g.B[1] = op.wv, g.bz = gs, g.ldb = op.ldw;
     g.M = M, g.K = d->D, g.N = d->F, g.gate = d->gate;
     g.bias[0] = bg, g.bias[1] = bv, g.biasz = gs;
-    g.o0 = h, g.o1 = a, g.o2 = v, g.ld0 = d->O ? ldf : d->F, g.ldf = ldf;
+    g.o0 = h, g.o1 = u, g.o2 = p, g.ld0 = d->O ? ldf : d->F, g.ldf = ldf;
     if (small) few<T, true, EPI_GATE_FWD>(g, nz, st);
     else gemm<T, true, true, EPI_GATE_FWD>(g, nz, part, st);
     if (!d->O) return;
-    Gemm<T> p = {};
-    p.nseg = p.nsel = 1;
-    p.A[0] = h, p.az = M * ldf, p.lda = ldf;
-    p.B[0] = op.wo, p.bz = gs, p.ldb = op.ldo;
-    p.M = M, p.K = d->F, p.N = d->O;
-    p.bias[0] = bo, p.biasz = gs;
-    p.c[0] = y, p.cz = M * d->O;
-    if (small) few<T, true, EPI_STORE>(p, nz, st);
-    else gemm<T, true, true, EPI_STORE>(p, nz, part, st);
+    Gemm<T> o = {};
+    o.nseg = o.nsel = 1;
+    o.A[0] = h, o.az = M * ldf, o.lda = ldf;
+    o.B[0] = op.wo, o.bz = gs, o.ldb = op.ldo;
+    o.M = M, o.K = d->F, o.N = d->O;
+    o.bias[0] = bo, o.biasz = gs;
+    o.c[0] = y, o.cz = M * d->O;
+    if (small) few<T, true, EPI_STORE>(o, nz, st);
+    else gemm<T, true, true, EPI_STORE>(o, nz, part, st);
 }
 
 template <typename T>
 void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, const T* wg, const T* wv, const T* wo, const T* h,
-         const T* a, const T* v, T* dx, T* dwg, T* dwv, T* dwo, T* dbg, T* dbv, T* dbo, int acc, void* pack, T* da, T* dv, T* dyp,
+         const T* u, const T* p, T* dx, T* dwg, T* dwv, T* dwo, T* dbg, T* dbv, T* dbo, int acc, void* pack, T* da, T* dv, T* dyp,
          float* part, hipStream_t st) {
     const int nz = grp_n(grp), ldf = ldf_of(d);
     const size_t M = d->rows / nz, gs = grp_stride(grp), D = d->D, F = d->F, O = d->O;
@@ -1311,8 +1297,8 @@ void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, c
             g.nseg = g.nsel = 1;
             g.A[0] = dy, g.az = M * ldy, g.lda = ldy;
             g.B[0] = op.wo, g.bz = gs, g.ldb = op.ldo;
-            g.M = M, g.K = O, g.N = d->F, g.gate = d->gate;
-            g.o0 = da, g.o1 = dv, g.i0 = a, g.i1 = v, g.ldf = ldf;
+            g.M = M, g.K = O, g.N = d->F;
+            g.o0 = da, g.o1 = dv, g.i0 = u, g.i1 = p, g.ldf = ldf;
             if ((dbg || dbv) && !small) g.sums = part;
             if (small) few<T, false, EPI_GATE_BWD>(g, nz, st);
             else gemm<T, true, false, EPI_GATE_BWD>(g, nz, part, st);
@@ -1323,7 +1309,7 @@ void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, c
             }
         } else if (M) {
             const size_t nb = ((size_t)d->rows * (ldf / 8) + 255) / 256;
-            gate_bwd_kernel<T><<<(unsigned)(nb < 16384 ? nb : 16384), 256, 0, st>>>(GateBwd<T>{dy, a, v, da, dv, (size_t)d->rows, d->F, ldf, d->gate});
+            gate_bwd_kernel<T><<<(unsigned)(nb < 16384 ? nb : 16384), 256, 0, st>>>(GateBwd<T>{dy, u, p, da, dv, (size_t)d->rows, d->F, ldf});
         }
     }
     if (dx) {
@@ -1386,16 +1372,16 @@ extern "C" size_t cg_gated_ff_pack_bytes(const cg_gated_dims* d, const cg_group*
 extern "C" size_t cg_gated_ff_fwd_workspace(const cg_gated_dims* d, const cg_group* grp) { return dims_ok(d, grp) ? fwd_part(d, grp) : 0; }
 
 extern "C" int cg_gated_ff_fwd(const cg_gated_dims* d, const cg_group* grp, const void* x, const void* wg, const void* wv, const void* wo,
-                               const void* bg, const void* bv, const void* bo, void* h, void* a, void* v, void* y, void* pack, void* ws,
+                               const void* bg, const void* bv, const void* bo, void* h, void* u, void* p, void* y, void* pack, void* ws,
                                size_t ws_bytes, cg_stream_t stream) {
-    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && !a == !v && (!d->O || wo) && (!d->rows || (x && h && (!d->O || y))),
+    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && !u == !p && (!d->O || wo) && (!d->rows || (x && h && (!d->O || y))),
                  "cg_gated_ff_fwd: bad args");
     const size_t need = fwd_part(d, grp);
     if (ws_bytes < need || (!ws && need) || (!pack && pack_bytes(d, grp, x, wg, wv, wo)))
         return cg_set_error(CG_ERR_WORKSPACE, "cg_gated_ff_fwd: workspace too small");
     if (!d->rows) return CG_OK;
     CG_DISPATCH_DT(d->dtype, T, (fwd<T>(d, grp, (const T*)x, (const T*)wg, (const T*)wv, (const T*)wo, (const T*)bg, (const T*)bv,
-                                        (const T*)bo, (T*)h, (T*)a, (T*)v, (T*)y, pack, (float*)ws, cg_s(stream))));
+                                        (const T*)bo, (T*)h, (T*)u, (T*)p, (T*)y, pack, (float*)ws, cg_s(stream))));
     CG_LAUNCH_CHECK("cg_gated_ff_fwd");
     return CG_OK;
 }
@@ -1408,10 +1394,10 @@ extern "C" size_t cg_gated_ff_bwd_workspace(const cg_gated_dims* d, const cg_gro
 }
 
 extern "C" int cg_gated_ff_bwd(const cg_gated_dims* d, const cg_group* grp, const void* dy, const void* x, const void* wg,
-                               const void* wv, const void* wo, const void* h, const void* a, const void* v, void* dx, void* dwg,
+                               const void* wv, const void* wo, const void* h, const void* u, const void* p, void* dx, void* dwg,
                                void* dwv, void* dwo, void* dbg, void* dbv, void* dbo, int accumulate, const void* pack, void* ws,
                                size_t ws_bytes, cg_stream_t stream) {
-    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && (!d->O || wo) && (!d->rows || (dy && x && a && v && (!d->O || h))),
+    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && (!d->O || wo) && (!d->rows || (dy && x && u && p && (!d->O || h))),
                  "cg_gated_ff_bwd: bad args");
     const size_t need = cg_gated_ff_bwd_workspace(d, grp);
     if (ws_bytes < need || (!ws && need) || (!pack && pack_bytes(d, grp, x, wg, wv, wo)))
@@ -1420,7 +1406,7 @@ extern "C" int cg_gated_ff_bwd(const cg_gated_dims* d, const cg_group* grp, cons
         char* w = (char*)ws;
         T *da = (T*)w, *dv = (T*)(w + bwd_hidden(d)), *dyp = (T*)(w + 2 * bwd_hidden(d));
         float* part = (float*)(w + 2 * bwd_hidden(d) + bwd_dy(d));
-        bwd<T>(d, grp, (const T*)dy, (const T*)x, (const T*)wg, (const T*)wv, (const T*)wo, (const T*)h, (const T*)a, (const T*)v, (T*)dx,
+        bwd<T>(d, grp, (const T*)dy, (const T*)x, (const T*)wg, (const T*)wv, (const T*)wo, (const T*)h, (const T*)u, (const T*)p, (T*)dx,
                (T*)dwg, (T*)dwv, (T*)dwo, (T*)dbg, (T*)dbv, (T*)dbo, accumulate, (void*)pack, da, dv, dyp, part, cg_s(stream));
     });
     CG_LAUNCH_CHECK("cg_gated_ff_bwd");

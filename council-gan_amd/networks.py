@@ -198,6 +198,60 @@ class LinearBlock(nn.Module):
         return ops.linear(x, self.fc.weight, self.fc.bias, act=self.activation_type)
 
 
+class ChannelNorm(nn.Module):
+    """Normalisation over the channels of every row (a vector, a token, a pixel): ops.channel_norm.  `LayerNorm` is the reference's
+    norm over C*H*W of a sample."""
+
+    def __init__(self, num_features, eps=1e-5, bias=True):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(num_features))
+        self.bias = nn.Parameter(torch.zeros(num_features)) if bias else None
+
+    def forward(self, x):
+        return ops.channel_norm(x, self.weight, self.bias, self.eps)
+
+
+class Dropout(nn.Module):
+    """residual + dropout(x): ops.dropout while training, the identity otherwise.  `state` ({seed, step}; seeded from torch's generator
+    unless given) advances with every call and belongs to the state_dict; p = 0 has none.  Calls advance it in the order of their
+    streams: two streams must not run the same module at once."""
+
+    def __init__(self, p=0.0, seed=None):
+        super().__init__()
+        if not 0 <= p < 1:
+            raise ValueError("Dropout: p must be in [0, 1), got %r" % (p,))
+        self.p = p
+        if p > 0:
+            self.register_buffer('state', ops.dropout_state(int(torch.randint(1 << 62, ())) if seed is None else seed, device='cpu'))
+
+    def forward(self, x, residual=None):
+        if self.p > 0 and self.training:
+            return ops.dropout(x, self.p, ops.dropout_key(self.state), residual)
+        return x if residual is None else residual + x
+
+
+class GatedBlock(nn.Module):
+    """x + dropout(gated_feed_forward(channel_norm(x))) over the channels of every row; `hidden` gated units (4 * dim by default)."""
+
+    def __init__(self, dim, hidden=None, activation='silu', dropout=0.0):
+        super().__init__()
+        if activation not in hip.GATE:
+            _unsupported("GatedBlock activation %r" % activation)
+        hidden = 4 * dim if hidden is None else hidden
+        self.activation = activation
+        self.norm = ChannelNorm(dim)
+        self.gate = nn.Linear(dim, hidden)
+        self.value = nn.Linear(dim, hidden)
+        self.out = nn.Linear(hidden, dim)
+        self.drop = Dropout(dropout)
+
+    def forward(self, x):
+        y = ops.gated_feed_forward(self.norm(x), self.gate.weight, self.value.weight, self.out.weight, self.gate.bias, self.value.bias,
+                                   self.out.bias, self.activation)
+        return self.drop(y, x)
+
+
 ##################################################################################
 # Sequential Models
 ##################################################################################
@@ -214,13 +268,17 @@ class ResBlocks(nn.Module):
 
 
 class MLP(nn.Module):
-    """networks.py:432-443."""
+    """networks.py:432-443.  block='gated': the hidden layers are residual GatedBlocks, with `dropout` on what they add."""
 
-    def __init__(self, input_dim, output_dim, dim, n_blk, norm='none', activ='relu'):
+    def __init__(self, input_dim, output_dim, dim, n_blk, norm='none', activ='relu', block='linear', dropout=0.0):
         super().__init__()
+        if block not in ('linear', 'gated'):
+            _unsupported("MLP block %r" % (block,))
+        if dropout and block != 'gated':
+            _unsupported("MLP dropout without gated blocks")
         model = [LinearBlock(input_dim, dim, norm=norm, activation=activ)]
         for _ in range(n_blk - 2):
-            model += [LinearBlock(dim, dim, norm=norm, activation=activ)]
+            model += [GatedBlock(dim, dropout=dropout) if block == 'gated' else LinearBlock(dim, dim, norm=norm, activation=activ)]
         model += [LinearBlock(dim, output_dim, norm='none', activation='none')]
         self.model = nn.Sequential(*model)
 
@@ -407,7 +465,8 @@ class AdaINGen(nn.Module):
                                     res_norm='adain', activ=self.activ, pad_type=pad_type,
                                     num_of_mask_dim_to_add=params['num_of_mask_dim_to_add'])
         self.mlp = MLP(input_dim=style_dim, output_dim=self.get_num_adain_params(self.dec), dim=mlp_dim, n_blk=3,
-                       norm='none', activ=self.activ)
+                       norm='none', activ=self.activ, block=params.get('mlp_block', 'linear'),
+                       dropout=params.get('mlp_dropout', 0.0))
         # column ranges of the MLP output per AdaIN layer, in modules() order (networks.py:303-312):
         # [start, start+C) -> bias ("mean"), [start+C, start+2C) -> weight ("std")
         start = 0

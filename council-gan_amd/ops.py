@@ -1816,7 +1816,8 @@ def _dropout_explain(x, residual, key):
 def gated_feed_forward(x, w_gate, w_value, w_out=None, b_gate=None, b_value=None, b_out=None, act="silu"):
     """(act(x w_gate^T + b_gate) * (x w_value^T + b_value)) w_out^T + b_out over the rows of x; without w_out the gated hidden units
     themselves.  w_gate / w_value [F, D], w_out [O, F] as nn.Linear keeps them, all in x's type; act: 'silu', 'gelu' (error function)
-    or 'sigmoid'.  Between the two products the hidden units (and, for the backward pass, both projections) are held in x's type.  fp32
+    or 'sigmoid'.  Sums, biases and gates are fp32; the hidden units and, for the backward pass, act(a) and v act'(a) (a, v: the two
+    projections) are rounded to x's type once and kept in it.  fp32
     products are six of three bfloat16 parts of either operand (as exact as an fp32 product; an infinite operand gives NaN).  Under
     ops.members(n) (fp32) every member's rows take its own parameters."""
     params = (w_gate, w_value, w_out, b_gate, b_value, b_out)
@@ -1847,8 +1848,8 @@ def _gated_explain(x, w_gate, w_value, w_out, b_gate, b_value, b_out, act):
     for name, p, shape in named:
         if p is not None or name == "w_value":
             _check_param(what, name, p, shape, x, (x.dtype,))
-    if max(D, F, w_out.shape[0] if w_out is not None else 0) > 1 << 21 or x.numel() // D >= (1 << 31) - 1:
-        raise ValueError("%s: at most 2^21 channels or hidden units and 2^31 - 2 rows" % what)
+    if max(D, F, w_out.shape[0] if w_out is not None else 0) > 1 << 21 or x.numel() // D > 1 << 30:
+        raise ValueError("%s: at most 2^21 channels or hidden units and 2^30 rows" % what)
     _check_gpu(what, x)
     raise ValueError("%s: bad arguments" % what)
 

@@ -42,7 +42,7 @@ import torch.nn as nn
 
 from . import hip, ops
 from .hip import check, ptr, stream
-from .networks import AdaINGen, MsImageDis, MsImageDisCouncil
+from .networks import AdaINGen, Dropout, MsImageDis, MsImageDisCouncil
 from .optim import FlatAdam, ParamPool
 from .graphs import HostInputs, Segment
 from .parallel import CouncilShard
@@ -231,6 +231,7 @@ class Council_Trainer(nn.Module):
                     net = self._nets(kind, d)[i]
                     for b in net.buffers():
                         b.data = b.data.to(dev)
+                    self._replica_masks(net)
         # One pool per optimizer kind over this rank's members: member k's parameters / gradients / Adam moments are slice
         # k of the pool's flat tensors, at a uniform stride -- the layout member-batched launches address (optim.ParamPool)
         self._pools = {'gen': ParamPool([self.gen_opt_s[i] for i in local]),
@@ -322,6 +323,11 @@ class Council_Trainer(nn.Module):
         self._iter_serials = {}
         self._iter_eager, self._phase = True, 0
         self._overlap = os.environ.get('CG_OVERLAP_UPDATES', '0' if (self.shard.dp > 1 or self._graph_mode) else '1') != '0'
+        if any(isinstance(m, Dropout) and m.p > 0 for d in self._dirs for i in local for m in self._nets('gen', d)[i].modules()):
+            # every decode advances the mask state of its generator: the updates run in program order, on one stream
+            if self._overlap and 'CG_OVERLAP_UPDATES' in os.environ:
+                raise hip.HipError("gen.mlp_dropout excludes CG_OVERLAP_UPDATES=1")
+            self._overlap = False
         if self._graph_mode and self._overlap:
             raise hip.HipError("CG_GRAPH=1 replays each update on one stream: it excludes CG_OVERLAP_UPDATES=1")
         self._side = [torch.cuda.Stream(device=dev), torch.cuda.Stream(device=dev)] if self._overlap else []
@@ -1332,6 +1338,12 @@ class Council_Trainer(nn.Module):
                 opt.materialize('cpu')
         return torch.device('cpu')
 
+    def _replica_masks(self, net):
+        """Replicas of a member hold the same weights and seeds and see different samples: each draws its own dropout masks."""
+        for m in net.modules():
+            if isinstance(m, Dropout) and m.p > 0 and self.shard.slice_idx:
+                m.state[0] += self.shard.slice_idx
+
     @staticmethod
     def _plain_state(net):
         """state_dict with independent, contiguous (OIHW) tensors: the parameters are channels_last VIEWS into the
@@ -1373,6 +1385,7 @@ class Council_Trainer(nn.Module):
                         continue
                     print('loading: ' + name)
                     self._nets(kind, d)[i].load_state_dict(torch.load(name, map_location=dev)[d])
+                    self._replica_masks(self._nets(kind, d)[i])
                     if kind == 'gen':
                         iterations = int(name[-11:-3])
             try:

@@ -81,7 +81,7 @@ def gate(a, act):
 def gated_ref(x, wg, wv, wo, bg, bv, bo, act, dy):
     """{name: (value, bound without the output's own rounding)}: rows x [M, D], all inputs as the kernel reads them.
 
-    The kernel holds a, v, h, da, dv in x's type (one rounding ut each) and adds in fp32; a product of K terms is off by at most
+    The kernel holds h, u = act(a), p = v act'(a), da and dv in x's type (one rounding ut each) and adds in fp32; a product of K terms is off by at most
     (K + 8) U sum|terms|, 4 more roundings an fp32 product that is put together from parts (its parts below 2^-23 are left out, less than 4 U)."""
     t = x.dtype
     ut, eta = u(t), torch.finfo(t).smallest_normal * u(t)       # one rounding: relative, and half a step of the smallest numbers
@@ -106,7 +106,7 @@ def gated_ref(x, wg, wv, wo, bg, bv, bo, act, dy):
         a = a + bg.double()
     if bv is not None:
         v = v + bv.double()
-    ea, ev = ea + ut * ab(a) + U * ab(a) + eta, ev + ut * ab(v) + U * ab(v) + eta
+    ea, ev = ea + U * ab(a), ev + U * ab(v)
     g, dg = gate(a, act)
     # |act''| <= 1.2 for the three gates; a few roundings of exp / erf (4 U relative each)
     eg, edg = ab(dg) * ea + 1.2 * ea * ea + 16 * U * ab(g), 1.2 * ea + 16 * U * (ab(dg) + 1)
@@ -126,8 +126,11 @@ def gated_ref(x, wg, wv, wo, bg, bv, bo, act, dy):
         out["y"] = (h, eh)
         dh, edh = dy, torch.zeros_like(dy)
     da, dv = dh * v * dg, dh * g
-    eda = edh * ab(v * dg) + ab(dh) * (ev * ab(dg) + ab(v) * edg + ev * edg) + (ut + 4 * U) * ab(da) + eta
-    edv = edh * ab(g) + ab(dh) * eg + edh * eg + (ut + 2 * U) * ab(dv) + eta
+    # u and p as they are kept, then da = dh p and dv = dh u
+    ekp = ev * ab(dg) + ab(v) * edg + ev * edg + (ut + 2 * U) * ab(v * dg) + eta
+    eku = eg + ut * ab(g) + eta
+    eda = edh * ab(v * dg) + ab(dh) * ekp + edh * ekp + (ut + 2 * U) * ab(da) + eta
+    edv = edh * ab(g) + ab(dh) * eku + edh * eku + (ut + 2 * U) * ab(dv) + eta
     p, ep = lin(da, wg.t().contiguous(), dp=eda)
     q, eq = lin(dv, wv.t().contiguous(), dp=edv)
     out["dx"] = (p + q, ep + eq + (F + 12) * U * (ab(p) + ab(q)))

@@ -17,8 +17,9 @@ def pytest_configure(config):
 
 # Cheap, wide parity first; the heaviest full-width runs last -- with `-x` one fault must not hide the operator suite
 # (round 4: an abort in the graph test, then tenth in line, cost the driver's run 190 tests).
-_ORDER = ["test_host_cpu", "test_channel_mlp_cpu", "test_oracle_golden", "test_ref_interop_cpu", "test_parallel_gloo",
-          "test_gpu_ops", "test_gpu_channel_mlp", "test_gpu_golden", "test_gpu_parity_full", "test_gpu_parity_targets", "test_gpu_tools",
+_ORDER = ["test_host_cpu", "test_channel_mlp_cpu", "test_channel_blocks_cpu", "test_oracle_golden", "test_ref_interop_cpu", "test_parallel_gloo",
+          "test_gpu_ops", "test_gpu_channel_mlp", "test_gpu_channel_blocks", "test_gpu_golden",
+          "test_gpu_parity_full", "test_gpu_parity_targets", "test_gpu_tools",
           "test_gpu_world", "test_gpu_graph", "test_gpu_stress", "test_gpu_perf"]
 
 
