@@ -280,14 +280,15 @@ template <int ROWS, int NT, bool KC, bool GATE> struct Operand {
         if (!KC) return (unsigned)(chunk ^ (ROWS >= 128 ? (row & 3) << 2 : (row >> 1 & 1) << 2));
         return (unsigned)(chunk ^ ((row >> 2) & 3));
     }
-    __device__ __forceinline__ void store(char* lds, const Regs& raw) const {
+    // FLIP: rows 32 .. 63 of every 64 with the other sign (gemm_kernel)
+    template <bool FLIP> __device__ __forceinline__ void store(char* lds, const Regs& raw) const {
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             typedef E E4 __attribute__((ext_vector_type(4)));
             const int r = lrow(tid, i), c = lch(tid);
             float x[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = raw.q[i][e];
+            for (int e = 0; e < 4; ++e) x[e] = FLIP && (i * (NT / CPR) >> 5 & 1) ? -raw.q[i][e] : raw.q[i][e];
             char* d = lds + r * PITCH + swz(r, c >> 1) * 16 + (c & 1) * 8;
 #pragma unroll
             for (int p = 0; p < P; ++p) {
@@ -402,6 +403,9 @@ __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)
     }
 }
 
+// The matrix pipe cuts its sums off downwards a few bits below fp32, so every result is low by some 1e-7 of its size, and a sum of 65536
+// of them (a bias gradient) by 1.4e-6, where its random errors come to 4e-7.  So half of A's rows go through with the other sign: the
+// errors of neighbouring row blocks cancel in any sum over rows (no time is lost by it).
 // One LDS buffer, loads one K-step ahead in registers, and three blocks on a CU where the registers allow it (not with the operands of the
 // gate's backward epilogue): 510 us instead of 577 for the gate product of 65536 x 256 x 1024 with two blocks and two steps ahead.
 template <int BM, int BN, int WM, int WN, bool KA, bool KB, int EPI>
@@ -444,8 +448,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && EPI != EPI
         const int k0 = (g.nseg == 2 && step >= kt ? step - kt : step) * BK;
         a.fix(ra, k0, (int)g.K, m0, g.M);
         b.fix(rb, k0, (int)g.K, n0, g.N);
-        a.store(smem, ra);
-        b.store(smem + OA::BYTES, rb);
+        a.template store<KA>(smem, ra);
+        b.template store<false>(smem + OA::BYTES, rb);
     };
     auto compute = [&](const char* from) {
 #pragma unroll
@@ -480,6 +484,12 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && EPI != EPI
         }
     }
 
+    if (KA)
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+            if ((wm / 32 + i) & 1)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = -acc[i][j];
     // the accumulators leave through LDS
     __syncthreads();
     store_tile<T, EPI, TM, TN>(g, acc, (float*)smem + wid * 32 * EP, lane, m0 + wm, n0 + (EPI == EPI_GATE_FWD ? wn / 2 : wn), z, sel,

@@ -330,6 +330,24 @@ def test_gated_feed_forward_gradient_against_differences(cga):
         assert abs(got - want) < 96 * (e * e * 100 + 40 * R.U / (2 * e)), (k, got, want)
 
 
+def test_gated_feed_forward_errors_have_no_common_sign(cga):
+    """Errors that share a sign grow with the rows in a bias gradient: the mean error over many rows is far below one rounding."""
+    g = gen(41)
+    M, D, F = 8192, 512, 96
+    x, ps, dy = gated_inputs(g, M, D, F, 64, True, F32)
+    h = cga.ops.gated_feed_forward(x, ps[0], ps[1], None, ps[3], ps[4])
+    x64, wg, wv, bg, bv = (t.double() for t in (x, ps[0], ps[1], ps[3], ps[4]))
+    v = x64 @ wv.t().contiguous() + bv
+    h64 = R.gate(x64 @ wg.t().contiguous() + bg, "silu")[0] * v
+    err = (h.double() - h64).mean(0) / h64.square().mean(0).sqrt()
+    # A product of K = 512 is 6 * 512 / 16 = 192 additions to a running sum that grows to the result (0.7 of its size on average), each off
+    # by up to half a step, 2^-24 of what it rounds, evenly: 192^0.5 / 3^0.5 * 0.7 * 2^-24 = 3.3e-7 of the result.  Gate and value together
+    # 2^0.5 of that, their mean over 8192 rows 1 / 90.5 of it: 5.2e-9, and the largest of 96 columns stays below 5 times that, 2.6e-8.
+    assert float(err.abs().max()) < 2.0 ** -25
+    # over all columns the mean's spread is 5.2e-9 / 96^0.5 = 5.3e-10; 2^-28 is 7 times that
+    assert float(err.mean().abs()) < 2.0 ** -28
+
+
 def test_results_do_not_change_from_call_to_call(cga):
     for dtype in DTYPES:
         x, ps, dy = gated_inputs(gen(10), 2100, 200, 300, 100, True, dtype)
