@@ -8,11 +8,13 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <array>
@@ -88,7 +90,7 @@ struct Buffer {
     }
 };
 
-struct Target { Tensor out, ret; bool add = false; };       // what the kernel writes, what the node returns
+struct Target { Tensor out, ret, shared; bool add = false; };       // what the kernel writes, what the node returns
 Target target(const Tensor& p, const Buffer& buf, bool wanted, int members) {
     Target r;
     if (!p.defined() || !wanted) return r;
@@ -101,6 +103,38 @@ Target target(const Tensor& p, const Buffer& buf, bool wanted, int members) {
     TORCH_CHECK(members == 1, "member-batched backward needs the pool's gradient buffers");
     r.out = r.ret = at::empty(p.sizes(), p.options());
     return r;
+}
+
+// Targets that share a buffer (a tensor that serves as two parameters): all but the first get memory of their own, since one launch may
+// write them side by side; `settle` adds it to the buffer.
+template <size_t N> void separate(std::array<Target, N>& t, int members) {
+    for (size_t i = 1; i < N; ++i)
+        for (size_t j = 0; j < i; ++j)
+            if (t[i].add && t[j].out.defined() && t[i].out.data_ptr() == t[j].out.data_ptr()) {
+                TORCH_CHECK(members == 1, "member-batched backward: one parameter is used twice in a call");
+                t[i].shared = t[i].out;
+                t[i].out = at::empty_like(t[i].shared);
+                t[i].add = false;
+                break;
+            }
+}
+template <size_t N> void settle(const std::array<Target, N>& t) {
+    for (const Target& x : t)
+        if (x.shared.defined()) Tensor(x.shared).add_(x.out);
+}
+
+// A backward pass captured into a graph must not meet a gradient accumulator that an eager graph holds: it belongs to that graph's
+// stream, which the engine would make wait for the capture, and the capture (or the process) ends with that.
+void refuse_eager_graph(const char* what, std::initializer_list<std::pair<const Tensor*, const Buffer*>> leaves) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const auto& [t, buf] : leaves) {
+        if (!grad_on(*t) || !t->is_leaf() || (buf && buf->t.defined())) continue;
+        const auto acc = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!acc) continue;
+        const auto st = acc->stream();
+        TORCH_CHECK(!st || st->id() == c10::hip::getCurrentHIPStream(t->device().index()).id(), what,
+                    ": captured while an eager graph of the same leaves lives: drop what it computed first");
+    }
 }
 
 struct Members {
@@ -128,20 +162,23 @@ struct ChannelNorm : public torch::autograd::Node {
         variable_list out(3);
         if (!grads[0].defined()) return out;
         const Tensor x = x_.unpack(), w = w_.unpack(), dy = dense(grads[0]);
-        const size_t C = w.numel(), rows = x.numel() / C;
+        const size_t C = w.numel(), rows = stats_.size(1);
+        TORCH_CHECK((size_t)x.numel() == rows * C && dy.numel() == x.numel(), "channel_norm: an input changed its size since the forward pass");
         const bool need_w = task_should_compute_output(1), need_b = b_.defined() && task_should_compute_output(2);
         Tensor dx;
         if (task_should_compute_output(0)) out[0] = dx = at::empty_like(x);
-        Target dw = target(w, wbuf, need_w, members.g.n), db = target(b_, bbuf, need_b, members.g.n);
+        std::array<Target, 2> t{target(w, wbuf, need_w, members.g.n), target(b_, bbuf, need_b, members.g.n)};
+        separate(t, members.g.n);
         const int dt = dt_of(x.scalar_type()), wdt = dt_of(w.scalar_type());
         const size_t nws = need_w || need_b ? api.norm_bwd_ws(members.get(), rows, (int)C, dt) : 0;
         const Tensor ws = scratch(nws, x);
         float* st = (float*)stats_.data_ptr();
-        check(api.norm_bwd(members.get(), ptr(dy), ptr(x), ptr(w), st, st + rows, ptr(dx), ptr(dw.out), ptr(db.out), dw.add | db.add << 1,
+        check(api.norm_bwd(members.get(), ptr(dy), ptr(x), ptr(w), st, st + rows, ptr(dx), ptr(t[0].out), ptr(t[1].out), t[0].add | t[1].add << 1,
                            rows, (int)C, dt, wdt, ptr(ws), nws, stream_of(x)),
               "cg_channel_norm_bwd");
-        out[1] = dw.ret;
-        out[2] = db.ret;
+        settle(t);
+        out[1] = t[0].ret;
+        out[2] = t[1].ret;
         return out;
     }
 };
@@ -171,6 +208,7 @@ py::object channel_norm(const Tensor& x, const Tensor& w, const std::optional<Te
         const size_t rows = x.numel() / C;
         {
             const at::NoGradGuard plain;
+            if (record) refuse_eager_graph("channel_norm", {{&x, nullptr}, {&w, &node->wbuf}, {&b, &node->bbuf}});
             xd = dense(x);
             wd = w.contiguous();
             if (b.defined()) bd = b.contiguous();
@@ -229,7 +267,9 @@ py::object dropout(const Tensor& x, const std::optional<Tensor>& residual, int t
         py::gil_scoped_release unlock;
         const c10::DeviceGuard device(x.device());
         {
+            const bool record = c10::GradMode::is_enabled();
             const at::NoGradGuard plain;
+            if (record) refuse_eager_graph("dropout", {{&x, nullptr}, {&res, nullptr}});
             const Tensor xd = dense(x), rd = res.defined() ? dense(res) : res;
             y = at::empty_like(xd);
             check(api.dropout(ptr(xd), ptr(rd), ptr(y), xd.numel(), threshold, ptr(key), dt, stream_of(x)), "cg_dropout");
@@ -255,6 +295,7 @@ struct Gated : public torch::autograd::Node {
     cg_gated_dims dims{};
     Members members;
     std::array<Buffer, 6> bufs;
+    std::array<void*, 4> read{};      // x, wg, wv, wo as the forward pass read them
 
     std::string name() const override { return "GatedFeedForward"; }
     void release_variables() override {
@@ -272,6 +313,9 @@ struct Gated : public torch::autograd::Node {
         if (!grads[0].defined()) return out;
         const Tensor x = x_.unpack(), dy = dense(grads[0]);
         const std::array<Tensor, 6> p{wg_.unpack(), wv_.unpack(), dims.O ? wo_.unpack() : Tensor(), biases[0], biases[1], biases[2]};
+        // (pack_ holds copies of those that needed one)
+        TORCH_CHECK((read == std::array<void*, 4>{ptr(x), ptr(p[0]), ptr(p[1]), ptr(p[2])}) && x.numel() == dims.rows * dims.D,
+                    "gated_feed_forward: an operand moved since the forward pass");
         Tensor dx;
         if (task_should_compute_output(0)) out[0] = dx = at::empty_like(x);
         std::array<void*, 6> to;
@@ -279,9 +323,12 @@ struct Gated : public torch::autograd::Node {
         std::array<Target, 6> t;
         for (int i = 0; i < 6; ++i) {
             t[i] = target(p[i], bufs[i], task_should_compute_output(1 + i), members.g.n);
+            out[1 + i] = t[i].ret;
+        }
+        separate(t, members.g.n);
+        for (int i = 0; i < 6; ++i) {
             to[i] = ptr(t[i].out);
             add |= t[i].add << i;
-            out[1 + i] = t[i].ret;
         }
         const size_t nws = api.gated_bwd_ws(&dims, members.get());
         const Tensor ws = scratch(nws, x);
@@ -290,6 +337,7 @@ struct Gated : public torch::autograd::Node {
         check(api.gated_bwd(&dims, members.get(), ptr(dy), ptr(x), ptr(p[0]), ptr(p[1]), ptr(p[2]), ptr(h_), u, vd, ptr(dx), to[0], to[1], to[2],
                             to[3], to[4], to[5], add, ptr(pack_), ptr(ws), nws, stream_of(x)),
               "cg_gated_ff_bwd");
+        settle(t);
         return out;
     }
 };
@@ -303,7 +351,8 @@ py::object gated(const Tensor& x, const Tensor& wg, const Tensor& wv, const std:
     const int dt = dt_of(x.scalar_type());
     auto like = [&](const Tensor& t) { return t.scalar_type() == x.scalar_type() && t.device() == x.device(); };
     if (!x.is_cuda() || dt < 0 || gate < 0 || wg.dim() != 2 || wv.dim() != 2 || wg.sizes() != wv.sizes() || !like(wg) || !like(wv) ||
-        channels(x) != wg.size(1) || wg.size(0) < 1 || wg.size(1) < 1 || wg.size(0) > MAX_WIDTH || wg.size(1) > MAX_WIDTH || x.numel() / wg.size(1) > 1 << 30)
+        channels(x) != wg.size(1) || wg.size(0) < 1 || wg.size(1) < 1 || wg.size(0) > MAX_WIDTH || wg.size(1) > MAX_WIDTH ||
+        x.numel() / wg.size(1) > 1 << 30)
         return py::none();
     const int64_t F = wg.size(0), D = wg.size(1);
     if (wo.defined() && (wo.dim() != 2 || wo.size(1) != F || wo.size(0) < 1 || wo.size(0) > MAX_WIDTH || !like(wo))) return py::none();
@@ -331,6 +380,9 @@ py::object gated(const Tensor& x, const Tensor& wg, const Tensor& wv, const std:
         cg_gated_dims dims{rows, (int32_t)D, (int32_t)F, (int32_t)O, dt, gate, 0};
         {
             const at::NoGradGuard plain;
+            if (record)
+                refuse_eager_graph("gated_feed_forward", {{&x, nullptr}, {&wg, &node->bufs[0]}, {&wv, &node->bufs[1]}, {&wo, &node->bufs[2]},
+                                                          {&b[0], &node->bufs[3]}, {&b[1], &node->bufs[4]}, {&b[2], &node->bufs[5]}});
             xd = dense(x);
             for (Tensor& t : p)
                 if (t.defined()) t = t.contiguous();
@@ -366,6 +418,7 @@ py::object gated(const Tensor& x, const Tensor& wg, const Tensor& wv, const std:
             node->pack_ = pack;
             node->dims = dims;
             node->members = members;
+            node->read = {ptr(xd), ptr(p[0]), ptr(p[1]), ptr(p[2])};
             if (!O) y = h;
             torch::autograd::set_history(y, node);
         } else if (!O) {

@@ -49,10 +49,10 @@ def norm_ref(x, w, b, eps, dy):
 
 
 # -- dropout -----------------------------------------------------------------------------------
-def keep_mask(n, p, seed, step):
-    """numpy restatement of the draw: Philox4x32-10 (Salmon et al., 2011), 16 bits an element."""
+def keep_mask(n, p, seed, step, first=0):
+    """numpy restatement of the draw: Philox4x32-10 (Salmon et al., 2011), 16 bits an element; n elements from `first` (a multiple of 8)."""
     import numpy as np
-    b = np.arange((n + 7) // 8, dtype=np.uint64)
+    b = np.arange((n + 7) // 8, dtype=np.uint64) + np.uint64(first // 8)
     m32 = np.uint64(0xffffffff)
     seed, step = np.uint64(seed & (2 ** 64 - 1)), np.uint64(step & (2 ** 64 - 1))
     c = [b & m32, b >> np.uint64(32), np.full_like(b, step & m32), np.full_like(b, step >> np.uint64(32))]

@@ -348,6 +348,57 @@ def test_gated_feed_forward_errors_have_no_common_sign(cga):
     assert float(err.mean().abs()) < 2.0 ** -28
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ID.get)
+@pytest.mark.parametrize("rows", [31, 32, 33, 34])
+def test_gated_feed_forward_where_few_rows_end(cga, rows, dtype):
+    x, ps, dy = gated_inputs(gen(rows), rows, 72, 136, 40, True, dtype)
+    gated_case(cga, x, ps, dy, "silu")
+
+
+# ------------------------------------------------------------------------------------------
+# more than 2^32 elements: the rows at the end are those of a small call, or what the formula gives
+# ------------------------------------------------------------------------------------------
+def huge(rows, C, seed):
+    """bf16 rows; the last 64 of their own"""
+    x = torch.empty(rows, C, dtype=BF16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(seed))
+    assert x.numel() > 2 ** 32
+    return x
+
+
+def test_channel_norm_past_32_bits(cga):
+    C = 2056
+    x, dy = huge(2 ** 21 + 7, C, 1).requires_grad_(True), huge(2 ** 21 + 7, C, 2)
+    g = gen(1)
+    w, b = rnd(g, C, shift=1.0, scale=0.3, dtype=BF16), rnd(g, C, scale=0.3, dtype=BF16)
+    y = cga.ops.channel_norm(x, w, b)
+    dx, = torch.autograd.grad(y, x, dy)
+    ref = R.norm_ref(x[-64:].detach(), w, b, 1e-5, dy[-64:])
+    R.check("y", y[-64:], *ref["y"])
+    R.check("dx", dx[-64:], *ref["dx"])
+
+
+def test_dropout_past_32_bits(cga):
+    x = huge(2 ** 21 + 7, 2056, 3)
+    y = cga.ops.dropout(x, 0.25, key_of(5, 6))
+    n, tail = x.numel(), 4096
+    keep = R.keep_mask(tail, 0.25, 5, 6, first=n - tail).cuda()
+    v = torch.where(keep, x.view(-1)[-tail:].double() * R.scale_of(0.25), torch.zeros((), dtype=torch.float64, device="cuda"))
+    R.check("y", y.view(-1)[-tail:], v, 2 * R.U * v.abs())
+
+
+def test_gated_feed_forward_past_32_bits(cga):
+    rows, D, F = 2 ** 22 + 5, 8, 1032          # the hidden units pass 2^32 elements
+    g = gen(4)
+    x, ps, _ = gated_inputs(g, 1, D, F, D, True, BF16)
+    x = torch.empty(rows, D, dtype=BF16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(4)).requires_grad_(True)
+    dy = torch.empty(rows, D, dtype=BF16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(5))
+    y = cga.ops.gated_feed_forward(x, *ps)
+    dx, = torch.autograd.grad(y, x, dy)
+    ref = R.gated_ref(x[-64:].detach(), *ps, "silu", dy[-64:])
+    R.check("y", y[-64:], *ref["y"])
+    R.check("dx", dx[-64:], *ref["dx"])
+
+
 def test_results_do_not_change_from_call_to_call(cga):
     for dtype in DTYPES:
         x, ps, dy = gated_inputs(gen(10), 2100, 200, 300, 100, True, dtype)
@@ -509,6 +560,58 @@ def test_gradients_add_to_the_optimizer_buffers(cga):
     for a, t in zip(once, p):
         # the second pass adds the same value again: 2 a exactly
         assert torch.equal(t.grad, 2 * a)
+
+
+def test_one_buffer_for_two_parameters(cga):
+    """A tensor that serves as two parameters gets the sum of both gradients in its one buffer."""
+    g = gen(32)
+    D = 48
+    (p,), pool = pooled(cga, 1, D, D, g)
+    w, wg, b = p[0], p[2], p[5]
+    x, dy = rnd(g, 70, D), rnd(g, 70, D)
+
+    def run(leaf_w, leaf_g, leaf_b):
+        return cga.ops.gated_feed_forward(cga.ops.channel_norm(x, leaf_w[0], leaf_w[1]), *leaf_g, *leaf_b)
+    run((w, w), (wg, wg, wg), (b, b, b)).backward(dy)
+    apart = [[t.detach().clone().requires_grad_(True) for _ in range(k)] for t, k in ((w, 2), (wg, 3), (b, 3))]
+    grads = torch.autograd.grad(run(*apart), [t for ts in apart for t in ts], dy)
+    for t, gs in ((w, grads[:2]), (wg, grads[2:5]), (b, grads[5:])):
+        want = sum(v.double() for v in gs)
+        # the same gradients, added in fp32: two more roundings of partial sums
+        tol = 3 * R.U * sum(v.double().abs() for v in gs)
+        assert bool(((t._cg_grad.double() - want).abs() <= tol).all())
+
+
+def test_an_operand_that_moved_is_refused(cga):
+    x, ps, dy = gated_inputs(gen(33), 40, 33, 47, 31, False, F16)
+    leaves = [t.requires_grad_(True) for t in ps[:3]]
+    y = cga.ops.gated_feed_forward(x, *leaves)
+    leaves[1].data = leaves[1].detach().clone()
+    with pytest.raises(RuntimeError, match="moved since"):
+        y.backward(dy)
+
+
+def test_capture_beside_a_living_eager_graph_is_refused(cga):
+    x, ps, dy = gated_inputs(gen(34), 40, 32, 48, 32, False, F32)
+    w = torch.ones(32, device="cuda", requires_grad=True)
+    leaves = [t.requires_grad_(True) for t in ps[:3]]
+    ops = [lambda: cga.ops.gated_feed_forward(x, *leaves), lambda: cga.ops.channel_norm(x, w),
+           lambda: cga.ops.dropout(w, 0.5, key)]
+    key = key_of(1, 2)
+    alive = [f() for f in ops]
+    gr = torch.cuda.CUDAGraph()
+    refused = []
+    with torch.cuda.graph(gr):
+        for f in ops:
+            try:
+                f()
+            except RuntimeError as e:
+                refused.append("eager graph of the same leaves" in str(e))
+        with torch.no_grad():
+            y = cga.ops.channel_norm(x, w)          # no gradient, no objection
+    assert refused == [True] * 3
+    gr.replay()
+    assert torch.equal(y, alive[1])
 
 
 def test_member_batched_refusals(cga):
