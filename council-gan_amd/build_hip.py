@@ -29,10 +29,11 @@ OUT_DIR = os.path.join(HERE, "lib")
 OBJ_DIR = os.path.join(OUT_DIR, "obj")
 OUT = os.path.join(OUT_DIR, "libcouncilgan_hip.so")
 STAMP = OUT + ".stamp"
-CFLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result"] + os.environ.get("CG_HIPCC_FLAGS", "").split()
-FLAGS = CFLAGS + ["-shared"]
 # no packed fp32 arithmetic: some of its forms have given wrong results on this hardware now and then
-UNIT_FLAGS = {u: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-inline-asm"] for u in CHANNEL_UNITS}
+CFLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result", "-Xclang", "-target-feature", "-Xclang",
+          "-packed-fp32-ops"] + os.environ.get("CG_HIPCC_FLAGS", "").split()
+FLAGS = CFLAGS + ["-shared"]
+UNIT_FLAGS = {u: ["-Wno-inline-asm"] for u in CHANNEL_UNITS}
 
 
 def _digest(paths=DEPS):
