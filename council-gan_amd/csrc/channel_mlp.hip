@@ -17,6 +17,8 @@ inline size_t grp_stride(const cg_group* g) { return g && g->n > 1 ? (size_t)g->
 // one reading of x and dy; the blocks' sums are then joined in block order (the same result on every run).
 // Rows of any width: the last chunk of a row is moved back to end with the row; the elements that it shares with its neighbour are
 // masked out of the sums, and both lanes store the same value for them.
+// Bound by memory: 65536 x 256 fp32 forward 22 us (6.0 TB/s), backward 35 us (5.8 TB/s) and 4 us to join; 16384 x 4096 bf16 46 us
+// (5.9 TB/s), 85 us (4.7 TB/s) and 5 us.
 // ------------------------------------------------------------------------------------------
 constexpr int NT = 256;
 
@@ -69,6 +71,7 @@ template <typename T, int TPR, int NV> struct Columns {
     }
     __device__ __forceinline__ bool mine(int j, int e) const { return e >= first[j]; }
     __device__ __forceinline__ bool any(int j) const { return first[j] < W; }
+    __device__ __forceinline__ bool shares(int j) const { return first[j] > 0 && first[j] < W; }
 };
 
 template <typename T, typename W_, int TPR, int NV>
@@ -168,28 +171,40 @@ __global__ __launch_bounds__(NT) void channel_norm_bwd_kernel(Norm<T, W_> n) {
         nr = n.rstd[r];
     };
     if (rows) fetch((size_t)blockIdx.x * RPB + g);
+    // dy goes into the sums with zeros in the elements that are not the thread's own (a mask on the raw chunk: the sums themselves take no
+    // selects, which were half of the loop's instructions), and as it is into the dx that a shared chunk stores
+    typedef unsigned Bits __attribute__((ext_vector_type(4)));
     float wv[NV][W], sw[NV][W] = {}, sb[NV][W] = {};
+    Bits own[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) cg_load<W_, W>(w + col.at[j], W, wv[j]);
+    for (int j = 0; j < NV; ++j) {
+        cg_load<W_, W>(w + col.at[j], W, wv[j]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            own[j][k] = W == 4 ? (col.mine(j, k) ? ~0u : 0u) : (col.mine(j, 2 * k) ? 0xffffu : 0u) | (col.mine(j, 2 * k + 1) ? 0xffff0000u : 0u);
+    }
     for (size_t i0 = (size_t)blockIdx.x * RPB; i0 < rows; i0 += step) {
         const size_t i = i0 + g;
         const bool live = i < rows;
         const float m = nm, rs = nr;
         float v[NV][W], d[NV][W], s[2] = {0.f, 0.f};
+        V raw[NV];
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+            raw[j] = nd[j];
+            if (!live) raw[j] = V{};
+            const V md = __builtin_bit_cast(V, __builtin_bit_cast(Bits, raw[j]) & own[j]);
 #pragma unroll
             for (int e = 0; e < W; ++e) {
                 v[j][e] = ((float)nx[j][e] - m) * rs;
-                d[j][e] = (float)nd[j][e];
-                if (live && col.mine(j, e)) {
-                    sw[j][e] += d[j][e] * v[j][e];
-                    sb[j][e] += d[j][e];
-                }
+                d[j][e] = (float)md[e];
+                sw[j][e] += d[j][e] * v[j][e];
+                sb[j][e] += d[j][e];
                 d[j][e] *= wv[j][e];
-                s[0] += col.mine(j, e) ? d[j][e] : 0.f;
-                s[1] += col.mine(j, e) ? d[j][e] * v[j][e] : 0.f;
+                s[0] += d[j][e];
+                s[1] += d[j][e] * v[j][e];
             }
+        }
         if (i0 + step < rows) fetch(i + step);
         if (dx) {
             row_sum<TPR, 2>(s, sm);
@@ -197,6 +212,9 @@ __global__ __launch_bounds__(NT) void channel_norm_bwd_kernel(Norm<T, W_> n) {
             if (live)
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
+                    if (col.shares(j))
+#pragma unroll
+                        for (int e = 0; e < W; ++e) d[j][e] = (float)raw[j][e] * wv[j][e];
 #pragma unroll
                     for (int e = 0; e < W; ++e) d[j][e] = rs * (d[j][e] - s1 - v[j][e] * s2);
                     if (col.any(j)) cg_store<T>(dx + (row0 + i) * C + col.at[j], W, d[j]);
@@ -373,6 +391,7 @@ NormKind norm_kind(int C, int esz) {
     if (C < W) return {0, 0};
     const int ch = (C + W - 1) / W;
     if (ch <= 16) return {16, 1};
+    if (ch <= 32) return {32, 1};
     if (ch <= 64) return {64, 1};
     if (ch <= 128) return {64, 2};
     if (ch <= 256) return {64, 4};
@@ -380,12 +399,15 @@ NormKind norm_kind(int C, int esz) {
     if (ch <= 1024) return {256, 4};
     return {0, 0};
 }
-// blocks of the backward pass = partial sums to join: enough to fill the chip, at least 4 rows for every row group
+// blocks of the backward pass = partial sums to join: at least 4 rows for every row group, and no more blocks than the chip holds at once
+// (the more chunks a thread has, the fewer): 16384 x 8192 bf16, 4 chunks, 156 us with 256 blocks, 171 with 512, 195 with 1024; 40000 x 2048
+// fp32, 2 chunks, 180 with 512, 259 with 256, 196 with 1024; 65536 x 256 fp32, 1 chunk, 35 with 1024, 57 with 256.
 int norm_blocks(size_t rows, int C, int esz) {
     const NormKind k = norm_kind(C, esz);
     if (!k.tpr) return (int)(rows < 1 ? 1 : (rows + 63) / 64 > 256 ? 256 : (rows + 63) / 64);
     const size_t b = (rows + NT / k.tpr * 4 - 1) / (NT / k.tpr * 4);
-    return (int)(b < 1 ? 1 : b > 1024 ? 1024 : b);
+    const size_t most = 1024 / k.nv;
+    return (int)(b < 1 ? 1 : b > most ? most : b);
 }
 
 template <typename T, typename W, int TPR, int NV> void norm_fwd(const Norm<T, W>& g, int members, hipStream_t st) {
@@ -398,6 +420,7 @@ template <typename T, typename W, int TPR, int NV> void norm_bwd(const Norm<T, W
 #define CG_NORM_KIND(kind, F, ...)                             \
     do {                                                       \
         if ((kind).tpr == 16) F<T, W, 16, 1>(__VA_ARGS__);     \
+        else if ((kind).tpr == 32) F<T, W, 32, 1>(__VA_ARGS__); \
         else if ((kind).tpr == 64) {                           \
             if ((kind).nv == 1) F<T, W, 64, 1>(__VA_ARGS__);   \
             else if ((kind).nv == 2) F<T, W, 64, 2>(__VA_ARGS__); \
