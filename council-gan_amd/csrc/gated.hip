@@ -32,6 +32,7 @@ template <typename T> struct Gemm {
     int gate;
     T *o0, *o1, *o2;          // EPI_GATE_FWD: h and, for the backward pass, u = act(a) and p = v act'(a); EPI_GATE_BWD: da, dv
     const T *i0, *i1;         // EPI_GATE_BWD: u, p
+    unsigned short* low;      // 16 bit: the third bytes of u and p (keep)
     int ld0, ldf;             // pitch of h; of u, p, da, dv.  A pitch beyond N is a multiple of 8 and its columns get zeros
     float* sums;              // EPI_GATE_BWD, or NULL: column sums of da and dv over a wave's rows, [member][2][strips][N]
     int strips;
@@ -82,6 +83,31 @@ template <bool FP32> __device__ __forceinline__ void gate_fn(float a, int gate, 
     }
 }
 
+// 16-bit types keep u and p for the backward pass as the upper 24 bits of their fp32 values: a plane of upper halves each, and one of both
+// third bytes.  Rounded to 16 bits they would put another full rounding into da and dv (the gradients 1.7 output roundings off instead
+// of 1.4); the third plane costs no time that can be measured (16384 x 2048 x 5632 bf16: 3048 us either way).  Cutting off is below 2^-15.
+__device__ __forceinline__ unsigned bits(float x) { return __builtin_bit_cast(unsigned, x); }
+__device__ __forceinline__ float from(unsigned x) { return __builtin_bit_cast(float, x); }
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void keep(const float (&u)[8], const float (&p)[8], u32x4& hu, u32x4& hp, u32x4& low) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const unsigned u0 = bits(u[2 * k]), u1 = bits(u[2 * k + 1]), p0 = bits(p[2 * k]), p1 = bits(p[2 * k + 1]);
+        hu[k] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+        hp[k] = __builtin_amdgcn_perm(p1, p0, 0x07060302u);
+        low[k] = __builtin_amdgcn_perm(p0, u0, 0x0c0c0501u) | __builtin_amdgcn_perm(p1, u1, 0x05010c0cu);
+    }
+}
+__device__ __forceinline__ void recall(float (&u)[8], float (&p)[8], const u32x4& hu, const u32x4& hp, const u32x4& low) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        u[2 * k] = from(__builtin_amdgcn_perm(hu[k], low[k], 0x0504000cu));
+        u[2 * k + 1] = from(__builtin_amdgcn_perm(hu[k], low[k], 0x0706020cu));
+        p[2 * k] = from(__builtin_amdgcn_perm(hp[k], low[k], 0x0504010cu));
+        p[2 * k + 1] = from(__builtin_amdgcn_perm(hp[k], low[k], 0x0706030cu));
+    }
+}
+
 // ------------------------------------------------------------------------------------------
 // epilogue of 8 consecutive columns: v = the sums (EPI_GATE_FWD: of the gate, w of the value projection).  What it reads is fetched
 // ahead: the biases of its columns once, the rest of a row (`Row`) while earlier rows are on their way out.
@@ -97,7 +123,7 @@ template <typename T> __device__ __forceinline__ void get(Chunk<T>& c, const T* 
         for (int i = 0; i < 8; ++i) c.q[i / W][i % W] = i < left ? p[i] : (T)0.f;
     }
 }
-template <typename T> struct Row { Chunk<T> x, y; };
+template <typename T> struct Row { Chunk<T> x, y, z; };
 template <typename T, int EPI> __device__ __forceinline__ void fetch_row(const Gemm<T>& g, size_t z, int sel, size_t m, int n, Row<T>& r) {
     const int left = m < g.M ? g.N - n : 0;
     if (EPI == EPI_STORE && (g.accumulate >> sel & 1)) get<T>(r.x, g.c[sel] + z * g.cz + m * g.N + n, left);
@@ -105,6 +131,7 @@ template <typename T, int EPI> __device__ __forceinline__ void fetch_row(const G
         const size_t o = (z * g.M + m) * g.ldf + n;
         get<T>(r.x, g.i0 + o, m < g.M ? g.ldf - n : 0);
         get<T>(r.y, g.i1 + o, m < g.M ? g.ldf - n : 0);
+        if (sizeof(T) == 2) get<T>(r.z, (const T*)g.low + o, m < g.M ? g.ldf - n : 0);
     }
 }
 struct Bias { float x[8], y[8]; };
@@ -134,8 +161,8 @@ __device__ __forceinline__ void emit(const Gemm<T>& g, size_t z, int sel, size_t
         float h[8], u, du;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            // h, and what the backward pass needs, are formed in fp32 from the sums and rounded once (16 bit: h, da and dv are operands of
-            // further 16-bit products; with u and p, and not a and v, in memory no rounding goes through the gate)
+            // formed in fp32 from the sums; 16 bit: h, da and dv are rounded as operands of further 16-bit products.  With u and p, and not a
+            // and v, in memory no rounding goes through the gate, and the backward pass evaluates none.
             w[i] += b.y[i];
             gate_fn<sizeof(T) == 4>(v[i] + b.x[i], g.gate, u, du);
             h[i] = i < left ? u * w[i] : 0.f;
@@ -144,14 +171,30 @@ __device__ __forceinline__ void emit(const Gemm<T>& g, size_t z, int sel, size_t
         }
         cg_store<T, 8>(g.o0 + (z * g.M + m) * g.ld0 + n, g.ld0 - n, h);
         if (g.o1) {
-            cg_store<T, 8>(g.o1 + of, g.ldf - n, v);
-            cg_store<T, 8>(g.o2 + of, g.ldf - n, w);
+            if constexpr (sizeof(T) == 2) {
+                typedef typename CgT<T>::V V;
+                u32x4 hu, hp, low;
+                keep(v, w, hu, hp, low);
+                *(V*)(g.o1 + of) = __builtin_bit_cast(V, hu);
+                *(V*)(g.o2 + of) = __builtin_bit_cast(V, hp);
+                *(V*)((T*)g.low + of) = __builtin_bit_cast(V, low);
+            } else {
+                cg_store<T, 8>(g.o1 + of, 8, v);
+                cg_store<T, 8>(g.o2 + of, 8, w);
+            }
         }
     } else {
+        float u[8], p[8];
+        if constexpr (sizeof(T) == 2) {
+            recall(u, p, __builtin_bit_cast(u32x4, row.x.q[0]), __builtin_bit_cast(u32x4, row.y.q[0]), __builtin_bit_cast(u32x4, row.z.q[0]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = row.x.q[i / W][i % W], p[i] = row.y.q[i / W][i % W];
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            w[i] = i < left ? v[i] * (float)row.x.q[i / W][i % W] : 0.f;
-            v[i] = i < left ? v[i] * (float)row.y.q[i / W][i % W] : 0.f;
+            w[i] = i < left ? v[i] * u[i] : 0.f;
+            v[i] = i < left ? v[i] * p[i] : 0.f;
             sx[i] += v[i];
             sy[i] += w[i];
         }
@@ -764,10 +807,26 @@ template <typename T, int EPI> __device__ __forceinline__ void emit1(const Gemm<
         w += g.bias[1] ? (float)g.bias[1][z * g.biasz + n] : 0.f;
         gate_fn<sizeof(T) == 4>(v + (g.bias[0] ? (float)g.bias[0][z * g.biasz + n] : 0.f), g.gate, u, du);
         g.o0[(z * g.M + m) * g.ld0 + n] = (T)(u * w);
-        if (g.o1) g.o1[o] = (T)u, g.o2[o] = (T)(w * du);
+        if (!g.o1) return;
+        if constexpr (sizeof(T) == 2) {
+            const unsigned x = bits(u), y = bits(w * du);
+            ((unsigned short*)g.o1)[o] = (unsigned short)(x >> 16);
+            ((unsigned short*)g.o2)[o] = (unsigned short)(y >> 16);
+            g.low[o] = (unsigned short)((x >> 8 & 0xff) | (y & 0xff00));
+        } else {
+            g.o1[o] = u, g.o2[o] = w * du;
+        }
     } else {
-        g.o0[o] = (T)(v * (float)g.i1[o]);
-        g.o1[o] = (T)(v * (float)g.i0[o]);
+        float u, p;
+        if constexpr (sizeof(T) == 2) {
+            const unsigned low = g.low[o];
+            u = from((unsigned)((const unsigned short*)g.i0)[o] << 16 | (low & 0xff) << 8);
+            p = from((unsigned)((const unsigned short*)g.i1)[o] << 16 | (low & 0xff00));
+        } else {
+            u = g.i0[o], p = g.i1[o];
+        }
+        g.o0[o] = (T)(v * p);
+        g.o1[o] = (T)(v * u);
     }
 }
 template <typename T, bool KA, bool KB, int EPI, bool BLOCK> __global__ __launch_bounds__(256) void narrow_kernel(Gemm<T> g) {
@@ -1091,7 +1150,7 @@ template <typename T, bool KA, bool KB, int EPI> void gemm(Gemm<T>& g, int membe
 }
 
 // da, dv from a stored gradient of h (no output projection)
-template <typename T> struct GateBwd { const T *dh, *u, *p; T *da, *dv; size_t rows; int F, ldf; };
+template <typename T> struct GateBwd { const T *dh, *u, *p; const unsigned short* low; T *da, *dv; size_t rows; int F, ldf; };
 template <typename T> __global__ __launch_bounds__(256) void gate_bwd_kernel(GateBwd<T> g) {
     const size_t per = g.ldf / 8;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < g.rows * per; i += (size_t)gridDim.x * 256) {
@@ -1099,10 +1158,19 @@ template <typename T> __global__ __launch_bounds__(256) void gate_bwd_kernel(Gat
         const int n = (int)(i % per) * 8;
         float d[8], u[8], p[8];
         cg_load<T, 8>(g.dh + m * g.F + n, g.F - n, d);       // zeros behind F: da and dv end in zeros
-        cg_load<T, 8>(g.u + m * g.ldf + n, g.F - n, u);
-        cg_load<T, 8>(g.p + m * g.ldf + n, g.F - n, p);
+        if constexpr (sizeof(T) == 2) {
+            typedef typename CgT<T>::V V;
+            auto at = [&](const void* q) { return __builtin_bit_cast(u32x4, *(const V*)((const T*)q + m * g.ldf + n)); };
+            recall(u, p, at(g.u), at(g.p), at(g.low));
+        } else {
+            cg_load<T, 8>(g.u + m * g.ldf + n, 8, u);
+            cg_load<T, 8>(g.p + m * g.ldf + n, 8, p);
+        }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] *= d[e], u[e] *= d[e];
+        for (int e = 0; e < 8; ++e) {
+            p[e] = n + e < g.F ? p[e] * d[e] : 0.f;
+            u[e] = n + e < g.F ? u[e] * d[e] : 0.f;
+        }
         cg_store<T, 8>(g.da + m * g.ldf + n, 8, p);
         cg_store<T, 8>(g.dv + m * g.ldf + n, 8, u);
     }
@@ -1258,7 +1326,7 @@ inline int ldf_of(const cg_gated_dims* d) { return (int)pad8(d->F); }
 
 template <typename T>
 void fwd(const cg_gated_dims* d, const cg_group* grp, const T* x, const T* wg, const T* wv, const T* wo, const T* bg, const T* bv,
-         const T* bo, T* h, T* u, T* p, T* y, void* pack, float* part, hipStream_t st) {
+         const T* bo, T* h, T* kept, T* y, void* pack, float* part, hipStream_t st) {
     const int nz = grp_n(grp), ldf = ldf_of(d);
     const size_t M = d->rows / nz, gs = grp_stride(grp);
     const bool small = M <= FEW_ROWS;
@@ -1269,7 +1337,8 @@ void fwd(const cg_gated_dims* d, const cg_group* grp, const T* x, const T* wg, c
     g.B[0] = op.wg, g.B[1] = op.wv, g.bz = gs, g.ldb = op.ldw;
     g.M = M, g.K = d->D, g.N = d->F, g.gate = d->gate;
     g.bias[0] = bg, g.bias[1] = bv, g.biasz = gs;
-    g.o0 = h, g.o1 = u, g.o2 = p, g.ld0 = d->O ? ldf : d->F, g.ldf = ldf;
+    g.o0 = h, g.o1 = kept, g.o2 = kept ? kept + d->rows * ldf : nullptr, g.low = kept ? (unsigned short*)(kept + 2 * d->rows * ldf) : nullptr,
+     g.ld0 = d->O ? ldf : d->F, g.ldf = ldf;
     if (small) few<T, true, EPI_GATE_FWD>(g, nz, st);
     else gemm<T, true, true, EPI_GATE_FWD>(g, nz, part, st);
     if (!d->O) return;
@@ -1286,12 +1355,14 @@ void fwd(const cg_gated_dims* d, const cg_group* grp, const T* x, const T* wg, c
 
 template <typename T>
 void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, const T* wg, const T* wv, const T* wo, const T* h,
-         const T* u, const T* p, T* dx, T* dwg, T* dwv, T* dwo, T* dbg, T* dbv, T* dbo, int acc, void* pack, T* da, T* dv, T* dyp,
+         const T* kept, T* dx, T* dwg, T* dwv, T* dwo, T* dbg, T* dbv, T* dbo, int acc, void* pack, T* da, T* dv, T* dyp,
          float* part, hipStream_t st) {
     const int nz = grp_n(grp), ldf = ldf_of(d);
     const size_t M = d->rows / nz, gs = grp_stride(grp), D = d->D, F = d->F, O = d->O;
     const bool small = M <= FEW_ROWS;
     const Operands<T> op = operands<T>(d, grp, x, wg, wv, wo, pack, false, st);
+    const T *u = kept, *p = kept + d->rows * ldf;
+    unsigned short* low = (unsigned short*)(kept + 2 * d->rows * ldf);
     size_t ldy = O;
     if (O && packs(d, grp, dy, O)) {
         Pack<T> g = {};
@@ -1308,7 +1379,7 @@ void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, c
             g.A[0] = dy, g.az = M * ldy, g.lda = ldy;
             g.B[0] = op.wo, g.bz = gs, g.ldb = op.ldo;
             g.M = M, g.K = O, g.N = d->F;
-            g.o0 = da, g.o1 = dv, g.i0 = u, g.i1 = p, g.ldf = ldf;
+            g.o0 = da, g.o1 = dv, g.i0 = u, g.i1 = p, g.low = low, g.ldf = ldf;
             if ((dbg || dbv) && !small) g.sums = part;
             if (small) few<T, false, EPI_GATE_BWD>(g, nz, st);
             else gemm<T, true, false, EPI_GATE_BWD>(g, nz, part, st);
@@ -1319,7 +1390,7 @@ void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, c
             }
         } else if (M) {
             const size_t nb = ((size_t)d->rows * (ldf / 8) + 255) / 256;
-            gate_bwd_kernel<T><<<(unsigned)(nb < 16384 ? nb : 16384), 256, 0, st>>>(GateBwd<T>{dy, u, p, da, dv, (size_t)d->rows, d->F, ldf});
+            gate_bwd_kernel<T><<<(unsigned)(nb < 16384 ? nb : 16384), 256, 0, st>>>(GateBwd<T>{dy, u, p, low, da, dv, (size_t)d->rows, d->F, ldf});
         }
     }
     if (dx) {
@@ -1382,16 +1453,16 @@ extern "C" size_t cg_gated_ff_pack_bytes(const cg_gated_dims* d, const cg_group*
 extern "C" size_t cg_gated_ff_fwd_workspace(const cg_gated_dims* d, const cg_group* grp) { return dims_ok(d, grp) ? fwd_part(d, grp) : 0; }
 
 extern "C" int cg_gated_ff_fwd(const cg_gated_dims* d, const cg_group* grp, const void* x, const void* wg, const void* wv, const void* wo,
-                               const void* bg, const void* bv, const void* bo, void* h, void* u, void* p, void* y, void* pack, void* ws,
+                               const void* bg, const void* bv, const void* bo, void* h, void* kept, void* y, void* pack, void* ws,
                                size_t ws_bytes, cg_stream_t stream) {
-    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && !u == !p && (!d->O || wo) && (!d->rows || (x && h && (!d->O || y))),
+    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && (!d->O || wo) && (!d->rows || (x && h && (!d->O || y))),
                  "cg_gated_ff_fwd: bad args");
     const size_t need = fwd_part(d, grp);
     if (ws_bytes < need || (!ws && need) || (!pack && pack_bytes(d, grp, x, wg, wv, wo)))
         return cg_set_error(CG_ERR_WORKSPACE, "cg_gated_ff_fwd: workspace too small");
     if (!d->rows) return CG_OK;
     CG_DISPATCH_DT(d->dtype, T, (fwd<T>(d, grp, (const T*)x, (const T*)wg, (const T*)wv, (const T*)wo, (const T*)bg, (const T*)bv,
-                                        (const T*)bo, (T*)h, (T*)u, (T*)p, (T*)y, pack, (float*)ws, cg_s(stream))));
+                                        (const T*)bo, (T*)h, (T*)kept, (T*)y, pack, (float*)ws, cg_s(stream))));
     CG_LAUNCH_CHECK("cg_gated_ff_fwd");
     return CG_OK;
 }
@@ -1404,10 +1475,10 @@ extern "C" size_t cg_gated_ff_bwd_workspace(const cg_gated_dims* d, const cg_gro
 }
 
 extern "C" int cg_gated_ff_bwd(const cg_gated_dims* d, const cg_group* grp, const void* dy, const void* x, const void* wg,
-                               const void* wv, const void* wo, const void* h, const void* u, const void* p, void* dx, void* dwg,
+                               const void* wv, const void* wo, const void* h, const void* kept, void* dx, void* dwg,
                                void* dwv, void* dwo, void* dbg, void* dbv, void* dbo, int accumulate, const void* pack, void* ws,
                                size_t ws_bytes, cg_stream_t stream) {
-    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && (!d->O || wo) && (!d->rows || (dy && x && u && p && (!d->O || h))),
+    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && (!d->O || wo) && (!d->rows || (dy && x && kept && (!d->O || h))),
                  "cg_gated_ff_bwd: bad args");
     const size_t need = cg_gated_ff_bwd_workspace(d, grp);
     if (ws_bytes < need || (!ws && need) || (!pack && pack_bytes(d, grp, x, wg, wv, wo)))
@@ -1416,7 +1487,7 @@ extern "C" int cg_gated_ff_bwd(const cg_gated_dims* d, const cg_group* grp, cons
         char* w = (char*)ws;
         T *da = (T*)w, *dv = (T*)(w + bwd_hidden(d)), *dyp = (T*)(w + 2 * bwd_hidden(d));
         float* part = (float*)(w + 2 * bwd_hidden(d) + bwd_dy(d));
-        bwd<T>(d, grp, (const T*)dy, (const T*)x, (const T*)wg, (const T*)wv, (const T*)wo, (const T*)h, (const T*)u, (const T*)p, (T*)dx,
+        bwd<T>(d, grp, (const T*)dy, (const T*)x, (const T*)wg, (const T*)wv, (const T*)wo, (const T*)h, (const T*)kept, (T*)dx,
                (T*)dwg, (T*)dwv, (T*)dwo, (T*)dbg, (T*)dbv, (T*)dbo, accumulate, (void*)pack, da, dv, dyp, part, cg_s(stream));
     });
     CG_LAUNCH_CHECK("cg_gated_ff_bwd");

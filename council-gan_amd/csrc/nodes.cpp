@@ -290,7 +290,7 @@ constexpr int64_t MAX_WIDTH = 1 << 21;       // as the library has it
 // -- gated_feed_forward --------------------------------------------------------------------------------
 struct Gated : public torch::autograd::Node {
     SavedVariable x_, wg_, wv_, wo_;
-    Tensor h_, up_, pack_;      // up_: u and p; pack_: the forward pass's copies of operands that are not on 16 bytes
+    Tensor h_, kept_, pack_;      // kept_: u and p; pack_: the forward pass's copies of operands that are not on 16 bytes
     std::array<Tensor, 3> biases;
     cg_gated_dims dims{};
     Members members;
@@ -304,7 +304,7 @@ struct Gated : public torch::autograd::Node {
         wv_.reset_data();
         wo_.reset_data();
         h_.reset();
-        up_.reset();
+        kept_.reset();
         pack_.reset();
     }
     variable_list apply(variable_list&& grads) override {
@@ -332,9 +332,7 @@ struct Gated : public torch::autograd::Node {
         }
         const size_t nws = api.gated_bwd_ws(&dims, members.get());
         const Tensor ws = scratch(nws, x);
-        char* u = (char*)up_.data_ptr();
-        char* vd = u + up_.nbytes() / 2;
-        check(api.gated_bwd(&dims, members.get(), ptr(dy), ptr(x), ptr(p[0]), ptr(p[1]), ptr(p[2]), ptr(h_), u, vd, ptr(dx), to[0], to[1], to[2],
+        check(api.gated_bwd(&dims, members.get(), ptr(dy), ptr(x), ptr(p[0]), ptr(p[1]), ptr(p[2]), ptr(h_), ptr(kept_), ptr(dx), to[0], to[1], to[2],
                             to[3], to[4], to[5], add, ptr(pack_), ptr(ws), nws, stream_of(x)),
               "cg_gated_ff_bwd");
         settle(t);
@@ -374,7 +372,7 @@ py::object gated(const Tensor& x, const Tensor& wg, const Tensor& wv, const std:
         py::gil_scoped_release unlock;
         const c10::DeviceGuard device(x.device());
         Members members{{n, 0, stride}};
-        Tensor xd, h, up, pack;
+        Tensor xd, h, kept, pack;
         std::array<Tensor, 6> p{wg, wv, wo, b[0], b[1], b[2]};
         const int64_t rows = x.numel() / D;
         cg_gated_dims dims{rows, (int32_t)D, (int32_t)F, (int32_t)O, dt, gate, 0};
@@ -394,13 +392,12 @@ py::object gated(const Tensor& x, const Tensor& wg, const Tensor& wv, const std:
             const int64_t pitch = (F + 7) & ~(int64_t)7;
             h = O ? at::empty({rows, pitch}, x.options()) : rows_like(F);
             if (O) y = rows_like(O);
-            if (record) up = at::empty({2, rows, pitch}, x.options());
-            char* u = record ? (char*)up.data_ptr() : nullptr;
+            if (record) kept = at::empty({dt == CG_DT_F32 ? 2 : 3, rows, pitch}, x.options());
             pack = scratch(api.gated_pack(&dims, members.get(), ptr(xd), ptr(p[0]), ptr(p[1]), ptr(p[2])), x);
             const size_t nws = api.gated_fwd_ws(&dims, members.get());
             const Tensor ws = scratch(nws, x);
-            check(api.gated_fwd(&dims, members.get(), ptr(xd), ptr(p[0]), ptr(p[1]), ptr(p[2]), ptr(p[3]), ptr(p[4]), ptr(p[5]), ptr(h), u,
-                                record ? u + up.nbytes() / 2 : nullptr, ptr(y), ptr(pack), ptr(ws), nws, stream_of(x)),
+            check(api.gated_fwd(&dims, members.get(), ptr(xd), ptr(p[0]), ptr(p[1]), ptr(p[2]), ptr(p[3]), ptr(p[4]), ptr(p[5]), ptr(h), ptr(kept),
+                                ptr(y), ptr(pack), ptr(ws), nws, stream_of(x)),
                   "cg_gated_ff_fwd");
         }
         if (record) {
@@ -414,7 +411,7 @@ py::object gated(const Tensor& x, const Tensor& wg, const Tensor& wv, const std:
             }
             for (int i = 0; i < 3; ++i)
                 if (p[3 + i].defined()) node->biases[i] = p[3 + i].detach();
-            node->up_ = up;
+            node->kept_ = kept;
             node->pack_ = pack;
             node->dims = dims;
             node->members = members;

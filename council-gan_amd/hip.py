@@ -164,9 +164,9 @@ _SIGS = {
     "cg_dropout": (c_int, [_P, _P, _P, c_size_t, c_int, _P, c_int, _P]),
     "cg_gated_ff_fwd_workspace": (c_size_t, [POINTER(GatedDims), POINTER(Group)]),
     "cg_gated_ff_pack_bytes": (c_size_t, [POINTER(GatedDims), POINTER(Group), _P, _P, _P, _P]),
-    "cg_gated_ff_fwd": (c_int, [POINTER(GatedDims), POINTER(Group)] + [_P] * 13 + [c_size_t, _P]),
+    "cg_gated_ff_fwd": (c_int, [POINTER(GatedDims), POINTER(Group)] + [_P] * 12 + [c_size_t, _P]),
     "cg_gated_ff_bwd_workspace": (c_size_t, [POINTER(GatedDims), POINTER(Group)]),
-    "cg_gated_ff_bwd": (c_int, [POINTER(GatedDims), POINTER(Group)] + [_P] * 15 + [c_int, _P, _P, c_size_t, _P]),
+    "cg_gated_ff_bwd": (c_int, [POINTER(GatedDims), POINTER(Group)] + [_P] * 14 + [c_int, _P, _P, c_size_t, _P]),
     "cg_avgpool3s2_fwd": (c_int, [_P, _P, c_int, c_int, c_int, c_int, _P]),
     "cg_avgpool3s2_bwd": (c_int, [_P, _P, c_int, c_int, c_int, c_int, _P]),
     "cg_upsample2x_fwd": (c_int, [_P, _P, c_int, c_int, c_int, c_int, _P]),

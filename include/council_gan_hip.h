@@ -465,19 +465,20 @@ typedef struct cg_gated_dims {
     int32_t dtype, gate, reserved;
 } cg_gated_dims;
 /* a = x wg^T + bg, v = x wv^T + bv, h = gate(a) * v, y = h wo^T + bo; wg / wv [F][D], wo [O][F]; biases may be NULL.
- * u = gate(a), p = v gate'(a) (both or neither): kept for the backward pass.  Rows of u and p, and of h unless it is the result
- * (O = 0), are F rounded up to a multiple of 8 elements long.  pack: cg_gated_ff_pack_bytes of memory for copies of 16-bit operands whose rows do not start on 16
+ * kept, or NULL: u = gate(a) and p = v gate'(a) for the backward pass, planes of rows x F' elements (fp32: u, p; 16-bit types: the upper
+ * halves of u, of p as fp32 numbers, and their third bytes, p's above u's); F' is F rounded up to a multiple of 8, the length of the
+ * rows of h too unless it is the result (O = 0).  pack: cg_gated_ff_pack_bytes of memory for copies of 16-bit operands whose rows do not start on 16
  * bytes (0: may be NULL); the forward pass fills it, the backward pass reads it. */
 size_t cg_gated_ff_pack_bytes(const cg_gated_dims* d, const cg_group* grp, const void* x, const void* wg, const void* wv, const void* wo);
 size_t cg_gated_ff_fwd_workspace(const cg_gated_dims* d, const cg_group* grp);
 int cg_gated_ff_fwd(const cg_gated_dims* d, const cg_group* grp, const void* x, const void* wg, const void* wv, const void* wo,
-                    const void* bg, const void* bv, const void* bo, void* h, void* u, void* p, void* y, void* pack, void* ws,
+                    const void* bg, const void* bv, const void* bo, void* h, void* kept, void* y, void* pack, void* ws,
                     size_t ws_bytes, cg_stream_t stream);
 /* dy: gradient of y (of h when O is 0).  Any gradient may be NULL.  Bit i of `accumulate` adds to parameter gradient i of
  * {dwg, dwv, dwo, dbg, dbv, dbo} instead of overwriting it. */
 size_t cg_gated_ff_bwd_workspace(const cg_gated_dims* d, const cg_group* grp);
 int cg_gated_ff_bwd(const cg_gated_dims* d, const cg_group* grp, const void* dy, const void* x, const void* wg, const void* wv,
-                    const void* wo, const void* h, const void* u, const void* p, void* dx, void* dwg, void* dwv, void* dwo, void* dbg,
+                    const void* wo, const void* h, const void* kept, void* dx, void* dwg, void* dwv, void* dwo, void* dbg,
                     void* dbv, void* dbo, int accumulate, const void* pack, void* ws, size_t ws_bytes, cg_stream_t stream);
 
 /* ---- resampling --------------------------------------------------------------------------- */

@@ -81,7 +81,8 @@ def gate(a, act):
 def gated_ref(x, wg, wv, wo, bg, bv, bo, act, dy):
     """{name: (value, bound without the output's own rounding)}: rows x [M, D], all inputs as the kernel reads them.
 
-    The kernel holds h, u = act(a), p = v act'(a), da and dv in x's type (one rounding ut each) and adds in fp32; a product of K terms is off by at most
+    The kernel holds h, da and dv in x's type (one rounding ut each), u = act(a) and p = v act'(a) in the upper 24 bits of their fp32
+    values (16-bit types; cut off: below 2^-15 of the value) and adds in fp32; a product of K terms is off by at most
     (K + 8) U sum|terms|, 4 more roundings an fp32 product that is put together from parts (its parts below 2^-23 are left out, less than 4 U)."""
     t = x.dtype
     ut, eta = u(t), torch.finfo(t).smallest_normal * u(t)       # one rounding: relative, and half a step of the smallest numbers
@@ -127,8 +128,9 @@ def gated_ref(x, wg, wv, wo, bg, bv, bo, act, dy):
         dh, edh = dy, torch.zeros_like(dy)
     da, dv = dh * v * dg, dh * g
     # u and p as they are kept, then da = dh p and dv = dh u
-    ekp = ev * ab(dg) + ab(v) * edg + ev * edg + (ut + 2 * U) * ab(v * dg) + eta
-    eku = eg + ut * ab(g) + eta
+    kt = 0 if t == torch.float32 else 2.0 ** -15
+    ekp = ev * ab(dg) + ab(v) * edg + ev * edg + (kt + 2 * U) * ab(v * dg)
+    eku = eg + kt * ab(g)
     eda = edh * ab(v * dg) + ab(dh) * ekp + edh * ekp + (ut + 2 * U) * ab(da) + eta
     edv = edh * ab(g) + ab(dh) * eku + edh * eku + (ut + 2 * U) * ab(dv) + eta
     p, ep = lin(da, wg.t().contiguous(), dp=eda)

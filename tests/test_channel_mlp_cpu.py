@@ -76,15 +76,15 @@ def test_library_refuses_bad_arguments_before_any_launch():
     assert lib.cg_dropout(p, None, p, 4, 1, p, 3, None) == -1
     assert lib.cg_dropout_key(p, p, None) == -1
     d = hip.GatedDims(4, 8, 16, 8, 1, 0, 0)
-    args = [p] * 13
+    args = [p] * 12
     assert lib.cg_gated_ff_fwd(ctypes.byref(hip.GatedDims(4, 8, 16, 8, 1, 3, 0)), None, *args, 0, None) == -1
     assert lib.cg_gated_ff_fwd(ctypes.byref(d), ctypes.byref(hip.Group(2, 0, 32)), *args, 0, None) == -1   # members hold fp32
-    assert lib.cg_gated_ff_fwd(ctypes.byref(d), None, p, p, p, None, None, None, None, p, p, p, p, None, None, 0, None) == -1
-    assert lib.cg_gated_ff_bwd(ctypes.byref(d), None, *([p] * 15), 0, p, p, 0, None) == -3
+    assert lib.cg_gated_ff_fwd(ctypes.byref(d), None, p, p, p, None, None, None, None, p, p, p, None, None, 0, None) == -1
+    assert lib.cg_gated_ff_bwd(ctypes.byref(d), None, *([p] * 14), 0, p, p, 0, None) == -3
     assert b"workspace" in lib.cg_last_error()
     odd = hip.GatedDims(64, 9, 16, 8, 1, 0, 0)      # rows of 9 halves do not start on 16 bytes: the copies need memory
     assert lib.cg_gated_ff_pack_bytes(ctypes.byref(odd), None, p, p, p, p) >= (64 + 2 * 16) * 16 * 2
-    assert lib.cg_gated_ff_fwd(ctypes.byref(odd), None, p, p, p, p, None, None, None, p, p, p, p, None, p, 1 << 30, None) == -3
+    assert lib.cg_gated_ff_fwd(ctypes.byref(odd), None, p, p, p, p, None, None, None, p, p, p, None, p, 1 << 30, None) == -3
     assert lib.cg_gated_ff_pack_bytes(ctypes.byref(hip.GatedDims(64, 8, 16, 8, 1, 0, 0)), None, p, p, p, p) == 0
     assert lib.cg_gated_ff_pack_bytes(ctypes.byref(hip.GatedDims(64, 8, 16, 8, 1, 0, 0)), None, ctypes.c_void_p(258), p, p, p) > 0
 
