@@ -387,10 +387,13 @@ __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)
     const bool whole = g.splits == 1;
     Bias bias;
     float sx[8] = {}, sy[8] = {};
-    Row<T> row[2][PASSES];
+    // the fp32 rows of the gate's backward pass take 64 registers: one set of them, or the tiles lose their third block on a CU (1386 us
+    // instead of 1368 for the backward pass of 65536 x 256 x 1024)
+    constexpr int SETS = EPI == EPI_GATE_BWD && sizeof(T) == 4 ? 1 : 2;
+    Row<T> row[SETS][PASSES];
     auto fetch = [&](int i) {
 #pragma unroll
-        for (int pass = 0; pass < PASSES; ++pass) fetch_row<T, EPI>(g, z, sel, ml + i * 32 + pass * RPP, n, row[i & 1][pass]);
+        for (int pass = 0; pass < PASSES; ++pass) fetch_row<T, EPI>(g, z, sel, ml + i * 32 + pass * RPP, n, row[i % SETS][pass]);
     };
     if (whole) {
         fetch_bias<T, EPI>(g, z, n, bias);
@@ -404,7 +407,7 @@ __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)
             for (int r = 0; r < 16; ++r) ep[(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)) * EP + j * 32 + (lane & 31)] = acc[i][j][r];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
         __builtin_amdgcn_wave_barrier();
-        if (whole && i + 1 < TM) fetch(i + 1);
+        if (SETS == 2 && whole && i + 1 < TM) fetch(i + 1);
 #pragma unroll
         for (int pass = 0; pass < PASSES; ++pass) {
             const int at = (pass * RPP + lane / LPR) * EP + lane % LPR * 8;
@@ -417,7 +420,7 @@ __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)
             }
             if (m < g.M && n < g.N) {
                 if (whole) {
-                    emit<T, EPI>(g, z, sel, m, n, v, w, bias, row[i & 1][pass], sx, sy);
+                    emit<T, EPI>(g, z, sel, m, n, v, w, bias, row[i % SETS][pass], sx, sy);
                 } else {
                     const size_t np = pad8(g.N);
                     float* p = g.part + (((size_t)split * (gridDim.z / g.splits) + zs) * g.M + m) * planes<EPI>() * np + n;
@@ -426,6 +429,7 @@ __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)
                 }
             }
         }
+        if (SETS == 1 && whole && i + 1 < TM) fetch(i + 1);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
         __builtin_amdgcn_wave_barrier();
     }
@@ -449,10 +453,10 @@ __device__ __forceinline__ void store_tile(const Gemm<T>& g, const f32x16 (&acc)
 // The matrix pipe cuts its sums off downwards a few bits below fp32, so every result is low by some 1e-7 of its size, and a sum of 65536
 // of them (a bias gradient) by 1.4e-6, where its random errors come to 4e-7.  So half of A's rows go through with the other sign: the
 // errors of neighbouring row blocks cancel in any sum over rows (no time is lost by it).
-// One LDS buffer, loads one K-step ahead in registers, and three blocks on a CU where the registers allow it (not with the operands of the
-// gate's backward epilogue): 510 us instead of 577 for the gate product of 65536 x 256 x 1024 with two blocks and two steps ahead.
+// One LDS buffer, loads one K-step ahead in registers, and three blocks on a CU: 510 us instead of 577 for the gate product of
+// 65536 x 256 x 1024 with two blocks and two steps ahead.
 template <int BM, int BN, int WM, int WN, bool KA, bool KB, int EPI>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 && EPI != EPI_GATE_BWD ? 3 : 2) void gemm_kernel(Gemm<float> g) {
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, BM == 128 ? 3 : 2) void gemm_kernel(Gemm<float> g) {
     typedef float T;
     constexpr int NW = (BM / WM) * (BN / WN), NT = NW * 64, TM = WM / 32, TN = WN / 32;
     typedef Operand<BM, NT, KA, false> OA;
@@ -1238,6 +1242,10 @@ bool dims_ok(const cg_gated_dims* d, const cg_group* grp) {
            (grp_n(grp) == 1 || d->dtype == CG_DT_F32);
 }
 
+// what the kernels read 16 bytes at a time without a copy: the caller's buffers between the passes
+inline bool aligned16(const void* a, const void* b, const void* c, const void* d) {
+    return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) & 15) == 0;
+}
 inline size_t esize(int dt) { return dt == CG_DT_F32 ? 4 : 2; }
 inline size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -1455,7 +1463,8 @@ extern "C" size_t cg_gated_ff_fwd_workspace(const cg_gated_dims* d, const cg_gro
 extern "C" int cg_gated_ff_fwd(const cg_gated_dims* d, const cg_group* grp, const void* x, const void* wg, const void* wv, const void* wo,
                                const void* bg, const void* bv, const void* bo, void* h, void* kept, void* y, void* pack, void* ws,
                                size_t ws_bytes, cg_stream_t stream) {
-    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && (!d->O || wo) && (!d->rows || (x && h && (!d->O || y))),
+    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && (!d->O || wo) && (!d->rows || (x && h && (!d->O || y))) &&
+                     aligned16(d->O ? h : nullptr, kept, pack, ws),
                  "cg_gated_ff_fwd: bad args");
     const size_t need = fwd_part(d, grp);
     if (ws_bytes < need || (!ws && need) || (!pack && pack_bytes(d, grp, x, wg, wv, wo)))
@@ -1478,7 +1487,8 @@ extern "C" int cg_gated_ff_bwd(const cg_gated_dims* d, const cg_group* grp, cons
                                const void* wv, const void* wo, const void* h, const void* kept, void* dx, void* dwg,
                                void* dwv, void* dwo, void* dbg, void* dbv, void* dbo, int accumulate, const void* pack, void* ws,
                                size_t ws_bytes, cg_stream_t stream) {
-    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && (!d->O || wo) && (!d->rows || (dy && x && kept && (!d->O || h))),
+    CG_CHECK_ARG(dims_ok(d, grp) && wg && wv && (!d->O || wo) && (!d->rows || (dy && x && kept && (!d->O || h))) &&
+                     aligned16(d->O ? h : nullptr, kept, pack, ws),
                  "cg_gated_ff_bwd: bad args");
     const size_t need = cg_gated_ff_bwd_workspace(d, grp);
     if (ws_bytes < need || (!ws && need) || (!pack && pack_bytes(d, grp, x, wg, wv, wo)))

@@ -467,8 +467,8 @@ typedef struct cg_gated_dims {
 /* a = x wg^T + bg, v = x wv^T + bv, h = gate(a) * v, y = h wo^T + bo; wg / wv [F][D], wo [O][F]; biases may be NULL.
  * kept, or NULL: u = gate(a) and p = v gate'(a) for the backward pass, planes of rows x F' elements (fp32: u, p; 16-bit types: the upper
  * halves of u, of p as fp32 numbers, and their third bytes, p's above u's); F' is F rounded up to a multiple of 8, the length of the
- * rows of h too unless it is the result (O = 0).  pack: cg_gated_ff_pack_bytes of memory for copies of 16-bit operands whose rows do not start on 16
- * bytes (0: may be NULL); the forward pass fills it, the backward pass reads it. */
+ * rows of h too unless it is the result (O = 0).  pack: cg_gated_ff_pack_bytes of memory for copies of 16-bit operands whose rows do not
+ * start on 16 bytes (0: may be NULL); the forward pass fills it, the backward pass reads it.  h (O > 0), kept, pack and ws are on 16 bytes. */
 size_t cg_gated_ff_pack_bytes(const cg_gated_dims* d, const cg_group* grp, const void* x, const void* wg, const void* wv, const void* wo);
 size_t cg_gated_ff_fwd_workspace(const cg_gated_dims* d, const cg_group* grp);
 int cg_gated_ff_fwd(const cg_gated_dims* d, const cg_group* grp, const void* x, const void* wg, const void* wv, const void* wo,

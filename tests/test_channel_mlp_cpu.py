@@ -82,6 +82,12 @@ def test_library_refuses_bad_arguments_before_any_launch():
     assert lib.cg_gated_ff_fwd(ctypes.byref(d), None, p, p, p, None, None, None, None, p, p, p, None, None, 0, None) == -1
     assert lib.cg_gated_ff_bwd(ctypes.byref(d), None, *([p] * 14), 0, p, p, 0, None) == -3
     assert b"workspace" in lib.cg_last_error()
+    off = ctypes.c_void_p(264)                      # h, kept, pack and the workspace are on 16 bytes
+    for i in (7, 8, 10, 11):
+        assert lib.cg_gated_ff_fwd(ctypes.byref(d), None, *(off if k == i else p for k in range(12)), 1 << 30, None) == -1
+    for i in (5, 6, 14, 15):
+        a = [off if k == i else p for k in range(16)]
+        assert lib.cg_gated_ff_bwd(ctypes.byref(d), None, *a[:14], 0, *a[14:], 1 << 30, None) == -1
     odd = hip.GatedDims(64, 9, 16, 8, 1, 0, 0)      # rows of 9 halves do not start on 16 bytes: the copies need memory
     assert lib.cg_gated_ff_pack_bytes(ctypes.byref(odd), None, p, p, p, p) >= (64 + 2 * 16) * 16 * 2
     assert lib.cg_gated_ff_fwd(ctypes.byref(odd), None, p, p, p, p, None, None, None, p, p, p, None, p, 1 << 30, None) == -3
