@@ -1088,10 +1088,10 @@ template <typename T> __global__ __launch_bounds__(256) void few_grads_kernel(Fe
 }
 
 // Tile and number of K splits: 256 x 256 or 128 x 128 (16 bit), 128 x 128 or 64 x 64 (fp32; 4 waves of 64 x 64, 2 of 32 x 64).  The pair with
-// the least time by this account is taken: tiles run in rounds of as many as fit the chip; a tile takes its K-steps, longer where tiles
-// share a CU, and its epilogue; joining splits costs a launch, the lost fusions of the epilogue, and the partial sums' way out and back at
-// about 5 TB/s.  A split takes at least 4 K-steps.  The figures below are measured (us).  The number of members is left out: a member's
-// results do not depend on how many run beside it.
+// the least time by this account is taken: tiles run in rounds of as many as fit the chip, the last one with what is left; a tile takes
+// its K-steps, longer where tiles share a CU, and its epilogue; joining splits costs a launch, the lost fusions of the epilogue, and the
+// partial sums' way out and back at about 5 TB/s.  A split takes at least 4 K-steps.  The figures below are measured (us).  The number of
+// members is left out: a member's results do not depend on how many run beside it.
 struct Plan { int tile, splits; };
 Plan plan(size_t M, size_t N, size_t K, int nsel, int esz) {
     const size_t bk = esz == 4 ? 32 : 64, steps = (K + bk - 1) / bk, most = steps / 4 > 1 ? steps / 4 : 1;
@@ -1101,15 +1101,15 @@ Plan plan(size_t M, size_t N, size_t K, int nsel, int esz) {
     for (int c = 0; c < 2; ++c) {
         const int tile = esz == 2 ? 256 >> c : 128 >> c;
         const size_t t = (size_t)cg_div_up(M, tile) * cg_div_up(N, tile) * nsel;
+        const size_t slots = esz == 2 ? (tile == 256 ? 256 : 512) : tile == 128 ? 768 : 1024;      // what the chip holds
+        const double epilogue = esz == 2 ? (tile == 256 ? 8 : 4) : tile == 128 ? 5 : 2;
+        auto step = [&](size_t n) {       // a K-step where n tiles are at work
+            if (esz == 2) return tile == 256 ? 1.0 : n > 256 ? 0.9 : 0.7;
+            return tile == 128 ? (n > 512 ? 2.2 : n > 256 ? 1.6 : 1.4) : 1.4;
+        };
         for (size_t s = 1; s <= most && s <= 64; ++s) {
-            const size_t n = t * s;
-            double step, epilogue;
-            size_t slots;
-            if (tile == 256) step = 1.0, epilogue = 8, slots = 256;
-            else if (esz == 2) step = n > 256 ? 0.9 : 0.7, epilogue = 4, slots = 512;
-            else if (tile == 128) step = n > 512 ? 2.2 : n > 256 ? 1.6 : 1.4, epilogue = 5, slots = 768;
-            else step = 1.4, epilogue = 2, slots = 1024;
-            const double us = (double)((t * s + slots - 1) / slots) * ((double)((steps + s - 1) / s) * step + epilogue) +
+            const size_t n = t * s, k = (steps + s - 1) / s;
+            const double us = n / slots * (k * step(slots) + epilogue) + (n % slots ? k * step(n % slots) + epilogue : 0) +
                               (s > 1 ? 8.0 + 2.0 * 4 * s * M * N * nsel / 5e6 : 0);
             if (us < best) best = us, p = {tile, (int)s};
         }
