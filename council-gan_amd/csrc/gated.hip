@@ -30,7 +30,7 @@ template <typename T> struct Gemm {
     const T* bias[2];
     size_t biasz;
     int gate;
-    T *o0, *o1, *o2;          // EPI_GATE_FWD: h and, for the backward pass, u = act(a) and p = v act'(a); EPI_GATE_BWD: da, dv
+    T *o0, *o1, *o2;          // EPI_GATE_FWD: h and, for the backward pass, u = act(a) and p = v act'(a); EPI_GATE_BWD: da, dv (few rows: float)
     const T *i0, *i1;         // EPI_GATE_BWD: u, p
     unsigned short* low;      // 16 bit: the third bytes of u and p (keep)
     int ld0, ldf;             // pitch of h; of u, p, da, dv.  A pitch beyond N is a multiple of 8 and its columns get zeros
@@ -829,8 +829,8 @@ template <typename T, int EPI> __device__ __forceinline__ void emit1(const Gemm<
         } else {
             u = g.i0[o], p = g.i1[o];
         }
-        g.o0[o] = (T)(v * p);
-        g.o1[o] = (T)(v * u);
+        ((float*)g.o0)[o] = v * p;      // few rows multiply in fp32: da and dv are not rounded (narrow_kernel's T is float)
+        ((float*)g.o1)[o] = v * u;
     }
 }
 template <typename T, bool KA, bool KB, int EPI, bool BLOCK> __global__ __launch_bounds__(256) void narrow_kernel(Gemm<T> g) {
@@ -871,7 +871,7 @@ template <typename T, bool KA, bool KB, int EPI, bool BLOCK> __global__ __launch
 // joined through LDS in wave order.  v_mfma_f32_16x16x4_f32 takes 16 columns x 4 K-steps of the weights against 16 rows x 4 K-steps of
 // the rows, one value a lane (lane l: column or row l % 16, K-step l / 16): with weights that are K-contiguous a lane loads 16 bytes of
 // its row and the K-steps of a product are whichever the lanes hold; row-contiguous weights need no transposition at all.  Every type is
-// multiplied in fp32 (16-bit K-contiguous operands on v_mfma_f32_16x16x32, which takes the 16 bytes as they are).
+// multiplied in fp32 (16-bit K-contiguous operands on v_mfma_f32_16x16x32, which takes the 16 bytes as they are), and da and dv stay fp32.
 // ------------------------------------------------------------------------------------------
 constexpr int FEW_ROWS = 32, FEW_WAVES = 16;
 
@@ -887,17 +887,19 @@ template <typename T, int MT, bool KB, int EPI> __global__ __launch_bounds__(FEW
     constexpr int W = CgT<T>::N, NT = EPI == EPI_GATE_FWD || !KB ? 2 : 1;       // 16-column tiles: gate and value, or even and odd columns
     constexpr int REGS = MT * NT * 4;
     typedef typename CgT<T>::V V;
+    typedef std::conditional_t<EPI == EPI_STORE && !KB, float, T> TX;       // the rows: da and dv are fp32
+    typedef TX VX __attribute__((ext_vector_type(W), aligned(sizeof(TX))));
     __shared__ float sm[FEW_WAVES * REGS * 64];
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, l16 = lane & 15, lk = lane >> 4;
     const size_t z = blockIdx.y;
     const int n0 = blockIdx.x * (KB ? 16 : 32), K = (int)g.K;
     f32x4 acc[MT][NT] = {};
     for (int s = 0; s < g.nseg; ++s) {
-        const T* x[MT];
+        const TX* x[MT];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             const size_t m = i * 16 + l16;
-            x[i] = g.A[s] + z * g.az + (m < g.M ? m : g.M - 1) * g.lda;
+            x[i] = (const TX*)g.A[s] + z * g.az + (m < g.M ? m : g.M - 1) * g.lda;
         }
         if constexpr (KB) {
             const size_t n = n0 + l16 < g.N ? n0 + l16 : g.N - 1;
@@ -961,7 +963,7 @@ template <typename T, int MT, bool KB, int EPI> __global__ __launch_bounds__(FEW
             constexpr int U = (MT == 1 ? 64 : 32) / (4 * W);
             for (int k0 = wid * 4 * W * U; k0 < K; k0 += FEW_WAVES * 4 * W * U) {
                 V2 ba[U][W];
-                V xa[U][MT];
+                VX xa[U][MT];
 #pragma unroll
                 for (int q = 0; q < U; ++q) {
                     const int k = k0 + (q * 4 + lk) * W;
@@ -974,10 +976,10 @@ template <typename T, int MT, bool KB, int EPI> __global__ __launch_bounds__(FEW
 #pragma unroll
                     for (int i = 0; i < MT; ++i) {
                         if (k + W <= K) {
-                            xa[q][i] = *(const V*)(x[i] + k);
+                            xa[q][i] = *(const VX*)(x[i] + k);
                         } else {
 #pragma unroll
-                            for (int e = 0; e < W; ++e) xa[q][i][e] = k + e < K ? x[i][k + e] : (T)0.f;
+                            for (int e = 0; e < W; ++e) xa[q][i][e] = k + e < K ? x[i][k + e] : (TX)0.f;
                         }
                     }
                 }
@@ -1028,7 +1030,7 @@ template <typename T, bool KB, int EPI> void few(const Gemm<T>& g, int members, 
 
 // All parameter gradients of few rows in one launch: dW = P^T Q in tiles of 64 x 64 (4 waves of 16 x 64), db = column sums of P.
 template <typename T> struct FewGrads {
-    struct { const T *p, *q; T *dw, *db; int P, Q, ldp, ldq, tiles_q, first, add_w, add_b; } o[3];
+    struct { const void* p; const T* q; T *dw, *db; int P, Q, ldp, ldq, tiles_q, first, add_w, add_b, p32; } o[3];      // p32: p is fp32
     int n, M;
     size_t gs;
 };
@@ -1039,7 +1041,8 @@ template <typename T> __global__ __launch_bounds__(256) void few_grads_kernel(Fe
     const int tile = blockIdx.x - o.first, lane = threadIdx.x & 63, l16 = lane & 15, lk = lane >> 4;
     const size_t z = blockIdx.y;
     const int p0 = tile / o.tiles_q * 64 + (threadIdx.x >> 6) * 16, q0 = tile % o.tiles_q * 64;
-    const T *p = o.p + z * g.M * o.ldp, *q = o.q + z * g.M * o.ldq;
+    const size_t zp = z * g.M * o.ldp;
+    const T* q = o.q + z * g.M * o.ldq;
     const int pc = p0 + l16 < o.P ? p0 + l16 : o.P - 1;
     int qc[4];
 #pragma unroll
@@ -1052,7 +1055,8 @@ template <typename T> __global__ __launch_bounds__(256) void few_grads_kernel(Fe
         for (int h = 0; h < 2; ++h) {
             const int m = m0 + h * 4 + lk;
             const bool in = m < g.M;
-            a[h] = in ? (float)p[(size_t)m * o.ldp + pc] : 0.f;
+            const size_t at = zp + (size_t)m * o.ldp + pc;
+            a[h] = !in ? 0.f : o.p32 ? ((const float*)o.p)[at] : (float)((const T*)o.p)[at];
             sum += a[h];
 #pragma unroll
             for (int j = 0; j < 4; ++j) b[h][j] = in ? (float)q[(size_t)m * o.ldq + qc[j]] : 0.f;
@@ -1154,8 +1158,8 @@ template <typename T, bool KA, bool KB, int EPI> void gemm(Gemm<T>& g, int membe
 }
 
 // da, dv from a stored gradient of h (no output projection)
-template <typename T> struct GateBwd { const T *dh, *u, *p; const unsigned short* low; T *da, *dv; size_t rows; int F, ldf; };
-template <typename T> __global__ __launch_bounds__(256) void gate_bwd_kernel(GateBwd<T> g) {
+template <typename T> struct GateBwd { const T *dh, *u, *p; const unsigned short* low; void *da, *dv; size_t rows; int F, ldf; };
+template <typename T, typename TO> __global__ __launch_bounds__(256) void gate_bwd_kernel(GateBwd<T> g) {
     const size_t per = g.ldf / 8;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < g.rows * per; i += (size_t)gridDim.x * 256) {
         const size_t m = i / per;
@@ -1175,8 +1179,8 @@ template <typename T> __global__ __launch_bounds__(256) void gate_bwd_kernel(Gat
             p[e] = n + e < g.F ? p[e] * d[e] : 0.f;
             u[e] = n + e < g.F ? u[e] * d[e] : 0.f;
         }
-        cg_store<T, 8>(g.da + m * g.ldf + n, 8, p);
-        cg_store<T, 8>(g.dv + m * g.ldf + n, 8, u);
+        cg_store<TO, 8>((TO*)g.da + m * g.ldf + n, 8, p);
+        cg_store<TO, 8>((TO*)g.dv + m * g.ldf + n, 8, u);
     }
 }
 
@@ -1398,7 +1402,10 @@ void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, c
             }
         } else if (M) {
             const size_t nb = ((size_t)d->rows * (ldf / 8) + 255) / 256;
-            gate_bwd_kernel<T><<<(unsigned)(nb < 16384 ? nb : 16384), 256, 0, st>>>(GateBwd<T>{dy, u, p, low, da, dv, (size_t)d->rows, d->F, ldf});
+            const unsigned blocks = (unsigned)(nb < 16384 ? nb : 16384);
+            const GateBwd<T> g = {dy, u, p, low, da, dv, (size_t)d->rows, d->F, ldf};
+            if (small) gate_bwd_kernel<T, float><<<blocks, 256, 0, st>>>(g);
+            else gate_bwd_kernel<T, T><<<blocks, 256, 0, st>>>(g);
         }
     }
     if (dx) {
@@ -1415,17 +1422,17 @@ void bwd(const cg_gated_dims* d, const cg_group* grp, const T* dy, const T* x, c
         FewGrads<T> g = {};
         g.M = (int)M, g.gs = gs;
         int first = 0;
-        auto add = [&](const T* p, size_t P, size_t ldp, const T* q, size_t Q, size_t ldq, T* dw, T* db, int bit) {
+        auto add = [&](const T* p, int p32, size_t P, size_t ldp, const T* q, size_t Q, size_t ldq, T* dw, T* db, int bit) {
             if (!dw && !db) return;
             auto& o = g.o[g.n++];
-            o.p = p, o.q = q, o.dw = dw, o.db = db, o.P = (int)P, o.Q = (int)Q, o.ldp = (int)ldp, o.ldq = (int)ldq;
+            o.p = p, o.p32 = p32, o.q = q, o.dw = dw, o.db = db, o.P = (int)P, o.Q = (int)Q, o.ldp = (int)ldp, o.ldq = (int)ldq;
             o.tiles_q = dw ? (int)cg_div_up(Q, 64) : 1, o.first = first;
             o.add_w = acc >> bit & 1, o.add_b = acc >> (bit + 3) & 1;
             first += (int)cg_div_up(P, 64) * o.tiles_q;
         };
-        add(da, F, ldf, x, D, D, dwg, dbg, 0);
-        add(dv, F, ldf, x, D, D, dwv, dbv, 1);
-        if (O) add(dy, O, O, h, F, ldf, dwo, dbo, 2);
+        add(da, 1, F, ldf, x, D, D, dwg, dbg, 0);
+        add(dv, 1, F, ldf, x, D, D, dwv, dbv, 1);
+        if (O) add(dy, sizeof(T) == 4, O, O, h, F, ldf, dwo, dbo, 2);
         if (g.n) few_grads_kernel<T><<<dim3(first, nz), 256, 0, st>>>(g);
         return;
     }
@@ -1476,11 +1483,14 @@ extern "C" int cg_gated_ff_fwd(const cg_gated_dims* d, const cg_group* grp, cons
     return CG_OK;
 }
 
-static size_t bwd_hidden(const cg_gated_dims* d) { return up256((size_t)d->rows * ldf_of(d) * esize(d->dtype)); }
+// da or dv: fp32 for few rows
+static size_t bwd_hidden(const cg_gated_dims* d, const cg_group* grp) {
+    return up256((size_t)d->rows * ldf_of(d) * (d->rows / grp_n(grp) <= FEW_ROWS ? 4 : esize(d->dtype)));
+}
 static size_t bwd_dy(const cg_gated_dims* d) { return d->dtype == CG_DT_F32 ? 0 : up256((size_t)d->rows * pad8(d->O) * 2); }
 
 extern "C" size_t cg_gated_ff_bwd_workspace(const cg_gated_dims* d, const cg_group* grp) {
-    return dims_ok(d, grp) ? 2 * bwd_hidden(d) + bwd_dy(d) + bwd_part(d, grp) : 0;
+    return dims_ok(d, grp) ? 2 * bwd_hidden(d, grp) + bwd_dy(d) + bwd_part(d, grp) : 0;
 }
 
 extern "C" int cg_gated_ff_bwd(const cg_gated_dims* d, const cg_group* grp, const void* dy, const void* x, const void* wg,
@@ -1495,8 +1505,8 @@ extern "C" int cg_gated_ff_bwd(const cg_gated_dims* d, const cg_group* grp, cons
         return cg_set_error(CG_ERR_WORKSPACE, "cg_gated_ff_bwd: workspace too small");
     CG_DISPATCH_DT(d->dtype, T, {
         char* w = (char*)ws;
-        T *da = (T*)w, *dv = (T*)(w + bwd_hidden(d)), *dyp = (T*)(w + 2 * bwd_hidden(d));
-        float* part = (float*)(w + 2 * bwd_hidden(d) + bwd_dy(d));
+        T *da = (T*)w, *dv = (T*)(w + bwd_hidden(d, grp)), *dyp = (T*)(w + 2 * bwd_hidden(d, grp));
+        float* part = (float*)(w + 2 * bwd_hidden(d, grp) + bwd_dy(d));
         bwd<T>(d, grp, (const T*)dy, (const T*)x, (const T*)wg, (const T*)wv, (const T*)wo, (const T*)h, (const T*)kept, (T*)dx,
                (T*)dwg, (T*)dwv, (T*)dwo, (T*)dbg, (T*)dbv, (T*)dbo, accumulate, (void*)pack, da, dv, dyp, part, cg_s(stream));
     });

@@ -1816,8 +1816,8 @@ def _dropout_explain(x, residual, key):
 def gated_feed_forward(x, w_gate, w_value, w_out=None, b_gate=None, b_value=None, b_out=None, act="silu"):
     """(act(x w_gate^T + b_gate) * (x w_value^T + b_value)) w_out^T + b_out over the rows of x; without w_out the gated hidden units
     themselves.  w_gate / w_value [F, D], w_out [O, F] as nn.Linear keeps them, all in x's type; act: 'silu', 'gelu' (error function)
-    or 'sigmoid'.  Sums, biases and gates are fp32; the hidden units and the gradients of both projections are rounded to x's type once.
-    For the backward pass a call keeps three (16-bit types: four) times its hidden units.  fp32
+    or 'sigmoid'.  Sums, biases and gates are fp32; the hidden units and, of more than 32 rows, the gradients of both projections are
+    rounded to x's type once.  For the backward pass a call keeps three (16-bit types: four) times its hidden units.  fp32
     products are six of three bfloat16 parts of either operand (as exact as an fp32 product; an infinite operand gives NaN).  Under
     ops.members(n) (fp32) every member's rows take its own parameters."""
     params = (w_gate, w_value, w_out, b_gate, b_value, b_out)

@@ -81,7 +81,7 @@ def gate(a, act):
 def gated_ref(x, wg, wv, wo, bg, bv, bo, act, dy):
     """{name: (value, bound without the output's own rounding)}: rows x [M, D], all inputs as the kernel reads them.
 
-    The kernel holds h, da and dv in x's type (one rounding ut each), u = act(a) and p = v act'(a) in the upper 24 bits of their fp32
+    The kernel holds h, da and dv in x's type (one rounding ut each; da and dv of few rows in fp32), u = act(a) and p = v act'(a) in the upper 24 bits of their fp32
     values (16-bit types; cut off: below 2^-15 of the value) and adds in fp32; a product of K terms is off by at most
     (K + 8) U sum|terms|, 4 more roundings an fp32 product that is put together from parts (its parts below 2^-23 are left out, less than 4 U)."""
     t = x.dtype
