@@ -42,7 +42,8 @@ template <typename T> struct Gemm {
 
 // u = act(a), du = act'(a).  The epilogues evaluate this for every hidden unit, where the library's expf, division and erfcf took 16 of the
 // 39 us of a 777 x 2816 gate product: exponentials are one v_exp_f32 (of 2^x), reciprocals one v_rcp_f32, each good to an ulp.
-//   fp32: the argument's product with log2 e is carried in two parts (its rounding alone would cost |a| half ulps of the result);
+//   fp32: the argument's product with log2 e is carried in two parts (its rounding alone would cost |a| half ulps of the result).  Beyond
+//   -88.72 the exponential is infinite and the gate 0 (a clamp that kept it finite would leave silu a multiple of a);
 //   16 bit: one part -- the error stays below 2^-17 for every |a| that does not end in 0 or 1.
 // gelu, 16 bit: erfc(z) = t exp(-z^2 + P(t)), t = 1 / (1 + z / 2), with the degree-9 Chebyshev fit of Press et al., Numerical Recipes,
 // section 6.2 (relative error 1.2e-7 everywhere); fp32: the library's erfcf.
@@ -51,7 +52,7 @@ template <bool FP32> __device__ __forceinline__ float exp_neg(float a) {       /
     if (!FP32) return __builtin_amdgcn_exp2f(-a * L);
     const float c = __builtin_amdgcn_fmed3f(a, -104.f, 104.f), h = -c * L, l = -(__builtin_fmaf(c, L, h) + c * L_LO);
     const float e = __builtin_amdgcn_exp2f(h);
-    return __builtin_fmaf(e, l * 0.69314718f, e);
+    return h < 128.f ? __builtin_fmaf(e, l * 0.69314718f, e) : e;      // from 2^128 on e is infinite, and inf l + inf NaN where l < 0
 }
 template <bool FP32> __device__ __forceinline__ void gate_fn(float a, int gate, float& u, float& du) {
     if (gate == CG_GATE_GELU) {

@@ -270,6 +270,18 @@ def test_gated_feed_forward_gates(cga, act, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ID.get)
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+@pytest.mark.parametrize("rows,D", [(3, 24), (70, 2), (70, 40), (40, 1600), (700, 64)], ids=str)
+def test_gated_feed_forward_over_the_whole_range_of_the_gates(cga, rows, D, act, dtype):
+    """few rows, narrow rows, tiles, sums split over a long axis and several tiles.  The gate's weights are zero, so its arguments are the
+    biases exactly: from -200 to 200, and densely where exp(-a) leaves the range of fp32 (88.72) and where its last bit goes (104)."""
+    edges = torch.cat([torch.linspace(-200, 200, 301), -torch.linspace(88.5, 104.5, 401), torch.linspace(88.5, 104.5, 60)])
+    x, ps, dy = gated_inputs(gen(rows + D), rows, D, edges.numel(), 24, True, dtype)
+    ps[0], ps[3] = torch.zeros_like(ps[0]), edges.to(dtype).cuda()
+    gated_case(cga, x, ps, dy, act)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ID.get)
 def test_gated_feed_forward_large(cga, dtype):
     """several tiles in every direction, sums split over a long axis"""
     x, ps, dy = gated_inputs(gen(4), 5000, 520, 776, 392, True, dtype)
