@@ -21,6 +21,7 @@ inline size_t grp_stride(const cg_group* g) { return g && g->n > 1 ? (size_t)g->
 // (5.9 TB/s), 85 us (4.7 TB/s) and 5 us.
 // ------------------------------------------------------------------------------------------
 constexpr int NT = 256;
+constexpr int MAX_CHANNELS = 1 << 29;       // column indices, also of both sums next to each other (2 C), are ints
 
 // Every kernel of this file takes its arguments as one struct: the runtime looks up each pointer among a launch's arguments, 4 to 7 us
 // for the forward pass's seven pointers when the launching thread changes (the backward pass runs on autograd's own).
@@ -488,8 +489,9 @@ __global__ void dropout_key_kernel(KeyArgs g) {
 
 extern "C" int cg_channel_norm_fwd(const cg_group* grp, const void* x, const void* weight, const void* bias, void* y, float* mean,
                                    float* rstd, size_t rows, int C, int dtype, int wdtype, float eps, cg_stream_t stream) {
-    CG_CHECK_ARG((!rows || (x && y)) && weight && C > 0 && dt_ok(dtype) && (wdtype == dtype || wdtype == CG_DT_F32) && eps >= 0.f &&
-                     !mean == !rstd && rows % grp_n(grp) == 0, "cg_channel_norm_fwd: bad args");
+    CG_CHECK_ARG((!rows || (x && y)) && weight && C > 0 && C <= MAX_CHANNELS && dt_ok(dtype) &&
+                     (wdtype == dtype || wdtype == CG_DT_F32) && eps >= 0.f && !mean == !rstd && rows % grp_n(grp) == 0,
+                 "cg_channel_norm_fwd: bad args");
     if (!rows) return CG_OK;
     const int n = grp_n(grp);
     rows /= n;
@@ -508,7 +510,7 @@ extern "C" int cg_channel_norm_fwd(const cg_group* grp, const void* x, const voi
 }
 
 extern "C" size_t cg_channel_norm_bwd_workspace(const cg_group* grp, size_t rows, int C, int dtype) {
-    if (C <= 0 || !dt_ok(dtype)) return 0;
+    if (C <= 0 || C > MAX_CHANNELS || !dt_ok(dtype)) return 0;
     const int n = grp_n(grp), blocks = norm_blocks(rows / n, C, dtype == CG_DT_F32 ? 4 : 2);
     return blocks == 1 && norm_kind(C, dtype == CG_DT_F32 ? 4 : 2).tpr ? 0 : (size_t)n * blocks * 2 * C * sizeof(float);
 }
@@ -516,8 +518,8 @@ extern "C" size_t cg_channel_norm_bwd_workspace(const cg_group* grp, size_t rows
 extern "C" int cg_channel_norm_bwd(const cg_group* grp, const void* dy, const void* x, const void* weight, const float* mean,
                                    const float* rstd, void* dx, void* dweight, void* dbias, int accumulate, size_t rows, int C,
                                    int dtype, int wdtype, void* ws, size_t ws_bytes, cg_stream_t stream) {
-    CG_CHECK_ARG((!rows || (dy && x && mean && rstd)) && weight && C > 0 && dt_ok(dtype) && (wdtype == dtype || wdtype == CG_DT_F32) &&
-                     rows % grp_n(grp) == 0, "cg_channel_norm_bwd: bad args");
+    CG_CHECK_ARG((!rows || (dy && x && mean && rstd)) && weight && C > 0 && C <= MAX_CHANNELS && dt_ok(dtype) &&
+                     (wdtype == dtype || wdtype == CG_DT_F32) && rows % grp_n(grp) == 0, "cg_channel_norm_bwd: bad args");
     const int n = grp_n(grp);
     const size_t need = cg_channel_norm_bwd_workspace(grp, rows, C, dtype);
     const bool params = dweight || dbias;

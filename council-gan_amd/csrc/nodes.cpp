@@ -145,6 +145,8 @@ struct Members {
 template <typename N> std::shared_ptr<N> make_node() { return std::shared_ptr<N>(new N(), torch::autograd::deleteNode); }
 
 // -- channel_norm ----------------------------------------------------------------------------------
+constexpr int64_t MAX_CHANNELS = 1 << 29;       // as the library has it
+
 struct ChannelNorm : public torch::autograd::Node {
     SavedVariable x_, w_;
     Tensor b_, stats_;
@@ -188,7 +190,7 @@ py::object channel_norm(const Tensor& x, const Tensor& w, const std::optional<Te
     const Tensor b = bias.value_or(Tensor());
     const int64_t C = channels(x);
     const int dt = dt_of(x.scalar_type()), wdt = dt_of(w.scalar_type());
-    if (!x.is_cuda() || C < 1 || C > INT32_MAX || dt < 0 || !(eps >= 0) || w.dim() != 1 || w.size(0) != C || w.device() != x.device() ||
+    if (!x.is_cuda() || C < 1 || C > MAX_CHANNELS || dt < 0 || !(eps >= 0) || w.dim() != 1 || w.size(0) != C || w.device() != x.device() ||
         (wdt != dt && wdt != CG_DT_F32) ||
         (b.defined() && (b.dim() != 1 || b.size(0) != C || b.scalar_type() != w.scalar_type() || b.device() != x.device())))
         return py::none();

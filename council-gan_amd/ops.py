@@ -1740,8 +1740,8 @@ def _member_group(what, x, params):
 
 def channel_norm(x, weight, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the channels of every row (biased variance; ops.layer_norm is the
-    reference's norm over C*H*W of a sample).  weight / bias: [C], both in x's type or both fp32.  Under ops.members(n) every
-    member's rows take its own parameters."""
+    reference's norm over C*H*W of a sample).  weight / bias: [C], both in x's type or both fp32; at most 2^29 channels.  Under
+    ops.members(n) every member's rows take its own parameters."""
     n, stride = _member_group("channel_norm", x, [weight] if bias is None else [weight, bias]) if _G.n > 1 else (1, 0)
     try:
         y = hip.nodes().channel_norm(x, weight, bias, eps, n, stride, getattr(weight, "_cg_grad", None), getattr(bias, "_cg_grad", None))
@@ -1760,6 +1760,8 @@ def _norm_explain(x, weight, bias, eps):
     _check_param(what, "weight", weight, (C,), x, (x.dtype, torch.float32))
     if bias is not None:
         _check_param(what, "bias", bias, (C,), x, (weight.dtype,))
+    if C > 1 << 29:
+        raise ValueError("%s: at most 2^29 channels" % what)
     _check_gpu(what, x)
     raise ValueError("%s: bad arguments" % what)
 

@@ -441,7 +441,7 @@ int cg_layernorm_bwd(const float* dy, const float* x, const float* gamma, const 
 #define CG_DT_BF16 2
 
 /* y = (x - mean) * rstd * weight + bias over the C channels of every row; biased variance, rstd = 1 / sqrt(var + eps).
- * weight / bias: `wdtype` = dtype or CG_DT_F32; bias may be NULL.  mean / rstd (both or neither): [rows], for the backward pass. */
+ * C is at most 2^29.  weight / bias: `wdtype` = dtype or CG_DT_F32; bias may be NULL.  mean / rstd (both or neither): [rows], for the backward pass. */
 int cg_channel_norm_fwd(const cg_group* grp, const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
                         size_t rows, int C, int dtype, int wdtype, float eps, cg_stream_t stream);
 size_t cg_channel_norm_bwd_workspace(const cg_group* grp, size_t rows, int C, int dtype);

@@ -14,6 +14,8 @@ def t(*shape, dtype=torch.float32):
 
 
 KEY = torch.zeros(2, dtype=torch.int64)
+NO_DEVICE = -2              # CG_ERR_LAUNCH: what the check behind a backward pass says where there is no GPU
+WIDE = (1 << 29) + 1        # twice as many columns of sums no longer fit 31 bits with a step past their end
 REFUSED = [
     ("norm_int", lambda: ops.channel_norm(t(2, 4, dtype=torch.int32), t(4)), "float32, float16 or bfloat16"),
     ("norm_double", lambda: ops.channel_norm(t(2, 4, dtype=torch.float64), t(4)), "float32, float16 or bfloat16"),
@@ -26,6 +28,7 @@ REFUSED = [
     ("norm_bias_type", lambda: ops.channel_norm(t(2, 4, dtype=torch.float16), t(4), t(4, dtype=torch.float16)), "bias is"),
     ("norm_eps", lambda: ops.channel_norm(t(2, 4), t(4), None, -1.0), "eps"),
     ("norm_eps_nan", lambda: ops.channel_norm(t(2, 4), t(4), None, float("nan")), "eps"),
+    ("norm_wide", lambda: ops.channel_norm(t(0, WIDE), t(1).expand(WIDE)), "at most 2\\^29"),
     ("drop_p_one", lambda: ops.dropout(t(4), 1.0, KEY), "p must be"),
     ("drop_p_negative", lambda: ops.dropout(t(4), -0.1, KEY), "p must be"),
     ("drop_p_nan", lambda: ops.dropout(t(4), float("nan"), KEY), "p must be"),
@@ -93,6 +96,16 @@ def test_library_refuses_bad_arguments_before_any_launch():
     assert lib.cg_gated_ff_fwd(ctypes.byref(odd), None, p, p, p, p, None, None, None, p, p, p, None, p, 1 << 30, None) == -3
     assert lib.cg_gated_ff_pack_bytes(ctypes.byref(hip.GatedDims(64, 8, 16, 8, 1, 0, 0)), None, p, p, p, p) == 0
     assert lib.cg_gated_ff_pack_bytes(ctypes.byref(hip.GatedDims(64, 8, 16, 8, 1, 0, 0)), None, ctypes.c_void_p(258), p, p, p) > 0
+
+
+def test_library_refuses_rows_past_31_bits():
+    """no rows and no gradients: nothing is launched, whatever the answer"""
+    lib = hip.load()
+    p = ctypes.c_void_p(256)
+    for C, rc in ((WIDE - 1, 0), (WIDE, -1), ((1 << 31) - 1, -1)):
+        assert lib.cg_channel_norm_fwd(None, p, p, None, p, None, None, 0, C, 0, 0, 1e-5, None) == rc
+        assert lib.cg_channel_norm_bwd(None, p, p, p, p, p, None, None, None, 0, 0, C, 0, 0, p, 1 << 40, None) in (rc, rc or NO_DEVICE)
+        assert (lib.cg_channel_norm_bwd_workspace(None, 1, C, 0) == 0) == (rc != 0)
 
 
 def test_workspaces_of_any_size_are_finite():
