@@ -4,6 +4,7 @@
 // backward pass runs on the engine's own thread, often on another core complex, where every Python object it touches is a cache miss.
 // These nodes check the arguments, allocate, and call the library; ops.py explains what was wrong when one of them declines.
 // The library's entry points come in by address (`bind`), so that whichever build of it the process loaded is the one that runs.
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -60,6 +61,22 @@ void once(const char* what) {
 }
 Tensor scratch(size_t bytes, const Tensor& like) {
     return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+
+// What a node saved, dense.  Saved-tensor hooks (activation checkpointing, offloading) may bring it back elsewhere and in another layout,
+// but as the same values.
+Tensor saved(const SavedVariable& s, const char* what, int64_t numel, at::ScalarType type, const at::Device& device) {
+    const Tensor t = dense(s.unpack());
+    TORCH_CHECK(t.numel() == numel && t.scalar_type() == type && t.device() == device, what, s.has_hooks() ?
+                ": a saved tensor came back with another size, type or device" : ": an input changed its size since the forward pass");
+    return t;
+}
+// t itself, or a copy, so far off 16 bytes as `was`: a product's operands have a copy in `pack` or not by that
+Tensor placed(const Tensor& t, const void* was) {
+    if (!t.numel() || (((uintptr_t)t.data_ptr() ^ (uintptr_t)was) & 15) == 0) return t;
+    const int64_t off = ((uintptr_t)was & 15) / t.element_size();
+    const Tensor c = at::empty({t.numel() + off}, t.options()).narrow(0, off, t.numel()).as_strided(t.sizes(), t.strides());
+    return Tensor(c).copy_(t);
 }
 
 // the gradient buffer that a parameter's optimizer keeps (the parameter's _cg_grad), or nothing
@@ -148,8 +165,11 @@ template <typename N> std::shared_ptr<N> make_node() { return std::shared_ptr<N>
 constexpr int64_t MAX_CHANNELS = 1 << 29;       // as the library has it
 
 struct ChannelNorm : public torch::autograd::Node {
-    SavedVariable x_, w_;
-    Tensor b_, stats_;
+    SavedVariable x_, w_, stats_;
+    Tensor b_;
+    size_t rows = 0, C = 0;
+    at::ScalarType type{}, wtype{};
+    c10::Device device{c10::kCUDA, 0};
     Members members;
     Buffer wbuf, bbuf;
 
@@ -157,15 +177,15 @@ struct ChannelNorm : public torch::autograd::Node {
     void release_variables() override {
         x_.reset_data();
         w_.reset_data();
-        stats_.reset();
+        stats_.reset_data();
     }
     variable_list apply(variable_list&& grads) override {
         once("channel_norm");
         variable_list out(3);
         if (!grads[0].defined()) return out;
-        const Tensor x = x_.unpack(), w = w_.unpack(), dy = dense(grads[0]);
-        const size_t C = w.numel(), rows = stats_.size(1);
-        TORCH_CHECK((size_t)x.numel() == rows * C && dy.numel() == x.numel(), "channel_norm: an input changed its size since the forward pass");
+        const char* what = "channel_norm";
+        const Tensor x = saved(x_, what, rows * C, type, device), w = saved(w_, what, C, wtype, device),
+                     stats = saved(stats_, what, 2 * rows, at::kFloat, device), dy = dense(grads[0]);
         const bool need_w = task_should_compute_output(1), need_b = b_.defined() && task_should_compute_output(2);
         Tensor dx;
         if (task_should_compute_output(0)) out[0] = dx = at::empty_like(x);
@@ -174,7 +194,7 @@ struct ChannelNorm : public torch::autograd::Node {
         const int dt = dt_of(x.scalar_type()), wdt = dt_of(w.scalar_type());
         const size_t nws = need_w || need_b ? api.norm_bwd_ws(members.get(), rows, (int)C, dt) : 0;
         const Tensor ws = scratch(nws, x);
-        float* st = (float*)stats_.data_ptr();
+        float* st = (float*)stats.data_ptr();
         check(api.norm_bwd(members.get(), ptr(dy), ptr(x), ptr(w), st, st + rows, ptr(dx), ptr(t[0].out), ptr(t[1].out), t[0].add | t[1].add << 1,
                            rows, (int)C, dt, wdt, ptr(ws), nws, stream_of(x)),
               "cg_channel_norm_bwd");
@@ -226,7 +246,8 @@ py::object channel_norm(const Tensor& x, const Tensor& w, const std::optional<Te
             node->x_ = SavedVariable(xd, false);
             node->w_ = SavedVariable(wd, false);
             node->b_ = bd.defined() ? bd.detach() : bd;
-            node->stats_ = stats;
+            node->stats_ = SavedVariable(stats, false);
+            node->rows = rows, node->C = C, node->type = x.scalar_type(), node->wtype = w.scalar_type(), node->device = x.device();
             node->members = members;
             torch::autograd::set_history(y, node);
         }
@@ -245,7 +266,7 @@ struct Dropout : public torch::autograd::Node {
         once("dropout");
         variable_list out(2);
         if (!grads[0].defined()) return out;
-        const Tensor key = key_.unpack();
+        const Tensor key = saved(key_, "dropout", 2, at::kLong, grads[0].device());
         if (task_should_compute_output(0)) {
             const Tensor dy = dense(grads[0]);
             out[0] = at::empty_like(dy);
@@ -292,8 +313,11 @@ constexpr int64_t MAX_WIDTH = 1 << 21;       // as the library has it
 // -- gated_feed_forward --------------------------------------------------------------------------------
 struct Gated : public torch::autograd::Node {
     SavedVariable x_, wg_, wv_, wo_;
-    Tensor h_, kept_, pack_;      // kept_: u and p; pack_: the forward pass's copies of operands that are not on 16 bytes
+    SavedVariable h_, kept_, pack_;      // kept_: u and p; pack_: the forward pass's copies of operands that are not on 16 bytes
+    int64_t kept_n = 0, pack_n = 0;
     std::array<Tensor, 3> biases;
+    at::ScalarType type{};
+    c10::Device device{c10::kCUDA, 0};
     cg_gated_dims dims{};
     Members members;
     std::array<Buffer, 6> bufs;
@@ -305,19 +329,29 @@ struct Gated : public torch::autograd::Node {
         wg_.reset_data();
         wv_.reset_data();
         wo_.reset_data();
-        h_.reset();
-        kept_.reset();
-        pack_.reset();
+        h_.reset_data();
+        kept_.reset_data();
+        pack_.reset_data();
     }
     variable_list apply(variable_list&& grads) override {
         once("gated_feed_forward");
         variable_list out(7);
         if (!grads[0].defined()) return out;
-        const Tensor x = x_.unpack(), dy = dense(grads[0]);
-        const std::array<Tensor, 6> p{wg_.unpack(), wv_.unpack(), dims.O ? wo_.unpack() : Tensor(), biases[0], biases[1], biases[2]};
-        // (pack_ holds copies of those that needed one)
-        TORCH_CHECK((read == std::array<void*, 4>{ptr(x), ptr(p[0]), ptr(p[1]), ptr(p[2])}) && x.numel() == dims.rows * dims.D,
-                    "gated_feed_forward: an operand moved since the forward pass");
+        const char* what = "gated_feed_forward";
+        const int64_t D = dims.D, F = dims.F, O = dims.O;
+        auto operand = [&](const SavedVariable& s, int i, int64_t numel) {
+            const Tensor t = saved(s, what, numel, type, device);
+            TORCH_CHECK(s.has_hooks() || ptr(t) == read[i], what, ": an operand moved since the forward pass");
+            return placed(t, read[i]);
+        };
+        auto own = [&](const SavedVariable& s, int64_t numel, at::ScalarType as) {
+            return numel ? placed(saved(s, what, numel, as, device), nullptr) : Tensor();
+        };
+        const Tensor x = operand(x_, 0, dims.rows * D), dy = dense(grads[0]);
+        const std::array<Tensor, 6> p{operand(wg_, 1, F * D), operand(wv_, 2, F * D), O ? operand(wo_, 3, O * F) : Tensor(),
+                                      biases[0], biases[1], biases[2]};
+        const int64_t pitch = (F + 7) & ~(int64_t)7;
+        const Tensor h = own(h_, O ? dims.rows * pitch : 0, type), kept = own(kept_, kept_n, type), pack = own(pack_, pack_n, at::kByte);
         Tensor dx;
         if (task_should_compute_output(0)) out[0] = dx = at::empty_like(x);
         std::array<void*, 6> to;
@@ -334,8 +368,8 @@ struct Gated : public torch::autograd::Node {
         }
         const size_t nws = api.gated_bwd_ws(&dims, members.get());
         const Tensor ws = scratch(nws, x);
-        check(api.gated_bwd(&dims, members.get(), ptr(dy), ptr(x), ptr(p[0]), ptr(p[1]), ptr(p[2]), ptr(h_), ptr(kept_), ptr(dx), to[0], to[1], to[2],
-                            to[3], to[4], to[5], add, ptr(pack_), ptr(ws), nws, stream_of(x)),
+        check(api.gated_bwd(&dims, members.get(), ptr(dy), ptr(x), ptr(p[0]), ptr(p[1]), ptr(p[2]), ptr(h), ptr(kept), ptr(dx), to[0], to[1], to[2],
+                            to[3], to[4], to[5], add, ptr(pack), ptr(ws), nws, stream_of(x)),
               "cg_gated_ff_bwd");
         settle(t);
         return out;
@@ -409,12 +443,14 @@ py::object gated(const Tensor& x, const Tensor& wg, const Tensor& wv, const std:
             node->wv_ = SavedVariable(p[1], false);
             if (O) {
                 node->wo_ = SavedVariable(p[2], false);
-                node->h_ = h;
+                node->h_ = SavedVariable(h, false);
             }
             for (int i = 0; i < 3; ++i)
                 if (p[3 + i].defined()) node->biases[i] = p[3 + i].detach();
-            node->kept_ = kept;
-            node->pack_ = pack;
+            node->kept_ = SavedVariable(kept, false);
+            node->kept_n = kept.numel();
+            if (pack.defined()) node->pack_ = SavedVariable(pack, false), node->pack_n = pack.numel();
+            node->type = x.scalar_type(), node->device = x.device();
             node->dims = dims;
             node->members = members;
             node->read = {ptr(xd), ptr(p[0]), ptr(p[1]), ptr(p[2])};
@@ -447,8 +483,8 @@ void bind(const py::dict& d) {
 
 PYBIND11_MODULE(cg_nodes, m) {
     m.def("bind", &bind);
-    // None: the arguments do not fit (ops.py says which)
-    m.def("channel_norm", &channel_norm);
-    m.def("dropout", &dropout);
-    m.def("gated", &gated);
+    // None: the arguments do not fit (ops.py says which).  Wrapped: exceptions of saved-tensor hooks pass through as they are.
+    m.def("channel_norm", torch::wrap_pybind_function(channel_norm));
+    m.def("dropout", torch::wrap_pybind_function(dropout));
+    m.def("gated", torch::wrap_pybind_function(gated));
 }

@@ -92,6 +92,17 @@ def test_block_with_dropout_drops_what_it_adds(cga):
     assert bool(((g - want).abs() <= 8 * 2.0 ** -24 * (g.abs() + dy.abs() * 4 + (g - dy).abs())).all())
 
 
+def test_block_checkpointed(cga):
+    from torch.utils.checkpoint import checkpoint
+    torch.manual_seed(8)
+    b = cga.GatedBlock(32, 64).cuda()
+    x, dy = torch.randn(70, 32, device="cuda", requires_grad=True), torch.randn(70, 32, device="cuda")
+    leaves = [x] + list(b.parameters())
+    want = torch.autograd.grad(b(x), leaves, dy)
+    got = torch.autograd.grad(checkpoint(b, x, use_reentrant=False), leaves, dy)
+    assert all(torch.equal(a, c) for a, c in zip(want, got))
+
+
 @pytest.mark.parametrize("council,group,drop", [(2, None, 0.0), (2, None, 0.25), (2, 1, 0.25)])
 def test_trainer_with_a_gated_style_mlp(cga, council, group, drop):
     """Training runs, moves the block's weights, and a captured iteration repeats the eager one's bits, masks included."""

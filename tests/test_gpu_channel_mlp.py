@@ -603,6 +603,91 @@ def test_an_operand_that_moved_is_refused(cga):
         y.backward(dy)
 
 
+# rows, dims, shift: elements by which every operand starts off 16 bytes
+HOOKED = [(F32, 20, 64, 96, 0), (F32, 70, 33, 47, 1), (F16, 20, 64, 96, 1), (F16, 70, 64, 96, 1), (BF16, 90, 64, 96, 0), (BF16, 150, 33, 47, 0)]
+
+
+def shifted(t, k):
+    out = torch.empty(t.numel() + 16, dtype=t.dtype, device=t.device)[k:k + t.numel()].view(t.shape)
+    return out.copy_(t.detach())
+
+
+def train(cga, tensors, dy, hooks):
+    """a step of norm and gated block under saved-tensor hooks: y and all gradients"""
+    leaves = [t.detach().requires_grad_(True) for t in tensors]
+    with hooks:
+        y = cga.ops.gated_feed_forward(cga.ops.channel_norm(*leaves[:3]), *leaves[3:])
+    return [y.detach()] + list(torch.autograd.grad(y, leaves, dy))
+
+
+@pytest.mark.parametrize("dtype,rows,D,F,shift", HOOKED, ids=str)
+def test_saved_tensors_may_come_back_elsewhere(cga, dtype, rows, D, F, shift):
+    """on the host and back, and as copies on 16 bytes or off them, of any operand and of what the calls keep"""
+    g = gen(50)
+    x, ps, dy = gated_inputs(g, rows, D, F, 40, True, dtype)
+    ts = [shifted(t, shift) for t in (x, rnd(g, D, dtype=dtype), rnd(g, D, dtype=dtype), *ps)]
+    plain = torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t)
+    want = train(cga, ts, dy, plain)
+    import contextlib
+    for a, b in zip(want, train(cga, ts, dy, contextlib.nullcontext())):
+        assert torch.equal(a, b)
+    for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.save_on_cpu(pin_memory=True),
+                  torch.autograd.graph.saved_tensors_hooks(lambda t: shifted(t, 1), lambda t: t),
+                  torch.autograd.graph.saved_tensors_hooks(lambda t: shifted(t, 0), lambda t: t)):
+        got = train(cga, ts, dy, hooks)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_saved_images_may_come_back_in_another_layout(cga):
+    g = gen(51)
+    x, dy = rnd(g, 2, 24, 3, 5, dtype=F16).contiguous(memory_format=torch.channels_last), rnd(g, 2, 40, 3, 5, dtype=F16)
+    ts = [x, rnd(g, 24, dtype=F16), rnd(g, 24, dtype=F16), rnd(g, 40, 24, dtype=F16), rnd(g, 40, 24, dtype=F16)]
+    want = train(cga, ts, dy, torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t))
+    got = train(cga, ts, dy, torch.autograd.graph.saved_tensors_hooks(lambda t: t.contiguous(), lambda t: t))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_a_saved_tensor_that_comes_back_as_another_is_refused(cga):
+    g = gen(52)
+    x, ps, dy = gated_inputs(g, 40, 24, 32, 16, False, F32)
+    w = rnd(g, 24)
+    half = lambda t: t.half() if t.is_floating_point() else t.int()
+    for f in (lambda: cga.ops.gated_feed_forward(x.requires_grad_(True), *ps), lambda: cga.ops.channel_norm(x.requires_grad_(True), w),
+              lambda: cga.ops.dropout(x.requires_grad_(True), 0.5, key_of(1, 2))):
+        for change in (half, lambda t: t[..., :-1]):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+                y = f()
+            with pytest.raises(RuntimeError, match="came back"):
+                y.sum().backward()
+
+
+@pytest.mark.parametrize("dtype,rows", [(F32, 24), (F32, 500), (BF16, 500)], ids=str)
+def test_checkpointed(cga, dtype, rows):
+    """the same bits as without, and nothing kept but the input"""
+    from torch.utils.checkpoint import checkpoint
+    g = gen(53)
+    D, F = 256, 1024
+    x, ps, dy = gated_inputs(g, rows, D, F, D, True, dtype)
+    w, b = rnd(g, D, dtype=dtype), rnd(g, D, dtype=dtype)
+
+    def step(run):
+        leaves = [t.detach().clone().requires_grad_(True) for t in [x, w, b] + ps]
+
+        def f(t):
+            return t + cga.ops.gated_feed_forward(cga.ops.channel_norm(t, *leaves[1:3]), *leaves[3:])
+        before = torch.cuda.memory_allocated()
+        y = run(f, run(f, leaves[0]))
+        kept = torch.cuda.memory_allocated() - before
+        y.backward(dy)                                  # a reentrant checkpoint takes no autograd.grad
+        return kept, [y.detach()] + [t.grad for t in leaves]
+    kept0, want = step(lambda f, t: f(t))
+    kept1, got = step(lambda f, t: checkpoint(f, t, use_reentrant=False))
+    _, again = step(lambda f, t: checkpoint(f, t, use_reentrant=True))
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and all(torch.equal(a, b) for a, b in zip(want, again))
+    hidden = rows * F * x.element_size()
+    assert kept0 > 6 * hidden and kept1 <= 2 * rows * D * x.element_size() + 4096
+
+
 def test_capture_beside_a_living_eager_graph_is_refused(cga):
     x, ps, dy = gated_inputs(gen(34), 40, 32, 48, 32, False, F32)
     w = torch.ones(32, device="cuda", requires_grad=True)
