@@ -215,7 +215,8 @@ class ChannelNorm(nn.Module):
 class Dropout(nn.Module):
     """residual + dropout(x): ops.dropout while training, the identity otherwise.  `state` ({seed, step}; seeded from torch's generator
     unless given) advances with every call and belongs to the state_dict; p = 0 has none.  Calls advance it in the order of their
-    streams: two streams must not run the same module at once."""
+    streams: two streams must not run the same module at once.  A call that is given its `key` (ops.dropout_key(state), drawn outside
+    of a checkpointed function) leaves the state alone."""
 
     def __init__(self, p=0.0, seed=None):
         super().__init__()
@@ -225,14 +226,15 @@ class Dropout(nn.Module):
         if p > 0:
             self.register_buffer('state', ops.dropout_state(int(torch.randint(1 << 62, ())) if seed is None else seed, device='cpu'))
 
-    def forward(self, x, residual=None):
+    def forward(self, x, residual=None, key=None):
         if self.p > 0 and self.training:
-            return ops.dropout(x, self.p, ops.dropout_key(self.state), residual)
+            return ops.dropout(x, self.p, ops.dropout_key(self.state) if key is None else key, residual)
         return x if residual is None else residual + x
 
 
 class GatedBlock(nn.Module):
-    """x + dropout(gated_feed_forward(channel_norm(x))) over the channels of every row; `hidden` gated units (4 * dim by default)."""
+    """x + dropout(gated_feed_forward(channel_norm(x))) over the channels of every row; `hidden` gated units (4 * dim by default).
+    `key`: as Dropout takes it."""
 
     def __init__(self, dim, hidden=None, activation='silu', dropout=0.0):
         super().__init__()
@@ -246,10 +248,10 @@ class GatedBlock(nn.Module):
         self.out = nn.Linear(hidden, dim)
         self.drop = Dropout(dropout)
 
-    def forward(self, x):
+    def forward(self, x, key=None):
         y = ops.gated_feed_forward(self.norm(x), self.gate.weight, self.value.weight, self.out.weight, self.gate.bias, self.value.bias,
                                    self.out.bias, self.activation)
-        return self.drop(y, x)
+        return self.drop(y, x, key)
 
 
 ##################################################################################

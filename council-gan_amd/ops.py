@@ -1781,8 +1781,12 @@ def _check_key(what, t):
 
 def dropout_key(state):
     """The key of one dropout call: a copy of `state` taken on the device, whose step then advances -- captured into a graph, every
-    replay draws a new mask."""
+    replay draws a new mask.  Refused inside a running backward pass, where activation checkpointing runs its function again: the key
+    would be another than the forward pass's.  A checkpointed function takes its key as an argument."""
     _check_key("dropout_key", state)
+    if torch._C._current_graph_task_id() != -1:
+        raise hip.HipError("dropout_key: inside a backward pass a recomputed call would draw another mask: draw the key outside of "
+                           "the checkpointed function and pass it in")
     with torch.cuda.device(state.device):
         key = torch.empty_like(state)
         check(_lib().cg_dropout_key(state.data_ptr(), key.data_ptr(), hip._stream_handle()), "cg_dropout_key")

@@ -103,6 +103,35 @@ def test_block_checkpointed(cga):
     assert all(torch.equal(a, c) for a, c in zip(want, got))
 
 
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpointed_dropout_draws_no_other_mask(cga, reentrant):
+    """A checkpoint runs its function again inside the backward pass: a key drawn there would be another mask than the forward pass's."""
+    from torch.utils.checkpoint import checkpoint
+    torch.manual_seed(9)
+    b = cga.GatedBlock(32, 64, dropout=0.5).cuda()
+    x, dy = torch.randn(70, 32, device="cuda", requires_grad=True), torch.randn(70, 32, device="cuda")
+    with pytest.raises(cga.hip.HipError, match="another mask"):
+        checkpoint(b, x, use_reentrant=reentrant).backward(dy)
+    leaves = [x] + list(b.parameters())
+
+    def step(run):
+        for t in leaves:
+            t.grad = None
+        y = run(cga.ops.dropout_key(b.drop.state))
+        y.backward(dy)
+        return [y.detach()] + [t.grad for t in leaves]
+    saved = b.drop.state.clone()
+    want = step(lambda key: b(x, key))
+    assert b.drop.state.tolist() == [int(saved[0]), int(saved[1]) + 1]
+    b.drop.state.copy_(saved)
+    got = step(lambda key: checkpoint(b, x, key, use_reentrant=reentrant))
+    b.drop.state.copy_(saved)
+    drawn = step(lambda key: b(x, key))
+    assert all(torch.equal(a, c) and torch.equal(a, d) for a, c, d in zip(want, got, drawn))
+    b.drop.state.copy_(saved)
+    assert torch.equal(b(x), want[0])           # the key that the block draws by itself
+
+
 @pytest.mark.parametrize("council,group,drop", [(2, None, 0.0), (2, None, 0.25), (2, 1, 0.25)])
 def test_trainer_with_a_gated_style_mlp(cga, council, group, drop):
     """Training runs, moves the block's weights, and a captured iteration repeats the eager one's bits, masks included."""
