@@ -59,6 +59,11 @@ bool grad_on(const Tensor& t) { return t.defined() && t.requires_grad(); }
 void once(const char* what) {
     TORCH_CHECK(!c10::GradMode::is_enabled(), what, ": the backward pass cannot be differentiated again");
 }
+// the operators have no forward-mode formulas: a tangent would be lost without a word
+void refuse_tangents(const char* what, std::initializer_list<const Tensor*> inputs) {
+    for (const Tensor* t : inputs)
+        TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what, ": forward-mode differentiation is not supported");
+}
 Tensor scratch(size_t bytes, const Tensor& like) {
     return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
@@ -208,6 +213,7 @@ struct ChannelNorm : public torch::autograd::Node {
 py::object channel_norm(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, double eps, int n, int64_t stride,
                         const py::object& wbuf, const py::object& bbuf) {
     const Tensor b = bias.value_or(Tensor());
+    refuse_tangents("channel_norm", {&x, &w, &b});
     const int64_t C = channels(x);
     const int dt = dt_of(x.scalar_type()), wdt = dt_of(w.scalar_type());
     if (!x.is_cuda() || C < 1 || C > MAX_CHANNELS || dt < 0 || !(eps >= 0) || w.dim() != 1 || w.size(0) != C || w.device() != x.device() ||
@@ -280,6 +286,7 @@ struct Dropout : public torch::autograd::Node {
 
 py::object dropout(const Tensor& x, const std::optional<Tensor>& residual, int threshold, const Tensor& key) {
     const Tensor res = residual.value_or(Tensor());
+    refuse_tangents("dropout", {&x, &res});
     const int dt = dt_of(x.scalar_type());
     if (!x.is_cuda() || x.dim() < 1 || dt < 0 || key.scalar_type() != at::kLong || key.numel() != 2 || !key.is_contiguous() ||
         key.device() != x.device() ||
@@ -382,6 +389,7 @@ py::object gated(const Tensor& x, const Tensor& wg, const Tensor& wv, const std:
     const Tensor none;
     const Tensor wo = w_out.value_or(none);
     const std::array<Tensor, 3> b{b_gate.value_or(none), b_value.value_or(none), b_out.value_or(none)};
+    refuse_tangents("gated_feed_forward", {&x, &wg, &wv, &wo, &b[0], &b[1], &b[2]});
     const int dt = dt_of(x.scalar_type());
     auto like = [&](const Tensor& t) { return t.scalar_type() == x.scalar_type() && t.device() == x.device(); };
     if (!x.is_cuda() || dt < 0 || gate < 0 || wg.dim() != 2 || wv.dim() != 2 || wg.sizes() != wv.sizes() || !like(wg) || !like(wv) ||

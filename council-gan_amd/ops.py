@@ -1700,8 +1700,9 @@ def l1_mean(a, b):
 # accumulators are fp32, every stored value is rounded once.  Scratch memory comes from torch's caching allocator, per call: a captured
 # graph owns its own, and two graphs share none.  All of them run on the current stream of the tensors' device.  The calls and their
 # autograd nodes are C++ (csrc/nodes.cpp); a node declines arguments that do not fit, and the functions here say what is wrong with them.
-# Gradients of a parameter that carries `_cg_grad` are added to that buffer; the backward passes cannot be differentiated again.  All that a
-# call keeps for its backward pass goes through torch's saved-tensor hooks (activation checkpointing, offloading).
+# Gradients of a parameter that carries `_cg_grad` are added to that buffer; the backward passes cannot be differentiated again, and there
+# is no forward mode.  All that a call keeps for its backward pass goes through torch's saved-tensor hooks (activation checkpointing,
+# offloading).
 def _check_rows(what, x):
     if not isinstance(x, torch.Tensor) or x.dtype not in hip.DT:
         raise ValueError("%s: x must be a float32, float16 or bfloat16 tensor" % what)

@@ -66,6 +66,21 @@ def test_no_cpu_fallback():
             call()
 
 
+@pytest.mark.parametrize("call", [
+    lambda d: ops.channel_norm(d(2, 4), t(4)), lambda d: ops.channel_norm(t(2, 4), d(4)), lambda d: ops.channel_norm(t(2, 4), t(4), d(4)),
+    lambda d: ops.dropout(d(2, 4), 0.5, KEY), lambda d: ops.dropout(t(2, 4), 0.5, KEY, residual=d(2, 4)),
+    lambda d: ops.gated_feed_forward(d(2, 4), t(6, 4), t(6, 4)), lambda d: ops.gated_feed_forward(t(2, 4), t(6, 4), d(6, 4)),
+    lambda d: ops.gated_feed_forward(t(2, 4), t(6, 4), t(6, 4), d(3, 6)),
+    lambda d: ops.gated_feed_forward(t(2, 4), t(6, 4), t(6, 4), t(3, 6), b_out=d(3))],
+    ids=["norm_x", "norm_w", "norm_b", "drop_x", "drop_residual", "gated_x", "gated_value", "gated_out", "gated_bias"])
+def test_forward_mode_tangents_are_refused(call):
+    """none is lost in silence; the refusal comes before the one of the device"""
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call(lambda *s: fw.make_dual(torch.zeros(*s), torch.ones(*s)))
+
+
 def test_library_refuses_bad_arguments_before_any_launch():
     lib = hip.load()
     p = ctypes.c_void_p(256)
