@@ -52,7 +52,11 @@ int dt_of(at::ScalarType t) {
     return t == at::kFloat ? CG_DT_F32 : t == at::kHalf ? CG_DT_F16 : t == at::kBFloat16 ? CG_DT_BF16 : -1;
 }
 int64_t channels(const Tensor& x) { return x.dim() == 4 ? x.size(1) : x.dim() ? x.size(-1) : 0; }
-Tensor dense(const Tensor& t) { return t.dim() == 4 ? t.contiguous(at::MemoryFormat::ChannelsLast) : t.contiguous(); }
+// what a kernel reads: no gaps, and no sign kept as a bit beside the values (a view of a conjugate's imaginary part)
+Tensor dense(const Tensor& v) {
+    const Tensor t = v.is_neg() ? v.resolve_neg() : v;
+    return t.dim() == 4 ? t.contiguous(at::MemoryFormat::ChannelsLast) : t.contiguous();
+}
 // the device memory of a tensor that may be undefined (no data_ptr of a tensor without storage is taken)
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 bool grad_on(const Tensor& t) { return t.defined() && t.requires_grad(); }
@@ -238,8 +242,8 @@ py::object channel_norm(const Tensor& x, const Tensor& w, const std::optional<Te
             const at::NoGradGuard plain;
             if (record) refuse_eager_graph("channel_norm", {{&x, nullptr}, {&w, &node->wbuf}, {&b, &node->bbuf}});
             xd = dense(x);
-            wd = w.contiguous();
-            if (b.defined()) bd = b.contiguous();
+            wd = dense(w);
+            if (b.defined()) bd = dense(b);
             y = at::empty_like(xd);
             if (record) stats = at::empty({2, (int64_t)rows}, x.options().dtype(at::kFloat));
             float* st = record ? (float*)stats.data_ptr() : nullptr;
@@ -427,7 +431,7 @@ py::object gated(const Tensor& x, const Tensor& wg, const Tensor& wv, const std:
                                                           {&b[0], &node->bufs[3]}, {&b[1], &node->bufs[4]}, {&b[2], &node->bufs[5]}});
             xd = dense(x);
             for (Tensor& t : p)
-                if (t.defined()) t = t.contiguous();
+                if (t.defined()) t = dense(t);
             auto rows_like = [&](int64_t c) {
                 std::vector<int64_t> s = x.sizes().vec();
                 s[x.dim() == 4 ? 1 : x.dim() - 1] = c;

@@ -594,6 +594,26 @@ def test_one_buffer_for_two_parameters(cga):
         assert bool(((t._cg_grad.double() - want).abs() <= tol).all())
 
 
+def test_negated_views(cga):
+    """views that carry their sign as a bit (the imaginary part of a conjugate), as inputs, parameters and gradients"""
+    g = gen(35)
+    x, ps, dy = gated_inputs(g, 40, 24, 32, 24, True, F32)
+    w, b = rnd(g, 24), rnd(g, 24)
+    key = key_of(1, 2)
+    one = torch.complex(rnd(g, 1, 1), rnd(g, 1, 1)).conj().imag
+    assert one.is_neg() and one.is_contiguous()
+    n = torch._neg_view
+    for f, ts in ((lambda *t: cga.ops.channel_norm(*t), [x, w, b]), (lambda t, r: cga.ops.dropout(t, 0.25, key, r), [x, dy]),
+                  (lambda *t: cga.ops.gated_feed_forward(*t), [x] + ps)):
+        for i in range(len(ts)):
+            a = [n(t) if k == i else t for k, t in enumerate(ts)]
+            assert torch.equal(f(*a), f(*[t.resolve_neg().clone() for t in a]))
+        leaves = [t.detach().clone().requires_grad_(True) for t in ts]
+        for p, q in zip(torch.autograd.grad(f(*leaves), leaves, n(dy)), torch.autograd.grad(f(*leaves), leaves, -dy)):
+            assert torch.equal(p, q)
+    assert torch.equal(cga.ops.dropout(one, 0.0, key), one.resolve_neg())
+
+
 def test_an_operand_that_moved_is_refused(cga):
     x, ps, dy = gated_inputs(gen(33), 40, 33, 47, 31, False, F16)
     leaves = [t.requires_grad_(True) for t in ps[:3]]
