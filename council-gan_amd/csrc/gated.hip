@@ -873,6 +873,11 @@ template <typename T, bool KA, bool KB, int EPI, bool BLOCK> __global__ __launch
 // the rows, one value a lane (lane l: column or row l % 16, K-step l / 16): with weights that are K-contiguous a lane loads 16 bytes of
 // its row and the K-steps of a product are whichever the lanes hold; row-contiguous weights need no transposition at all.  Every type is
 // multiplied in fp32 (16-bit K-contiguous operands on v_mfma_f32_16x16x32, which takes the 16 bytes as they are), and da and dv stay fp32.
+// h is rounded to the type: as two 16-bit parts it would cost 8 % of a call of 1 x 1024 x 2816 bf16 and 24 % of 32 x 2048 x 5632.
+// FEW_ROWS: as many rows as a block's join has threads for (16 rows x 2 blocks x 2 tiles).  us of these kernels against the tiles, in replayed
+// graphs, serving and training: 16 x 256 x 1024 fp32 10 / 33 against 27 / 68, 32 rows 13 / 40 against 29 / 70; 32 x 1024 x 4096 fp32 37 / 135
+// against 44 / 123; bf16 16 x 1024 x 2816 13 / 61 against 24 / 75, 32 rows 16 / 105 against 25 / 82; 16 x 2048 x 5632 28 / 127 against
+// 35 / 114, 32 rows 37 / 227 against 34 / 115.  Of wide layers the tiles would be the better backward pass from some 17 rows on.
 // ------------------------------------------------------------------------------------------
 constexpr int FEW_ROWS = 32, FEW_WAVES = 16;
 

@@ -215,7 +215,8 @@ class ChannelNorm(nn.Module):
 class Dropout(nn.Module):
     """residual + dropout(x): ops.dropout while training, the identity otherwise.  `state` ({seed, step}; seeded from torch's generator
     unless given) advances with every call and belongs to the state_dict; p = 0 has none.  Calls advance it in the order of their
-    streams: two streams must not run the same module at once.  A call that is given its `key` (ops.dropout_key(state), drawn outside
+    streams: two streams must not run the same module at once.  Under ops.members(n) the lead member's state draws the mask of
+    all members' rows, and the others' stays as it was: another grouping of the members draws other masks.  A call that is given its `key` (ops.dropout_key(state), drawn outside
     of a checkpointed function) leaves the state alone."""
 
     def __init__(self, p=0.0, seed=None):
