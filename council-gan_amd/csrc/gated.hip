@@ -43,7 +43,8 @@ template <typename T> struct Gemm {
 // u = act(a), du = act'(a).  The epilogues evaluate this for every hidden unit, where the library's expf, division and erfcf took 16 of the
 // 39 us of a 777 x 2816 gate product: exponentials are one v_exp_f32 (of 2^x), reciprocals one v_rcp_f32, each good to an ulp.
 //   fp32: the argument's product with log2 e is carried in two parts (its rounding alone would cost |a| half ulps of the result).  Beyond
-//   -88.72 the exponential is infinite and the gate 0 (a clamp that kept it finite would leave silu a multiple of a);
+//   -88.72 the exponential is infinite and the gate 0 (a clamp that kept it finite would leave silu a multiple of a); from -87.34 on its
+//   reciprocal is below the normal numbers, which v_rcp_f32 gives as 0 (off by 1e-38, silu by 1e-36);
 //   16 bit: one part -- the error stays below 2^-17 for every |a| that does not end in 0 or 1.
 // gelu, 16 bit: erfc(z) = t exp(-z^2 + P(t)), t = 1 / (1 + z / 2), with the degree-9 Chebyshev fit of Press et al., Numerical Recipes,
 // section 6.2 (relative error 1.2e-7 everywhere); fp32: the library's erfcf.

@@ -1826,8 +1826,8 @@ def gated_feed_forward(x, w_gate, w_value, w_out=None, b_gate=None, b_value=None
     themselves.  w_gate / w_value [F, D], w_out [O, F] as nn.Linear keeps them, all in x's type; act: 'silu', 'gelu' (error function)
     or 'sigmoid'.  Sums, biases and gates are fp32; the hidden units and, of more than 32 rows, the gradients of both projections are
     rounded to x's type once.  For the backward pass a call keeps three (16-bit types: four) times its hidden units.  fp32
-    products are six of three bfloat16 parts of either operand (as exact as an fp32 product; an infinite operand gives NaN).  Under
-    ops.members(n) (fp32) every member's rows take its own parameters."""
+    products are six of three bfloat16 parts of either operand (as exact as an fp32 product; an operand that bfloat16 holds as
+    infinite gives NaN).  Under ops.members(n) (fp32) every member's rows take its own parameters."""
     params = (w_gate, w_value, w_out, b_gate, b_value, b_out)
     n, stride = _member_group("gated_feed_forward", x, [p for p in params if p is not None]) if _G.n > 1 else (1, 0)
     bufs = tuple([getattr(p, "_cg_grad", None) for p in params])
