@@ -1732,6 +1732,11 @@ def _member_group(what, x, params):
     pool = getattr(params[0], '_cg_pool', None)
     if pool is None or any(getattr(p, '_cg_pool', None) is not pool for p in params) or not all(p.is_contiguous() for p in params):
         raise hip.HipError("member-batched %s: the parameters must live in one optim.ParamPool" % what)
+    at = [pool.index_of(p) for p in params]
+    if any(i is None or i[0] != at[0][0] for i in at):
+        raise hip.HipError("member-batched %s: the parameters must be one member's" % what)
+    if at[0][0] + _G.n > len(pool.opts):
+        raise hip.HipError("member-batched %s: %d members from member %d on of a pool of %d" % (what, _G.n, at[0][0], len(pool.opts)))
     if x.dtype != torch.float32:
         raise hip.HipError("member-batched %s: the pools hold fp32 parameters" % what)
     rows = x.numel() // max(1, _check_rows(what, x))

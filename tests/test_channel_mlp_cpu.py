@@ -81,6 +81,24 @@ def test_forward_mode_tangents_are_refused(call):
             call(lambda *s: fw.make_dual(torch.zeros(*s), torch.ones(*s)))
 
 
+def test_members_past_the_end_of_the_pool_are_refused():
+    """a batched call reads and writes n members' parameters from its own on: all of them must be there"""
+    from council_gan_amd.optim import FlatAdam, ParamPool
+    ps = [[torch.nn.Parameter(torch.zeros(s)) for s in ((4,), (4,), (6, 4), (6, 4), (3, 6))] for _ in range(2)]
+    ParamPool([FlatAdam(p) for p in ps]).materialize("cpu")
+    a, b = ps
+    calls = [lambda p, q: ops.channel_norm(t(6, 4), p[0], q[1]), lambda p, q: ops.gated_feed_forward(t(6, 4), p[2], p[3], q[4])]
+    for f in calls:
+        with ops.members(3), pytest.raises(hip.HipError, match="pool of 2"):
+            f(a, a)
+        with ops.members(2), pytest.raises(hip.HipError, match="pool of 2"):
+            f(b, b)
+        with ops.members(2), pytest.raises(hip.HipError, match="one member"):
+            f(a, b)
+        with ops.members(2), pytest.raises(hip.HipError, match="no CPU fallback"):
+            f(a, a)
+
+
 def test_library_refuses_bad_arguments_before_any_launch():
     lib = hip.load()
     p = ctypes.c_void_p(256)
