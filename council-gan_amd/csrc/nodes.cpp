@@ -120,6 +120,8 @@ struct Target { Tensor out, ret, shared; bool add = false; };       // what the 
 Target target(const Tensor& p, const Buffer& buf, bool wanted, int members) {
     Target r;
     if (!p.defined() || !wanted) return r;
+    TORCH_CHECK(!buf.t.defined() || (buf.t.device() == p.device() && buf.t.sizes() == p.sizes()),
+                "a parameter's gradient buffer is on another device, or has another shape: its optimizer was materialized before the parameter moved");
     if (buf.t.defined() && buf.t.scalar_type() == p.scalar_type() && buf.t.is_contiguous()) {
         buf.touch();
         r.out = buf.t;

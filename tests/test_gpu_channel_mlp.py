@@ -574,6 +574,20 @@ def test_gradients_add_to_the_optimizer_buffers(cga):
         assert torch.equal(t.grad, 2 * a)
 
 
+def test_a_gradient_buffer_that_does_not_fit_is_refused(cga):
+    """on the host, as after optimizer.materialize("cpu") and module.cuda(), or of another size: nothing is written"""
+    g = gen(36)
+    x, dy = rnd(g, 20, 32), rnd(g, 20, 32)
+    for bad in (lambda t: torch.zeros(t.shape), lambda t: torch.zeros(t.numel() // 2, device="cuda")):
+        for i in range(8):
+            p = [t.detach().cuda().requires_grad_(True) for t in member_params(1, 32, 40, g)[0]]
+            p[i]._cg_grad = bad(p[i])
+            y = cga.ops.gated_feed_forward(cga.ops.channel_norm(x, p[0], p[1]), *p[2:])
+            with pytest.raises(RuntimeError, match="gradient buffer"):
+                y.backward(dy)
+            assert not p[i]._cg_grad.any()
+
+
 def test_one_buffer_for_two_parameters(cga):
     """A tensor that serves as two parameters gets the sum of both gradients in its one buffer."""
     g = gen(32)
