@@ -1,5 +1,8 @@
 """channel_norm, dropout and gated_feed_forward on the GPU against plain 64-bit forms (channel_mlp_ref.py), forward and backward:
 every type, odd sizes and strides, one row to long ones, no rows, streams, captured graphs, member-batched parameters."""
+import contextlib
+import gc
+
 import numpy as np
 import pytest
 import torch
@@ -662,7 +665,6 @@ def test_saved_tensors_may_come_back_elsewhere(cga, dtype, rows, D, F, shift):
     ts = [shifted(t, shift) for t in (x, rnd(g, D, dtype=dtype), rnd(g, D, dtype=dtype), *ps)]
     plain = torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t)
     want = train(cga, ts, dy, plain)
-    import contextlib
     for a, b in zip(want, train(cga, ts, dy, contextlib.nullcontext())):
         assert torch.equal(a, b)
     for hooks in (torch.autograd.graph.save_on_cpu(), torch.autograd.graph.save_on_cpu(pin_memory=True),
@@ -709,6 +711,7 @@ def test_checkpointed(cga, dtype, rows):
 
         def f(t):
             return t + cga.ops.gated_feed_forward(cga.ops.channel_norm(t, *leaves[1:3]), *leaves[3:])
+        gc.collect()                                    # what earlier tests left in cycles is not freed in between
         before = torch.cuda.memory_allocated()
         y = run(f, run(f, leaves[0]))
         kept = torch.cuda.memory_allocated() - before
